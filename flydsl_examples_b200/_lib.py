@@ -13,6 +13,7 @@ from pathlib import Path
 from . import build as _build
 
 DTYPE_FP32, DTYPE_BF16, DTYPE_FP16 = 1, 2, 3
+DTYPE_E4M3, DTYPE_E5M2 = 4, 5
 STATIC_SCRATCH_BYTES = 16 << 20  # B200_GEMM_STATIC_SCRATCH_BYTES
 COUNTER_BYTES = 1 << 20          # B200_GEMM_COUNTER_BYTES: ticket region at the start of a workspace
 
@@ -99,6 +100,42 @@ class Plan(C.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class Args8(C.Structure):
+    """b200_gemm_a8w8_args"""
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("a", "b", "a_scale", "b_scale", "out", "bias")]
+        + [(n, C.c_int64) for n in ("m", "n", "k", "lda", "ldb", "ldo", "sa_row", "sa_kb", "sb_col", "sb_kb")]
+        + [(n, C.c_int32) for n in ("a_trans", "b_trans", "a_dtype", "b_dtype", "a_block", "b_block", "out_dtype", "bias_dtype")]
+        + [("policy", Policy), ("status", C.c_void_p)]
+    )
+
+
+class QuantizeArgs(C.Structure):
+    """b200_gemm_quantize_args"""
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("ldx", C.c_int64),
+        ("in_dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("mode", C.c_int32),
+        ("reserved", C.c_int32),
+        ("q_row", C.c_void_p),
+        ("ldq_row", C.c_int64),
+        ("s_row", C.c_void_p),
+        ("sr_row", C.c_int64),
+        ("sr_group", C.c_int64),
+        ("q_col", C.c_void_p),
+        ("ldq_col", C.c_int64),
+        ("s_col", C.c_void_p),
+        ("sc_group", C.c_int64),
+        ("sc_col", C.c_int64),
+        ("colsum", C.c_void_p),
+        ("colsum_ld", C.c_int64),
+    ]
+
+
 class PeerHandle(C.Structure):
     """b200_peer_handle: plain bytes, safe to pickle with bytes(handle) and rebuild with from_buffer_copy."""
     _fields_ = [
@@ -120,6 +157,12 @@ EXPORTS = (
     "b200_gemm_workspace_bytes",
     "b200_gemm_num_variants",
     "b200_gemm_describe_variant",
+    "b200_gemm_a8w8",
+    "b200_gemm_a8w8_plan_query",
+    "b200_gemm_a8w8_prepare",
+    "b200_gemm_a8w8_launch",
+    "b200_gemm_a8w8_release",
+    "b200_gemm_quantize_a8",
     "b200_gemm_cast_bias",
     "b200_gemm_reduce_slots",
     "b200_peer_export",
@@ -175,6 +218,18 @@ def load() -> C.CDLL:
     lib.b200_gemm_describe_variant.argtypes = [C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.POINTER(C.c_int32),
                                                C.POINTER(C.c_int32)]
     lib.b200_gemm_describe_variant.restype = C.c_int
+    lib.b200_gemm_a8w8.argtypes = [C.POINTER(Args8), C.c_void_p]
+    lib.b200_gemm_a8w8.restype = C.c_int
+    lib.b200_gemm_a8w8_plan_query.argtypes = [C.POINTER(Args8), C.POINTER(Plan)]
+    lib.b200_gemm_a8w8_plan_query.restype = C.c_int
+    lib.b200_gemm_a8w8_prepare.argtypes = [C.POINTER(Args8), C.POINTER(C.c_void_p)]
+    lib.b200_gemm_a8w8_prepare.restype = C.c_int
+    lib.b200_gemm_a8w8_launch.argtypes = [C.c_void_p, C.c_void_p]
+    lib.b200_gemm_a8w8_launch.restype = C.c_int
+    lib.b200_gemm_a8w8_release.argtypes = [C.c_void_p]
+    lib.b200_gemm_a8w8_release.restype = None
+    lib.b200_gemm_quantize_a8.argtypes = [C.POINTER(QuantizeArgs), C.c_void_p]
+    lib.b200_gemm_quantize_a8.restype = C.c_int
     lib.b200_gemm_cast_bias.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
     lib.b200_gemm_cast_bias.restype = C.c_int
     lib.b200_gemm_reduce_slots.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,

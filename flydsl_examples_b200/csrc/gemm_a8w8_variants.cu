@@ -1,0 +1,34 @@
+// Instantiations of the 8-bit block-scaled GEMM kernel. Ring depths are the deepest that fit 227 KB of shared memory next to
+// the receive area of cluster split-K (single CTAs) or the store images (pairs); shallower rings were never faster.
+#include "gemm_a8w8_variants.h"
+
+namespace b200 {
+
+namespace {
+template <int TILE_Q, int STAGES, int CG>
+Variant8 make(int v_vector) {
+  Variant8 v;
+  v.tile_q = TILE_Q, v.cta_group = CG, v.stages = STAGES;
+  if (v_vector) {
+    v.fn = gemm_a8w8_sm100_kernel<TILE_Q, STAGES, CG, true>;
+    v.smem_bytes = Smem8<TILE_Q, STAGES, CG, true>::kDynBytes;
+  } else {
+    v.fn = gemm_a8w8_sm100_kernel<TILE_Q, STAGES, CG, false>;
+    v.smem_bytes = Smem8<TILE_Q, STAGES, CG, false>::kDynBytes;
+  }
+  static_assert(Smem8<TILE_Q, STAGES, CG, true>::kDynBytes <= 227 * 1024, "shared memory of a variant");
+  return v;
+}
+}  // namespace
+
+bool variant8(int tile_q, int cta_group, int v_vector, Variant8* out) {
+  if (cta_group == 1 && tile_q == 16) return *out = make<16, 10, 1>(v_vector), true;
+  if (cta_group == 1 && tile_q == 32) return *out = make<32, 9, 1>(v_vector), true;
+  if (cta_group == 1 && tile_q == 64) return *out = make<64, 7, 1>(v_vector), true;
+  if (cta_group == 1 && tile_q == 128) return *out = make<128, 4, 1>(v_vector), true;
+  if (cta_group == 2 && tile_q == 128) return *out = make<128, 7, 2>(v_vector), true;
+  if (cta_group == 2 && tile_q == 256) return *out = make<256, 5, 2>(v_vector), true;
+  return false;
+}
+
+}  // namespace b200

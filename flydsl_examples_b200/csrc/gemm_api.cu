@@ -10,19 +10,15 @@
 
 #include "../../include/b200_gemm.h"
 #include "aux_kernels.cuh"
+#include "host.h"
 #include "variants.h"
 
 namespace b200 {
 
-constexpr int kMaxDevices = 16;
 constexpr uint64_t kCounterBytes = 1u << 20;  // fixed ticket region at the start of the workspace (262144 tiles)
 
 // ------------------------------------------------------------------ driver entry point (no -lcuda link needed)
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn get_encode_fn() {
+EncodeTiledFn get_encode_fn() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
   std::call_once(once, []() {
@@ -339,7 +335,7 @@ static uint32_t make_idesc(int in_dtype, int u_mn, int v_mn, int mma_m, int mma_
          (uint32_t(mma_m >> 4) << 24);
 }
 
-static int set_cuda_error(cudaError_t e) {
+int set_cuda_error(cudaError_t e) {
   snprintf(g_last_cuda_error, sizeof(g_last_cuda_error), "%s", cudaGetErrorString(e));
   return B200_GEMM_ERR_LAUNCH;
 }

@@ -1,0 +1,21 @@
+// Host-side helpers shared by the translation units that export the C ABI.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+
+constexpr int kMaxDevices = 16;
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled, looked up once; null when the driver does not have it.
+EncodeTiledFn get_encode_fn();
+
+// Keeps the error's text for b200_gemm_strerror and returns B200_GEMM_ERR_LAUNCH.
+int set_cuda_error(cudaError_t e);
+
+}  // namespace b200

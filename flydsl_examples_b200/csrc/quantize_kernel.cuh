@@ -1,0 +1,275 @@
+// Quantization to 8-bit floating point with one power-of-two scale per group of 128, for sm_100a.
+//
+//   s = 2^ceil(log2(amax / MAX))  (amax: largest finite magnitude of the group; MAX = 448 or 57344, both 1.75 * 2^n; s = 1 for
+//   a group of zeros, never below 2^-126),  q = round_to_nearest_even(x / s)
+//
+// s is read off amax's exponent and mantissa (m * 2^e with 1 <= m < 2: s = 2^(e - n), doubled when m > 1.75), so x / s is an
+// exact product with a power of two and the conversion's is the only rounding. NaN becomes NaN; an infinity becomes NaN in
+// e4m3 and stays infinite in e5m2; neither touches its group's scale.
+//
+// Memory-bound: one pass. A block of 256 threads holds a 128 x 128 tile in registers (eight 16-byte loads of 16-bit values
+// in flight per thread, four blocks per SM), so the groups along rows (16 lanes: four shuffles), along columns and whole
+// blocks (one trip through shared memory) come from the same read, whichever of them are asked for.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+
+namespace b200 {
+
+constexpr int kQuantThreads = 256;
+
+struct QuantParams {
+  const void* x;
+  long long ldx;  // elements between rows of x (columns are contiguous)
+  int rows, cols;
+  int e5m2;
+  uint8_t* q_row;  // groups along a row (and 128 x 128 blocks, in block mode)
+  long long ldq_row;
+  float* s_row;
+  long long sr_row, sr_group;  // element strides of s_row: per row (per block of rows), per group
+  uint8_t* q_col;              // groups along a column
+  long long ldq_col;
+  float* s_col;
+  long long sc_group, sc_col;
+  float* colsum;  // optional: sums of the tile's columns, [tile row][cols_pitch]
+  long long colsum_ld;
+};
+
+// Exponent bits of the scale of a group with largest magnitude `amax` (finite, >= 0), in place in an fp32 word; 2^n * 1.75 is
+// the format's largest value.
+__device__ __forceinline__ uint32_t scale_bits(float amax, int n) {
+  const uint32_t bits = __float_as_uint(amax);
+  if (bits == 0) return 127u << 23;
+  int e = (int)(bits >> 23);
+  uint32_t man = bits & 0x7fffffu;
+  if (e == 0) return 1u << 23;  // an fp32 subnormal: the smallest scale
+  e += (man > 0x600000u) - n;   // mantissa above 1.75
+  return (uint32_t)(e < 1 ? 1 : e) << 23;
+}
+// 1 / s for a power of two s = 2^(b - 127), as fp32 bits; b is between 1 and 247, so the result is normal.
+__device__ __forceinline__ float inverse_of_scale(uint32_t bits) { return __uint_as_float((254u << 23) - bits); }
+
+__device__ __forceinline__ uint32_t pack_fp8x2(float lo, float hi, int e5m2) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+}
+
+template <typename T>
+struct RawRow;  // eight consecutive elements
+template <>
+struct RawRow<float> {
+  float v[8];
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+};
+template <>
+struct RawRow<__nv_bfloat16> {
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+};
+template <>
+struct RawRow<__half> {
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+    return i & 1 ? __high2float(h) : __low2float(h);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ RawRow<T> load_row8(const T* src, int n, bool vec) {
+  RawRow<T> r;
+  if (n >= 8 && vec) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+    if constexpr (sizeof(T) == 4) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(w[i]);
+    } else {
+      r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+    }
+  } else {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = i < n ? src[i] : 0.f;
+    } else {
+      const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        r.w[i] = (uint32_t)(2 * i < n ? s[2 * i] : 0) | ((uint32_t)(2 * i + 1 < n ? s[2 * i + 1] : 0) << 16);
+    }
+  }
+  return r;
+}
+
+// MODE: 1 = groups along rows, 2 = along columns, 4 = 128 x 128 blocks (written through the row members).
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantParams p) {
+  constexpr int kPasses = 8;  // rows per thread: ty, ty + 16, ...
+  __shared__ float red[8][128];
+  __shared__ float red2[8][128];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5;
+  const int tiles_c = (p.cols + 127) >> 7;
+  const int tr = blockIdx.x / tiles_c, tc = blockIdx.x - tr * tiles_c;
+  const int r0 = tr * 128, col = tc * 128 + tx * 8;
+  const int ncol = min(8, p.cols - col);  // may be <= 0
+  const int nrow = min(128, p.rows - r0);
+  const T* x = reinterpret_cast<const T*>(p.x);
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ((p.ldx * (long long)sizeof(T)) & 15) == 0;
+  const int n = p.e5m2 ? 15 : 8;
+
+  grid_dependency_wait();
+  grid_launch_dependents();
+  RawRow<T> v[kPasses];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = ty + 16 * i;
+    const bool in = r < nrow && ncol > 0;
+    v[i] = load_row8<T>(x + (in ? (long long)(r0 + r) * p.ldx + col : 0), in ? ncol : 0, vec);
+  }
+
+  // Magnitudes of finite values; a value that is not finite counts as zero and raises a flag.
+  bool odd = false;
+  auto mag = [&](float f) {
+    const float a = fabsf(f);
+    return a < __uint_as_float(0x7f800000u) ? a : 0.f;
+  };
+  float cmax[8], rmax[kPasses];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    rmax[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = v[i].get(j);
+      odd |= !(fabsf(f) < __uint_as_float(0x7f800000u));
+      const float a = mag(f);
+      if (MODE & 5) rmax[i] = fmaxf(rmax[i], a);
+      if (MODE & 2) cmax[j] = fmaxf(cmax[j], a);
+    }
+  }
+  // Eight values of one row times their inverse scales, converted and stored.
+  auto put = [&](uint8_t* dst, const RawRow<T>& raw, const float (&inv)[8], bool dvec) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = pack_fp8x2(raw.get(4 * h) * inv[4 * h], raw.get(4 * h + 1) * inv[4 * h + 1], p.e5m2);
+      const uint32_t hi = pack_fp8x2(raw.get(4 * h + 2) * inv[4 * h + 2], raw.get(4 * h + 3) * inv[4 * h + 3], p.e5m2);
+      w[h] = lo | (hi << 16);
+    }
+    if (odd) {  // the conversion clamps infinities to the largest value
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __float_as_uint(raw.get(j));
+        if ((b & 0x7fffffffu) == 0x7f800000u) {
+          const uint32_t code = p.e5m2 ? 0x7cu | ((b >> 24) & 0x80u) : 0x7fu;
+          w[j >> 2] = (w[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (code << (8 * (j & 3)));
+        }
+      }
+    }
+    if (dvec && ncol >= 8) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < ncol) dst[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+    }
+  };
+  const bool rvec = (reinterpret_cast<uintptr_t>(p.q_row) & 7) == 0 && (p.ldq_row & 7) == 0;
+  const bool cvec = (reinterpret_cast<uintptr_t>(p.q_col) & 7) == 0 && (p.ldq_col & 7) == 0;
+
+  if constexpr (MODE & 1) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
+      const int r = ty + 16 * i;
+      const uint32_t sb = scale_bits(rmax[i], n);
+      const float s = inverse_of_scale(sb);
+      const float inv[8] = {s, s, s, s, s, s, s, s};
+      if (r < nrow) {
+        if (ncol > 0) put(p.q_row + (long long)(r0 + r) * p.ldq_row + col, v[i], inv, rvec);
+        if (tx == 0) p.s_row[(long long)(r0 + r) * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+      }
+    }
+  }
+  if constexpr (MODE & 2) {
+    float csum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cmax[j] = fmaxf(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
+      csum[j] = 0.f;
+    }
+    if (p.colsum != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) csum[j] += v[i].get(j);
+        csum[j] += __shfl_xor_sync(0xffffffffu, csum[j], 16);
+      }
+    }
+    if ((threadIdx.x & 16) == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        red[warp][tx * 8 + j] = cmax[j];
+        if (p.colsum != nullptr) red2[warp][tx * 8 + j] = csum[j];
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float m = 0.f, t = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w][threadIdx.x]);
+      const uint32_t sb = scale_bits(m, n);
+      const int c = tc * 128 + threadIdx.x;
+      if (c < p.cols) {
+        p.s_col[(long long)tr * p.sc_group + (long long)c * p.sc_col] = __uint_as_float(sb);
+        if (p.colsum != nullptr) {
+#pragma unroll
+          for (int w = 0; w < 8; ++w) t += red2[w][threadIdx.x];
+          p.colsum[(long long)tr * p.colsum_ld + c] = t;
+        }
+      }
+      red[0][threadIdx.x] = inverse_of_scale(sb);
+    }
+    __syncthreads();
+    if (ncol > 0) {
+      float inv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) inv[j] = red[0][tx * 8 + j];
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = ty + 16 * i;
+        if (r < nrow) put(p.q_col + (long long)(r0 + r) * p.ldq_col + col, v[i], inv, cvec);
+      }
+    }
+  }
+  if constexpr (MODE & 4) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) m = fmaxf(m, rmax[i]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[0][warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w]);
+    const uint32_t sb = scale_bits(m, n);
+    if (threadIdx.x == 0) p.s_row[(long long)tr * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+    const float s = inverse_of_scale(sb);
+    const float inv[8] = {s, s, s, s, s, s, s, s};
+    if (ncol > 0) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = ty + 16 * i;
+        if (r < nrow) put(p.q_row + (long long)(r0 + r) * p.ldq_row + col, v[i], inv, rvec);
+      }
+    }
+  }
+}
+
+}  // namespace b200

@@ -1,0 +1,447 @@
+"""8-bit floating-point products with one scale for each block of 128: the operators next to `gemm_a16w16`.
+
+    q, s = quantize_a8(x, group="row")                     # values and power-of-two scales
+    c = gemm_a8w8(a, a_scale, b, b_scale, layout="nt")     # C[M, N] = A[M, K] @ B[K, N] (+ bias[N])
+    y = linear_a8w8(x, weight, bias)                       # a linear layer on the two, with its backward pass
+
+Operands are `torch.float8_e4m3fn` or `torch.float8_e5m2`, each its own. Products are exact, sums are fp32, the result is
+rounded once to `out_dtype`. Layout letters, `user_kwargs`, streams, `out` and errors follow `gemm_a16w16`; the kernels are in
+libb200_gemm.so (hand-written sm_100a CUDA), there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import threading
+from collections import OrderedDict
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .gemm_a16w16 import _num_sms, _workspace_for
+
+GROUP = 128
+_F8_ID = {torch.float8_e4m3fn: _lib.DTYPE_E4M3, torch.float8_e5m2: _lib.DTYPE_E5M2}
+_F_ID = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+_POLICY_KEYS = ("tile_n", "cta_group", "split_k", "group_m", "swap_ab", "max_ctas", "pdl", "wait_limit_us")
+
+
+def _blocks(n: int) -> int:
+    return -(-n // GROUP)
+
+
+# ------------------------------------------------------------------------------------------------------------ policy
+def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: bool, num_sms: int = 148) -> dict:
+    """Tile, split and operand order for a call without a tiling of its own.
+
+    Up to 64 rows of A the product streams the weights: B takes the 128-row side (swap_ab), the tokens fill a tile of 16 to
+    64 columns, and a cluster splits K until the CTAs fill the SMs. Above that the time of a call is taken as whole waves
+    times the cycles of a K block (the longer of the tensor time and the operands' way into the SM at 64 bytes a cycle),
+    and the cheapest of the tiles is used."""
+    kb = _blocks(k)
+    if m <= 64 and not a_transposed:
+        tile = 16 if m <= 16 else 32 if m <= 32 else 64
+        tiles = _blocks(n)
+        split = 1
+        while split < 16 and tiles * split * 2 <= num_sms and kb >= split * 4:
+            split *= 2
+        return {"tile_n": tile, "cta_group": 1, "swap_ab": True, "split_k": split}
+    best = None
+    for tile, cg in ((256, 2), (128, 2), (128, 1)):
+        if not b_transposed and tile // cg != 128:
+            continue  # a row-contiguous B arrives in boxes of 128 columns per CTA
+        tiles = -(-m // (128 * cg)) * -(-n // tile)
+        slots = num_sms // cg
+        cycles = max(tile * 2, (16384 + 128 * tile // cg) / 64)  # 128 x tile x 128 at 8192 products a cycle; bytes in
+        for split in (1, 2, 4, 8) if cg == 1 else (1,):
+            if split > 1 and (tiles * split > slots or kb < 4 * split):
+                continue
+            waves = -(-tiles * split // slots)
+            cost = waves * (-(-kb // split) * cycles + 1500 + (2000 if split > 1 else 0))
+            if best is None or cost < best[0]:
+                best = (cost, {"tile_n": tile, "cta_group": cg, "swap_ab": False, "split_k": split})
+    pol = best[1]
+    pol["group_m"] = 8 if m > 1024 else 0  # eight tile rows share the columns of B that L2 holds
+    return pol
+
+
+def _resolve(m, n, k, a_t, b_t, user_kwargs, num_sms) -> dict:
+    for key in user_kwargs:
+        if key not in _POLICY_KEYS:
+            raise ValueError(f"unknown gemm_a8w8 policy key {key!r}; expected some of {_POLICY_KEYS}")
+    if "tile_n" in user_kwargs:
+        pol = {"cta_group": 1, "swap_ab": False, "split_k": 1, "group_m": 0}
+    else:
+        pol = heuristic_a8w8(m, n, k, a_t, b_t, num_sms)
+        for key in ("cta_group", "split_k", "swap_ab"):
+            if key in user_kwargs:
+                raise ValueError(f"gemm_a8w8 policy key {key!r} needs 'tile_n' beside it")
+    pol.update(user_kwargs)
+    return pol
+
+
+# ----------------------------------------------------------------------------------------------------- prepared calls
+_PREPARED_MAX = 1024
+_prepared: "OrderedDict[tuple, tuple]" = OrderedDict()
+_prepared_lock = threading.Lock()
+
+
+def clear_prepared_calls() -> None:
+    """Drop every cached launch handle."""
+    with _prepared_lock:
+        items = list(_prepared.values())
+        _prepared.clear()
+    for handle, _, _ in items:
+        _lib.load().b200_gemm_a8w8_release(handle)
+
+
+def _describe(t: Optional[torch.Tensor]):
+    return None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype)
+
+
+def _launch_cached(key, stream_ptr) -> bool:
+    """Repeat of a call seen before. The lock is held over the launch: a handle is released only after it has left the table."""
+    with _prepared_lock:
+        ent = _prepared.get(key)
+        if ent is None:
+            return False
+        handle, dev, _ = ent
+        lib = _lib.load()
+        if torch.cuda.current_device() == dev:
+            rc = lib.b200_gemm_a8w8_launch(handle, stream_ptr)
+        else:
+            with torch.cuda.device(dev):
+                rc = lib.b200_gemm_a8w8_launch(handle, stream_ptr)
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_a8w8_launch failed ({rc}): {_lib.strerror(rc)}")
+    return True
+
+
+# -------------------------------------------------------------------------------------------------------------- GEMM
+def _check_operand(name: str, t: torch.Tensor, transposed: bool) -> int:
+    """Leading stride of an operand; raises unless the contiguous dimension has stride 1 and rows start on 16 bytes."""
+    rows, cols = t.shape
+    inner, lead = (t.stride(0), t.stride(1)) if transposed else (t.stride(1), t.stride(0))
+    n_inner, n_lead = (rows, cols) if transposed else (cols, rows)
+    if n_inner == 1:
+        inner = 1  # a stride of a size-1 dimension is arbitrary in torch
+    if n_lead == 1:
+        lead = max(-(-n_inner // 16) * 16, 16)
+    if inner != 1 or lead % 16 != 0 or lead < n_inner or t.data_ptr() % 16 != 0:
+        raise ValueError(
+            f"{name} does not satisfy the layout requirements for a {'column' if transposed else 'row'}-major input: expected "
+            f"stride({0 if transposed else 1}) == 1 and a 16-byte-aligned data pointer and leading stride; "
+            f"got shape={tuple(t.shape)} and stride={t.stride()}"
+        )
+    return lead
+
+
+def _check_scale(name: str, s: torch.Tensor, rows: int, kb: int, device) -> int:
+    """1 when the scale is one per 128 rows, 0 when one per row; s is [rows or blocks of rows, blocks of K]."""
+    if s.ndim != 2 or s.dtype != torch.float32 or s.shape[1] != kb or s.shape[0] not in (rows, _blocks(rows)):
+        raise ValueError(
+            f"{name} must be a float32 tensor with one scale per block of {GROUP} along K and per row or block of {GROUP} rows: "
+            f"expected {rows} or {_blocks(rows)} by {kb}, got {tuple(s.shape)} {s.dtype}"
+        )
+    if s.device != device:
+        raise ValueError(f"{name} is on {s.device}, the operands are on {device}")
+    return 0 if s.shape[0] == rows else 1
+
+
+def _fill_args(a, a_scale, b, b_scale, out, bias, a_t, b_t, pol) -> _lib.Args8:
+    m, k = a.shape
+    n = b.shape[1]
+    kb = _blocks(k)
+    args = _lib.Args8()
+    args.lda = _check_operand("A", a, a_t)
+    args.ldb = _check_operand("B", b, b_t)
+    args.a_block = _check_scale("a_scale", a_scale, m, kb, a.device)
+    args.b_block = _check_scale("b_scale (transposed)", b_scale.t(), n, kb, a.device)
+    args.a, args.b, args.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
+    args.a_scale, args.b_scale = a_scale.data_ptr(), b_scale.data_ptr()
+    args.bias = None if bias is None else bias.data_ptr()
+    args.m, args.n, args.k, args.ldo = m, n, k, n
+    args.sa_row, args.sa_kb = a_scale.stride()
+    args.sb_kb, args.sb_col = b_scale.stride()
+    args.a_trans, args.b_trans = int(a_t), int(b_t)
+    args.a_dtype, args.b_dtype = _F8_ID[a.dtype], _F8_ID[b.dtype]
+    args.out_dtype = _F_ID[out.dtype]
+    args.bias_dtype = 0 if bias is None else _F_ID[bias.dtype]
+    p = args.policy
+    p.tile_n, p.cta_group, p.split_k = pol["tile_n"], pol["cta_group"], pol["split_k"]
+    p.swap_ab, p.group_m = int(pol["swap_ab"]), pol.get("group_m", 0)
+    p.max_ctas, p.wait_limit_us = pol.get("max_ctas", 0), pol.get("wait_limit_us", 0)
+    p.no_pdl = 0 if pol.get("pdl", True) else 1
+    return args
+
+
+def _validate(a, a_scale, b, b_scale, layout):
+    layout = layout.lower()
+    if layout not in ("nn", "nt", "tn", "tt"):
+        raise ValueError(f"unsupported GEMM layout: {layout!r}; expected 'nn', 'nt', 'tn', or 'tt'")
+    assert a.ndim == 2 and b.ndim == 2
+    assert b.shape[0] == a.shape[1], f"A is {tuple(a.shape)}, B is {tuple(b.shape)}"
+    if a.dtype not in _F8_ID or b.dtype not in _F8_ID:
+        raise ValueError(f"gemm_a8w8 takes float8_e4m3fn or float8_e5m2 operands, got {a.dtype} and {b.dtype}")
+    assert a.device == b.device
+    assert b_scale.ndim == 2, f"b_scale has {b_scale.ndim} dimensions"
+    return layout[0] == "t", layout[1] == "t"
+
+
+def gemm_a8w8(
+    a: torch.Tensor,
+    a_scale: torch.Tensor,
+    b: torch.Tensor,
+    b_scale: torch.Tensor,
+    out: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    user_kwargs: dict = {},
+    stream: Optional[torch.cuda.Stream] = None,
+    layout: str = "nt",
+    out_dtype: Optional[torch.dtype] = None,
+) -> torch.Tensor:
+    """C[M, N] = A[M, K] @ B[K, N] (+ bias[N]) from 8-bit operands with scales, fp32 sums and one final rounding.
+
+    a [M, K], b [K, N]: logical shapes; `layout` says which dimension of each is contiguous ('n' row-major, 't' column-major), as
+    in `gemm_a16w16`. Bases and leading strides are multiples of 16 bytes (`quantize_a8` pads its outputs).
+    a_scale: float32 [M, ceil(K / 128)] or [ceil(M / 128), ceil(K / 128)]; b_scale: float32 [ceil(K / 128), N] or
+    [ceil(K / 128), ceil(N / 128)]; any strides. `out` may be any contiguous tensor of M * N elements; `out_dtype` (default:
+    out's, else bfloat16) and the bias are float32, bfloat16 or float16. Asynchronous on `stream`.
+
+    user_kwargs: tile_n (16, 32, 64, 128; with cta_group 2: 128, 256), cta_group, split_k (K blocks of a tile over the CTAs of a
+    cluster), swap_ab, group_m, max_ctas, pdl, wait_limit_us; without tile_n the tiling is chosen by `heuristic_a8w8`."""
+    key = None
+    if out is not None and a.is_cuda:
+        stream_ptr = (torch.cuda.current_stream(a.device) if stream is None else stream).cuda_stream
+        key = (_describe(a), _describe(a_scale), _describe(b), _describe(b_scale), _describe(out), _describe(bias),
+               tuple(sorted(user_kwargs.items())) if user_kwargs else (), stream_ptr, layout, out_dtype, a.get_device(),
+               a_scale.get_device(), b.get_device(), b_scale.get_device(), out.get_device())
+        if _launch_cached(key, stream_ptr):
+            return out.view(-1, b.shape[1])
+
+    a_t, b_t = _validate(a, a_scale, b, b_scale, layout)
+    m, k = a.shape
+    n = b.shape[1]
+    device = a.device
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if out is None else out.dtype
+    if out_dtype not in _F_ID:
+        raise ValueError(f"unsupported output dtype {out_dtype}; expected float32, bfloat16 or float16")
+    if bias is not None:
+        if bias.dtype not in _F_ID:
+            raise ValueError(f"unsupported bias dtype {bias.dtype}; expected float32, bfloat16 or float16")
+        assert bias.ndim == 1 and bias.shape[0] == n and bias.device == device
+    out_in, bias_in = out, bias
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=device)
+    else:
+        assert out.dtype == out_dtype
+        assert out.device == device
+        assert out.is_contiguous()
+        assert out.numel() == m * n, f"out has {out.numel()} elements, the product {m * n}"
+    out = out.view(m, n)
+    pol = _resolve(m, n, k, a_t, b_t, user_kwargs, _num_sms(device) if a.is_cuda else 148)
+    if m and n and k:
+        args = _fill_args(a, a_scale, b, b_scale, out, bias, a_t, b_t, pol)
+    assert a.is_cuda, "gemm_a8w8 runs on CUDA tensors only (there is no CPU path)"
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        with torch.cuda.stream(stream):
+            if bias is None:
+                out.zero_()
+            else:
+                out.copy_(bias.to(out.dtype).expand(m, n))
+        return out
+    args.status = _workspace_for(device, stream).status.data_ptr()
+    lib = _lib.load()
+    handle = C.c_void_p()
+    with torch.cuda.device(device):
+        rc = lib.b200_gemm_a8w8_prepare(C.byref(args), C.byref(handle))
+        if rc != 0:
+            raise RuntimeError(f"b200_gemm_a8w8_prepare failed ({rc}): {_lib.strerror(rc)}")
+        rc = lib.b200_gemm_a8w8_launch(handle, stream.cuda_stream)
+    if rc != 0:
+        lib.b200_gemm_a8w8_release(handle)
+        raise RuntimeError(f"b200_gemm_a8w8_launch failed ({rc}): {_lib.strerror(rc)}")
+    if key is not None and bias is bias_in and out_in is not None:
+        evicted = []
+        with _prepared_lock:
+            old = _prepared.pop(key, None)
+            if old is not None:
+                evicted.append(old)
+            _prepared[key] = (handle, a.get_device(), n)
+            while len(_prepared) > _PREPARED_MAX:
+                evicted.append(_prepared.popitem(last=False)[1])
+        for h, _, _ in evicted:
+            lib.b200_gemm_a8w8_release(h)
+    else:
+        lib.b200_gemm_a8w8_release(handle)
+    return out
+
+
+def plan(a, a_scale, b, b_scale, layout="nt", user_kwargs: dict = {}, out_dtype=torch.bfloat16) -> dict:
+    """What a call with these arguments would launch (tile, cluster split, grid, shared memory)."""
+    a_t, b_t = _validate(a, a_scale, b, b_scale, layout)
+    pol = _resolve(a.shape[0], b.shape[1], a.shape[1], a_t, b_t, user_kwargs, 148)
+    args = _fill_args(a, a_scale, b, b_scale, torch.empty(0, dtype=out_dtype), None, a_t, b_t, pol)
+    pl = _lib.Plan()
+    rc = _lib.load().b200_gemm_a8w8_plan_query(C.byref(args), C.byref(pl))
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_a8w8_plan_query failed ({rc}): {_lib.strerror(rc)}")
+    return pl.as_dict()
+
+
+# --------------------------------------------------------------------------------------------------------- quantizer
+def _pitched(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """[rows, cols] with rows that start on 16-byte boundaries."""
+    pitch = -(-cols // 16) * 16
+    buf = torch.empty((rows, pitch), dtype=dtype, device=device)
+    return buf if pitch == cols else buf[:, :cols]
+
+
+def _is_row_major(x: torch.Tensor) -> bool:
+    rows, cols = x.shape
+    return (cols <= 1 or x.stride(1) == 1) and (rows <= 1 or x.stride(0) >= cols)
+
+
+def _row_major(x: torch.Tensor) -> torch.Tensor:
+    return x if _is_row_major(x) else x.contiguous()
+
+
+_GROUPS = {"row": 1, "col": 2, "both": 3, "block": 4}
+
+
+def _quantize(x, group, dtype, stream, want_colsum=False):
+    if group not in _GROUPS:
+        raise ValueError(f"unknown group {group!r}; expected one of {tuple(_GROUPS)}")
+    if dtype not in _F8_ID:
+        raise ValueError(f"quantize_a8 makes float8_e4m3fn or float8_e5m2, not {dtype}")
+    if x.dtype not in _F_ID:
+        raise ValueError(f"quantize_a8 takes float32, bfloat16 or float16, not {x.dtype}")
+    assert x.ndim == 2, f"quantize_a8 takes a matrix, got {x.ndim} dimensions"
+    rows, cols = x.shape
+    if not _is_row_major(x):
+        raise ValueError(f"x must be row-major: expected stride(1) == 1; got shape={tuple(x.shape)} and stride={x.stride()}")
+    assert x.is_cuda, "quantize_a8 runs on CUDA tensors only (there is no CPU path)"
+    device = x.device
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    mode = _GROUPS[group]
+    args = _lib.QuantizeArgs()
+    args.x, args.rows, args.cols, args.ldx = x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols
+    args.in_dtype, args.out_dtype, args.mode = _F_ID[x.dtype], _F8_ID[dtype], mode
+    got = []
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        if mode != 2:
+            q = _pitched(rows, cols, dtype, device)
+            # the product reads the scales of 128 rows at a time: rows are the contiguous dimension
+            s = torch.empty((_blocks(cols), _blocks(rows) if mode == 4 else rows), dtype=torch.float32, device=device).t()
+            args.q_row, args.ldq_row, args.s_row = q.data_ptr(), max(q.stride(0), cols), s.data_ptr()
+            args.sr_row, args.sr_group = s.stride()
+            got += [q, s]
+        if mode in (2, 3):
+            q = _pitched(rows, cols, dtype, device)
+            s = torch.empty((_blocks(rows), cols), dtype=torch.float32, device=device)
+            args.q_col, args.ldq_col, args.s_col = q.data_ptr(), max(q.stride(0), cols), s.data_ptr()
+            args.sc_group, args.sc_col = s.stride()
+            got += [q, s]
+        if want_colsum:
+            sums = torch.empty((_blocks(rows), -(-cols // 4) * 4), dtype=torch.float32, device=device)
+            args.colsum, args.colsum_ld = sums.data_ptr(), sums.shape[1]
+            got.append(sums)
+        rc = _lib.load().b200_gemm_quantize_a8(C.byref(args), stream.cuda_stream)
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
+    return tuple(got)
+
+
+def quantize_a8(x: torch.Tensor, group: str = "row", dtype: torch.dtype = torch.float8_e4m3fn,
+                stream: Optional[torch.cuda.Stream] = None) -> tuple:
+    """8-bit values and scales of a row-major matrix x [R, C] (float32, bfloat16 or float16), in groups of 128.
+
+    group: "row" -> (q [R, C], s [R, ceil(C / 128)]), the operand of a product over C; "col" -> (q [R, C], s [ceil(R / 128), C]),
+    of one over R (used as `q.t()`, `s.t()`, or as B with `q`, `s`); "both" -> all four from one read of x; "block" ->
+    (q, s [ceil(R / 128), ceil(C / 128)]), a weight's, which serves products over either dimension.
+
+    A group's scale is the smallest power of two (at least 2^-126) that brings its largest finite magnitude to the format's
+    largest value or below; 1 for a group of zeros. q is x / s rounded to nearest even, the only rounding. NaN stays NaN; an
+    infinity becomes NaN in e4m3 and stays infinite in e5m2; neither changes its group's scale. Asynchronous on `stream`."""
+    return _quantize(x, group, dtype, stream)
+
+
+# ------------------------------------------------------------------------------------------------------ linear layer
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, grad_dtype):
+        x2 = _row_major(x.reshape(-1, x.shape[-1]))
+        need_dw = weight.requires_grad
+        f8 = torch.float8_e4m3fn
+        if need_dw:
+            xr, sxr, xc, sxc = _quantize(x2, "both", f8, None)
+        else:
+            xr, sxr = _quantize(x2, "row", f8, None)
+            xc = sxc = None
+        wq, sw = _quantize(_row_major(weight), "block", f8, None)
+        y = gemm_a8w8(xr, sxr, wq.t(), sw.t(), bias=bias, layout="nt", out_dtype=x.dtype)
+        ctx.save_for_backward(xc, sxc, wq if x.requires_grad else None, sw if x.requires_grad else None)
+        ctx.meta = (x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype, grad_dtype)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xc, sxc, wq, sw = ctx.saved_tensors
+        shape, x_dtype, w_dtype, b_dtype, f8 = ctx.meta
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        g = _row_major(dy.reshape(-1, dy.shape[-1]))  # an expanded gradient (of a sum) is spread out here
+        dx = dw = db = None
+        col = need_w or need_b
+        got = list(_quantize(g, "both" if need_x and col else "col" if col else "row", f8, None, want_colsum=need_b))
+        if need_x:
+            gr, sgr = got[:2]
+            got = got[2:]
+            dx = gemm_a8w8(gr, sgr, wq, sw, layout="nn", out_dtype=x_dtype).view(shape)
+        if need_w:
+            gc, sgc = got[:2]
+            dw = gemm_a8w8(gc.t(), sgc.t(), xc, sxc, layout="tn", out_dtype=w_dtype)
+        if need_b:
+            db = _sum_rows(got[-1], g.shape[1], b_dtype)
+        return dx, dw, db, None
+
+
+def _sum_rows(parts: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+    """Sum over the first dimension of fp32 [parts, pitch], in order, rounded once; the first n columns."""
+    pitch = parts.shape[1]
+    out = torch.empty(pitch, dtype=dtype, device=parts.device)
+    if parts.shape[0] == 0:
+        return out.zero_()[:n]
+    with torch.cuda.device(parts.device):
+        rc = _lib.load().b200_gemm_reduce_slots(parts.data_ptr(), pitch, parts.shape[0], out.data_ptr(), None, 1, pitch, _F_ID[dtype], 0,
+                                                torch.cuda.current_stream(parts.device).cuda_stream)
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_reduce_slots failed ({rc}): {_lib.strerror(rc)}")
+    return out[:n]
+
+
+def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                grad_dtype: torch.dtype = torch.float8_e4m3fn) -> torch.Tensor:
+    """y = x @ weight.T (+ bias) in 8-bit floating point, with its backward pass; x [..., K], weight [N, K], bias [N] of float32,
+    bfloat16 or float16, y in x's type.
+
+    Forward: x in groups of 128 along K, the weight in 128 x 128 blocks, both e4m3. Backward: the output's gradient is quantized
+    to `grad_dtype` once along N (for dx, against the weight as it was quantized) and once along the rows (for dweight, against x
+    quantized along the rows in the forward pass); dbias is the sum of the unquantized gradient in fp32, in a fixed order.
+    Gradients have their tensor's type."""
+    assert weight.ndim == 2 and x.ndim >= 1 and x.shape[-1] == weight.shape[1], f"x is {tuple(x.shape)}, weight {tuple(weight.shape)}"
+    assert x.is_cuda, "linear_a8w8 runs on CUDA tensors only (there is no CPU path)"
+    assert x.device == weight.device
+    if grad_dtype not in _F8_ID:
+        raise ValueError(f"grad_dtype must be float8_e4m3fn or float8_e5m2, not {grad_dtype}")
+    if bias is not None:
+        assert bias.shape == (weight.shape[0],) and bias.device == x.device
+    return _Linear8.apply(x, weight, bias, grad_dtype)

@@ -20,6 +20,9 @@ extern "C" {
 #define B200_GEMM_DTYPE_FP32 1
 #define B200_GEMM_DTYPE_BF16 2
 #define B200_GEMM_DTYPE_FP16 3
+/* 8-bit floating point, operands of b200_gemm_a8w8 and outputs of b200_gemm_quantize_a8 only */
+#define B200_GEMM_DTYPE_E4M3 4
+#define B200_GEMM_DTYPE_E5M2 5
 
 /* error codes */
 #define B200_GEMM_OK 0
@@ -240,6 +243,69 @@ int b200_gemm_selftest(void* cuda_stream, int32_t* failed_case);
  * usable. `status` is a device int32[4] that the caller zeroed. Takes the place of the unbounded flag spin of the
  * reference's split-K protocol (kernels/gemm_a16w16_gfx950_utils.py:216-247), which has no such exit. */
 int b200_gemm_wait_selftest(int32_t* status, uint32_t limit_us, void* cuda_stream);
+
+/* ---------------------------------------------------------------------------------------------------------------------
+ * 8-bit floating point with a scale for each block of 128.
+ *   C[m, n] = sum over K blocks b of 128: sa[m, b] * sb[b, n] * (sum over k in b of A[m, k] * B[k, n])  (+ bias[n])
+ * Products are exact and summed in fp32 on the tensor cores per block; the scaled sums are added in fp32; one rounding.
+ * A scale belongs to one row of A (column of B), or to 128 of them (a_block / b_block: rows m with m / 128 equal). K need not
+ * be a multiple of 128: the last block is shorter. Layouts as for b200_gemm_a16w16, so the forward product of a linear
+ * layer, its input gradient and its weight gradient are all this entry point. Operand bases and leading strides are
+ * multiples of 16 bytes (b200_gemm_quantize_a8's caller pads the pitch); anything else is refused. */
+typedef struct b200_gemm_a8w8_args {
+  const void* a;        /* A[0,0], 8-bit                                                                           */
+  const void* b;        /* B[0,0], 8-bit; B is logically [K,N]                                                      */
+  const float* a_scale; /* scale of (row m, K block b): a_scale[(a_block ? m / 128 : m) * sa_row + b * sa_kb]            */
+  const float* b_scale; /* scale of (column n, K block b): b_scale[(b_block ? n / 128 : n) * sb_col + b * sb_kb]         */
+  void* out;            /* C[0,0], row-major, row stride ldo elements                                                */
+  const void* bias;     /* bias[N], contiguous, of bias_dtype; NULL = none                                          */
+  int64_t m, n, k;
+  int64_t lda, ldb, ldo;              /* leading strides in elements, as for b200_gemm_args                              */
+  int64_t sa_row, sa_kb, sb_col, sb_kb; /* strides of the scales in elements                                               */
+  int32_t a_trans, b_trans;
+  int32_t a_dtype, b_dtype;     /* B200_GEMM_DTYPE_E4M3 or _E5M2, each operand its own                               */
+  int32_t a_block, b_block;     /* 1: a scale per 128 rows of A / columns of B, 0: one per row / column               */
+  int32_t out_dtype, bias_dtype; /* B200_GEMM_DTYPE_FP32, _BF16 or _FP16, in any combination                           */
+  b200_gemm_policy policy; /* tile_n 16, 32, 64, 128 (one CTA per 128 rows) or 128, 256 (cta_group 2); split_k > 1: the K blocks
+                              of a tile over that many CTAs of a cluster (a power of two up to 16; cta_group 1), summed
+                              in a fixed order through distributed shared memory; group_m, swap_ab, max_ctas, no_pdl,
+                              wait_limit_us as in the 16-bit GEMM; stages, tile_k, stream_k and loader must be 0. An operand
+                              on the MMA N axis that is not K-contiguous needs tile_n / cta_group == 128              */
+  int32_t* status;         /* as in b200_gemm_args                                                                  */
+} b200_gemm_a8w8_args;
+
+int b200_gemm_a8w8(const b200_gemm_a8w8_args* args, void* cuda_stream);
+/* What the call would launch (fields of the 16-bit GEMM that have no meaning here are 0); no workspace is needed. */
+int b200_gemm_a8w8_plan_query(const b200_gemm_a8w8_args* args, b200_gemm_plan* plan);
+/* Plan once, launch many times: as b200_gemm_prepare / launch / release. */
+typedef struct b200_gemm_a8w8_handle b200_gemm_a8w8_handle;
+int b200_gemm_a8w8_prepare(const b200_gemm_a8w8_args* args, b200_gemm_a8w8_handle** handle);
+int b200_gemm_a8w8_launch(const b200_gemm_a8w8_handle* handle, void* cuda_stream);
+void b200_gemm_a8w8_release(b200_gemm_a8w8_handle* handle);
+
+/* The quantizer that makes such operands: x[rows, cols] (fp32, bf16 or fp16; columns contiguous, row stride ldx) in groups of
+ * 128. The scale of a group is the smallest power of two, at least 2^-126, that brings its largest finite magnitude to the
+ * format's largest value (448 or 57344) or below, and 1 for a group of zeros; q = round_to_nearest_even(x / scale), the only
+ * rounding. NaN stays NaN; an infinity becomes NaN in e4m3 and stays infinite in e5m2; neither changes its group's scale. */
+typedef struct b200_gemm_quantize_args {
+  const void* x;
+  int64_t rows, cols, ldx;
+  int32_t in_dtype, out_dtype; /* FP32 / BF16 / FP16; E4M3 / E5M2                                                     */
+  int32_t mode;                /* 1: groups of 128 columns in a row; 2: of 128 rows in a column; 3: both, two outputs from one
+                                  read; 4: 128 x 128 blocks (written through q_row, s_row)                            */
+  int32_t reserved;
+  void* q_row;
+  int64_t ldq_row;
+  float* s_row; /* scale of (row r, or r / 128 in mode 4; group c / 128): s_row[r * sr_row + g * sr_group]                */
+  int64_t sr_row, sr_group;
+  void* q_col;
+  int64_t ldq_col;
+  float* s_col; /* scale of (group r / 128, column c): s_col[g * sc_group + c * sc_col]                                 */
+  int64_t sc_group, sc_col;
+  float* colsum; /* optional, modes 2 and 3: fp32 sums of x over each group of 128 rows, [group][colsum_ld]            */
+  int64_t colsum_ld;
+} b200_gemm_quantize_args;
+int b200_gemm_quantize_a8(const b200_gemm_quantize_args* args, void* cuda_stream);
 
 /* Text for an error code; for B200_GEMM_ERR_LAUNCH the last CUDA error string seen by this thread. */
 const char* b200_gemm_strerror(int code);

@@ -1,0 +1,381 @@
+"""The 8-bit block-scaled product, its quantizer and the linear layer against plain 64-bit forms.
+
+Bounds. An 8-bit product is exact in fp32. With S = sum |a| |b| times the scales, a K block's sum on the tensor core is off
+by a few units of 2^-23 of its S (four accumulating instructions; 8 units are allowed), each fp32 addition of the running
+sum and each product of scales adds at most 2^-24 of S: |error| <= (8 + blocks) * 2^-23 * S, plus half a step of the output type.
+"""
+import functools
+
+import pytest
+import torch
+
+from flydsl_examples_b200.gemm_a16w16 import check_status
+from flydsl_examples_b200.gemm_a8w8 import clear_prepared_calls, gemm_a8w8, linear_a8w8, plan, quantize_a8
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
+LARGEST = {E4: 448.0, E5: 57344.0}
+
+
+def blocks(n):
+    return -(-n // 128)
+
+
+def operand(g, rows, k, dtype, block, transposed, pad=0):
+    """[rows, k] 8-bit values, `transposed`: rows contiguous, with rows padded to 16 bytes + pad, and random scales. The padding
+    and everything around the matrix is NaN."""
+    r, c = (k, rows) if transposed else (rows, k)
+    pitch = -(-c // 16) * 16 + pad
+    buf = torch.full((r, pitch), 0x7F, dtype=torch.uint8, device=DEV)
+    vals = torch.randn(r, c, generator=g, device=DEV) * 2
+    buf[:, :c] = vals.to(dtype).view(torch.uint8)
+    q = buf.view(dtype)[:, :c]
+    q = q.t() if transposed else q
+    nb = blocks(rows) if block else rows
+    s = torch.rand(nb, blocks(k), generator=g, device=DEV) + 0.25
+    return q, s
+
+
+def values(q, s):
+    """64-bit values of an operand [rows, k]."""
+    rows, k = q.shape
+    wide = s.double().repeat_interleave(128, 1)[:, :k]
+    if s.shape[0] != rows:
+        wide = wide.repeat_interleave(128, 0)[:rows]
+    return q.float().double() * wide
+
+
+def check(got, a, sa, b, sb, bias=None):
+    """got against A @ B^T (+ bias); a [M, K], b [N, K]."""
+    va, vb = values(a, sa), values(b, sb)
+    ref, mag = va @ vb.t(), va.abs() @ vb.abs().t()
+    if bias is not None:
+        ref = ref + bias.double()
+        mag = mag + bias.double().abs()
+    bound = (8 + blocks(a.shape[1])) * 2.0 ** -23 * mag + torch.finfo(got.dtype).eps / 2 * ref.abs()
+    bound = bound * (1 + 1e-6) + (2.0 ** -25 if got.dtype == torch.float16 else 0)  # half a step among fp16 subnormals
+    bad = (got.double() - ref).abs() > bound
+    bad |= ~got.isfinite()
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), got[bad][:4].tolist(), ref[bad][:4].tolist())
+
+
+def run(m, n, k, layout="nt", ad=E4, bd=E4, a_block=False, b_block=True, out_dtype=torch.bfloat16, bias=False, kw={}, seed=0, pad=0,
+        repeats=1):
+    g = torch.Generator(device=DEV).manual_seed(seed + m + 7 * n + 13 * k)
+    a, sa = operand(g, m, k, ad, a_block, layout[0] == "t", pad)
+    b, sb = operand(g, n, k, bd, b_block, layout[1] == "n", pad)
+    bv = torch.randn(n, generator=g, device=DEV).to(torch.bfloat16) if bias else None
+    out = torch.full((m, n), float("nan"), dtype=out_dtype, device=DEV)
+    for _ in range(repeats):
+        got = gemm_a8w8(a, sa, b.t(), sb.t(), out, bias=bv, user_kwargs=kw, layout=layout)
+    check_status()
+    assert got.data_ptr() == out.data_ptr()
+    check(got, a, sa, b, sb, bv)
+    return got
+
+
+VARIANTS = [
+    {"tile_n": 128}, {"tile_n": 128, "cta_group": 2}, {"tile_n": 256, "cta_group": 2}, {"tile_n": 64}, {"tile_n": 32}, {"tile_n": 16},
+]
+
+
+@pytest.mark.parametrize("kw", VARIANTS, ids=str)
+@pytest.mark.parametrize("b_block", [True, False])
+def test_variants_small(kw, b_block):
+    run(200, 264, 328, kw=kw, b_block=b_block)
+
+
+@pytest.mark.parametrize("kw", VARIANTS, ids=str)
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16])
+def test_variants_outputs_and_bias(kw, out_dtype):
+    run(300, 520, 1000, kw=kw, out_dtype=out_dtype, bias=True)
+    run(300, 520, 1000, kw=kw, out_dtype=out_dtype, bias=True, a_block=True, b_block=False)
+
+
+@pytest.mark.parametrize("layout", ["nn", "nt", "tn", "tt"])
+@pytest.mark.parametrize("kw", [{"tile_n": 128}, {"tile_n": 256, "cta_group": 2}, {"tile_n": 128, "swap_ab": True}, {}], ids=str)
+@pytest.mark.parametrize("types", [(E4, E4), (E5, E4), (E4, E5), (E5, E5)], ids=["44", "54", "45", "55"])
+def test_layouts_and_types(layout, kw, types):
+    run(272, 400, 656, layout, *types, a_block=False, b_block=False, kw=kw, pad=32)
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("split", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("swap", [True, False])
+def test_cluster_split(tile, split, swap):
+    # 17 K blocks: uneven slices; ragged against every tile
+    m, n = (tile - 3, 390) if swap else (390, tile * 2 - 3)
+    kw = {"tile_n": tile, "split_k": split, "swap_ab": swap}
+    x = run(m, n, 2100, kw=kw, out_dtype=torch.float32, bias=True, b_block=swap, repeats=3)
+    y = run(m, n, 2100, kw=kw, out_dtype=torch.float32, bias=True, b_block=swap)
+    assert torch.equal(x, y)  # summed in a fixed order
+
+
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 33, 64, 65, 127, 129, 255, 513])
+@pytest.mark.parametrize("n,k", [(128, 128), (130, 4096), (1000, 16), (7, 1), (2050, 129)])
+def test_default_policy_odd_sizes(m, n, k):
+    run(m, n, k)
+    run(m, n, k, b_block=False, a_block=True, out_dtype=torch.float32, bias=True)
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 4096), (1000, 3000, 4100), (4096, 2304, 1152), (20000, 130, 260), (130, 20000, 260)])
+@pytest.mark.parametrize("layout", ["nt", "nn", "tn"])
+def test_ordinary_sizes(m, n, k, layout):
+    run(m, n, k, layout, b_block=layout != "tn", repeats=2)
+
+
+def test_unaligned_output_rows_and_storage_offset():
+    # an odd N leaves C's rows off 16-byte boundaries: no TMA stores
+    for kw in ({"tile_n": 256, "cta_group": 2}, {"tile_n": 128}, {}):
+        run(300, 517, 400, kw=kw, bias=True)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    a, sa = operand(g, 70, 300, E4, False, False)
+    b, sb = operand(g, 90, 300, E4, True, False)
+    flat = torch.full((70 * 90 + 9,), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = gemm_a8w8(a, sa, b.t(), sb.t(), flat[3:-6])
+    check(got.view(70, 90), a, sa, b, sb)
+    assert (flat[:3] == 7).all() and (flat[-6:] == 7).all()
+
+
+def test_scale_strides_and_extremes():
+    g = torch.Generator(device=DEV).manual_seed(6)
+    m, n, k = 260, 300, 520
+    a, sa = operand(g, m, k, E4, False, False)
+    b, sb = operand(g, n, k, E4, True, False)
+    want = gemm_a8w8(a, sa, b.t(), sb.t(), out_dtype=torch.float32)
+    wide = torch.full((m * 2, blocks(k) * 3), float("nan"), device=DEV)
+    wide[::2, ::3] = sa
+    assert torch.equal(want, gemm_a8w8(a, wide[::2, ::3], b.t(), sb.t(), out_dtype=torch.float32))
+    assert torch.equal(want, gemm_a8w8(a, sa.t().contiguous().t(), b.t(), sb.t().contiguous(), out_dtype=torch.float32))
+    # one scale for everything: a broadcast tensor of strides 0
+    one = torch.full((1, 1), 0.5, device=DEV)
+    got = gemm_a8w8(a, one.expand(m, blocks(k)), b.t(), one.expand(blocks(k), blocks(n)), out_dtype=torch.float32)
+    check(got, a, one.expand(m, blocks(k)), b, one.expand(blocks(n), blocks(k)))
+    # scales at the ends of fp32: the two of a block are multiplied in fp32 and stay finite here
+    check(gemm_a8w8(a, sa * 2.0 ** 60, b.t(), sb.t() * 2.0 ** -60, out_dtype=torch.float32), a, sa * 2.0 ** 60, b, sb * 2.0 ** -60)
+
+
+def test_nan_stays_in_its_row_and_column():
+    g = torch.Generator(device=DEV).manual_seed(7)
+    for kw in ({"tile_n": 128}, {"tile_n": 256, "cta_group": 2}, {"tile_n": 64, "swap_ab": True, "split_k": 2}):
+        a, sa = operand(g, 140, 300, E4, False, False)
+        b, sb = operand(g, 150, 300, E4, True, False)
+        a.view(torch.uint8)[5, 299] = 0x7F
+        b.view(torch.uint8)[149, 0] = 0xFF
+        got = gemm_a8w8(a, sa, b.t(), sb.t(), user_kwargs=kw, out_dtype=torch.float32)
+        bad = got.isnan()
+        assert bad[5].all() and bad[:, 149].all() and int(bad.sum()) == 140 + 150 - 1
+
+
+def test_other_stream_graph_and_two_callers():
+    g = torch.Generator(device=DEV).manual_seed(8)
+    a, sa = operand(g, 33, 1024, E4, False, False)
+    b, sb = operand(g, 640, 1024, E4, True, False)
+    want = gemm_a8w8(a, sa, b.t(), sb.t())
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    got = gemm_a8w8(a, sa, b.t(), sb.t(), stream=s)
+    s.synchronize()
+    assert torch.equal(want, got)
+    # captured and replayed on changed inputs
+    out = torch.empty_like(want)
+    gemm_a8w8(a, sa, b.t(), sb.t(), out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, qs = quantize_a8(want, "row")
+        gemm_a8w8(a, sa, b.t(), sb.t(), out)
+    a.view(torch.uint8).copy_(a.view(torch.uint8).flip(0).contiguous())
+    sa.copy_(sa.flip(0).contiguous())
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want.flip(0))
+    # two streams at once
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(want) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, o in zip(streams, outs):
+            with torch.cuda.stream(st):
+                gemm_a8w8(a, sa, b.t(), sb.t(), o)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], want.flip(0))
+    check_status()
+    clear_prepared_calls()
+
+
+# --------------------------------------------------------------------------------------------------------- quantizer
+def groups64(x, rg, cg, dtype):
+    """Scales by comparison and exact quotients in fp64; torch's conversion of the exact fp32 quotient."""
+    big = LARGEST[dtype]
+    r, c = x.shape
+    v = torch.where(x.isfinite(), x, torch.zeros_like(x)).double().abs()
+    v = torch.nn.functional.pad(v, (0, -c % cg, 0, -r % rg)).view(-(-r // rg), rg, -(-c // cg), cg).amax((1, 3))
+    e = torch.full_like(v, -126.0)
+    for p in range(-126, 128):  # smallest power of two that suffices
+        e = torch.where(v / 2.0 ** (p - 1) > big, torch.full_like(e, float(p)), e) if p > -126 else e
+    s = torch.where(v > 0, torch.exp2(e), torch.ones_like(v))
+    wide = s.repeat_interleave(rg, 0)[:r].repeat_interleave(cg, 1)[:, :c]
+    return (x.double() / wide).float().to(dtype), s.float()
+
+
+def same8(q, want):
+    nan = q.float().isnan()
+    return torch.equal(nan, want.float().isnan()) and torch.equal(q.float()[~nan], want.float()[~nan])
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (3, 130), (128, 128), (129, 257), (32, 7168), (300, 1000), (1000, 72)])
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dtype", [E4, E5])
+def test_quantize(rows, cols, x_dtype, dtype):
+    g = torch.Generator(device=DEV).manual_seed(rows * 1000 + cols)
+    x = (torch.randn(rows, cols, generator=g, device=DEV) * torch.exp2(torch.randint(-12, 13, (rows, cols), generator=g, device=DEV))).to(x_dtype)
+    for group, sizes in (("row", [(1, 128)]), ("col", [(128, 1)]), ("both", [(1, 128), (128, 1)]), ("block", [(128, 128)])):
+        got = quantize_a8(x, group, dtype)
+        for i, (rg, cg) in enumerate(sizes):
+            q, s = groups64(x, rg, cg, dtype)
+            assert got[2 * i].dtype == dtype and same8(got[2 * i], q), group
+            assert torch.equal(got[2 * i + 1], s), group
+
+
+@pytest.mark.parametrize("dtype", [E4, E5])
+def test_quantize_borders_and_specials(dtype):
+    x = torch.zeros(256, 256, device=DEV)
+    x[1, :] = torch.tensor([448.0, 448.00003, 447.9, 57344.0, 57344.004, 1e-38, 1e-45, 3e38] * 32, device=DEV)
+    x[2, 3], x[2, 4], x[2, 5], x[2, 6] = float("inf"), float("-inf"), float("nan"), 3.0
+    x[3, :128] = 2.0 ** -120
+    x[4, :128] = 1.1754944e-38  # smallest normal
+    x[5, :128] = 1e-45          # smallest subnormal
+    x[6, :] = float("nan")
+    x[7, 0], x[7, 1:9] = 448.0, torch.tensor([8.5, 9.5, 0.0009765625, 0.0029296875, -8.5, 17.0, 19.0, 2.0 ** -10], device=DEV)  # ties
+    for group, (rg, cg) in (("row", (1, 128)), ("col", (128, 1)), ("block", (128, 128))):
+        q, s = groups64(x, rg, cg, dtype)
+        got, gs = quantize_a8(x, group, dtype)
+        assert torch.equal(gs, s) and same8(got, q)
+
+
+def test_quantize_strides_offsets_and_neighbours():
+    g = torch.Generator(device=DEV).manual_seed(9)
+    big = torch.randn(140, 701, generator=g, device=DEV).to(torch.bfloat16)
+    for x in (big[3:133, 5:330], big[:, 1:], big[::2, 8:264], big[:1, :5], big[7:8].expand(1, 701)):
+        for group in ("row", "col", "block"):
+            got, want = quantize_a8(x, group), quantize_a8(x.contiguous(), group)
+            assert same8(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_quantize_feeds_the_product():
+    g = torch.Generator(device=DEV).manual_seed(10)
+    x = torch.randn(77, 500, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randn(333, 500, generator=g, device=DEV).to(torch.bfloat16)
+    dy = torch.randn(77, 333, generator=g, device=DEV).to(torch.bfloat16)
+    xr, sxr, xc, sxc = quantize_a8(x, "both")
+    wq, sw = quantize_a8(w, "block")
+    gr, sgr, gc, sgc = quantize_a8(dy, "both", E5)
+    check(gemm_a8w8(xr, sxr, wq.t(), sw.t(), out_dtype=torch.float32), xr, sxr, wq, sw)
+    check(gemm_a8w8(gr, sgr, wq, sw, layout="nn", out_dtype=torch.float32), gr, sgr, wq.t(), sw.t())
+    check(gemm_a8w8(gc.t(), sgc.t(), xc, sxc, layout="tn", out_dtype=torch.float32), gc.t(), sgc.t(), xc.t(), sxc.t())
+
+
+# ------------------------------------------------------------------------------------------------------ linear layer
+def reference_linear(x, w, b, dy, grad_dtype):
+    """(value, magnitude, blocks) of y, dx, dw in fp64 by the definition."""
+    def val(t, rg, cg, dtype):
+        q, s = groups64(t.float(), rg, cg, dtype)
+        return q.float().double() * s.double().repeat_interleave(rg, 0)[: t.shape[0]].repeat_interleave(cg, 1)[:, : t.shape[1]]
+    wq = val(w, 128, 128, E4)
+    pairs = ((val(x, 1, 128, E4), wq.t()), (val(dy, 1, 128, grad_dtype), wq), (val(dy, 128, 1, grad_dtype).t(), val(x, 128, 1, E4)))
+    got = [(p @ q, p.abs() @ q.abs(), blocks(p.shape[1])) for p, q in pairs]
+    if b is not None:
+        got[0] = (got[0][0] + b.double(), got[0][1] + b.double().abs(), got[0][2])
+    return got
+
+
+def near(got, ref):
+    want, mag, nb = ref
+    eps = torch.finfo(got.dtype).eps / 2
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 0
+    return bool(((got.double() - want).abs() <= (8 + nb) * 2.0 ** -23 * mag + eps * 1.000001 * want.abs() + tiny).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 8, 16), (100, 72, 200), (300, 513, 260), (512, 384, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("grad_dtype", [E4, E5])
+def test_linear_and_its_gradients(m, n, k, dtype, grad_dtype):
+    g = torch.Generator(device=DEV).manual_seed(m + n + k)
+    x = torch.randn(m, k, generator=g, device=DEV).to(dtype).requires_grad_()
+    w = (torch.randn(n, k, generator=g, device=DEV) / k ** 0.5).to(dtype).requires_grad_()
+    b = torch.randn(n, generator=g, device=DEV).to(dtype).requires_grad_()
+    dy = torch.randn(m, n, generator=g, device=DEV).to(dtype)
+    y = linear_a8w8(x, w, b, grad_dtype)
+    y.backward(dy)
+    ref = reference_linear(x.detach(), w.detach(), b.detach(), dy, grad_dtype)
+    assert y.dtype == x.grad.dtype == w.grad.dtype == b.grad.dtype == dtype
+    for got, want in zip((y.detach(), x.grad, w.grad), ref):
+        assert near(got, want)
+    want, mag = dy.double().sum(0), dy.double().abs().sum(0)
+    assert ((b.grad.double() - want).abs() <= (m + 1) * 2.0 ** -24 * mag + torch.finfo(dtype).eps / 2 * 1.000001 * want.abs()).all()
+    check_status()
+
+
+def test_linear_gradient_against_differences():
+    # quantization is piecewise constant, so differences are taken on operands that 8 bits hold exactly: small integers whose
+    # groups all have the same scale; the layer is then the exact bilinear product
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randint(-4, 5, (6, 256), generator=g, device=DEV).float()
+    w = torch.randint(-4, 5, (5, 256), generator=g, device=DEV).float()
+    x[:, ::128], w[:, ::128] = 7.0, 7.0
+    dy = torch.randint(-2, 3, (6, 5), generator=g, device=DEV).float()
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    linear_a8w8(xl, wl).backward(dy)
+    loss = lambda x_, w_: (linear_a8w8(x_, w_) * dy).sum().item()  # noqa: E731
+    for i, j in ((0, 1), (3, 77), (5, 255)):
+        up, down = x.clone(), x.clone()
+        up[i, j] += 1
+        down[i, j] -= 1
+        assert (loss(up, w) - loss(down, w)) / 2 == xl.grad[i, j].item()
+    for i, j in ((0, 1), (4, 200)):
+        up, down = w.clone(), w.clone()
+        up[i, j] += 1
+        down[i, j] -= 1
+        assert (loss(x, up) - loss(x, down)) / 2 == wl.grad[i, j].item()
+
+
+def test_linear_partial_gradients_shapes_and_broadcast_gradient():
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(2, 3, 160, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randn(96, 160, generator=g, device=DEV).to(torch.bfloat16)
+    b = torch.randn(96, generator=g, device=DEV).to(torch.bfloat16)
+    dy = torch.ones(1, 1, 1, device=DEV, dtype=torch.bfloat16).expand(2, 3, 96)
+    full = None
+    for need in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1)):
+        leaves = [t.clone().requires_grad_(bool(f)) for t, f in zip((x, w, b), need)]
+        y = linear_a8w8(*leaves)
+        assert y.shape == (2, 3, 96)
+        y.backward(dy)
+        got = [t.grad for t in leaves]
+        full = full or got
+        for f, a_, b_ in zip(need, got, full):
+            assert (a_ is None) if not f else torch.equal(a_, b_)
+    with torch.no_grad():
+        assert linear_a8w8(x[:0], w, b).shape == (0, 3, 96)
+    leaves = [t.clone().requires_grad_() for t in (x[:0], w, b)]
+    linear_a8w8(*leaves).sum().backward()
+    assert leaves[0].grad.shape == (0, 3, 160) and not leaves[1].grad.any() and not leaves[2].grad.any()
+    xt = x.view(6, 160).t().contiguous().t()  # column-major input
+    assert torch.equal(linear_a8w8(xt, w, b), linear_a8w8(x.view(6, 160), w, b))
+
+
+def test_no_offset_over_32_bits_wraps():
+    # 2^31 bytes of output: the last rows lie past a signed 32-bit offset
+    m, n, k = 270000, 4096, 128
+    g = torch.Generator(device=DEV).manual_seed(11)
+    a, sa = operand(g, m, k, E4, False, False)
+    b, sb = operand(g, n, k, E4, True, False)
+    got = gemm_a8w8(a, sa, b.t(), sb.t())
+    for lo in (0, 131000, m - 300):
+        check(got[lo:lo + 300], a[lo:lo + 300], sa[lo:lo + 300], b, sb)
+    q, s = quantize_a8(got, "both")[:2]
+    q2, s2 = quantize_a8(got[m - 256:].contiguous(), "row")
+    assert same8(q[m - 256:], q2) and torch.equal(s[m - 256:], s2)
