@@ -136,6 +136,17 @@ class QuantizeArgs(C.Structure):
     ]
 
 
+class MoeArgs(C.Structure):
+    """b200_gemm_moe_args"""
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("x", "logits", "w13", "w2", "out")]
+        + [(n, C.c_int64) for n in ("tokens", "hidden", "inner", "experts", "ldx", "logits_row", "logits_col", "w13_expert", "w13_row",
+                                    "w2_expert", "w2_row", "ldo")]
+        + [(n, C.c_int32) for n in ("top_k", "renormalize", "dtype", "logits_dtype", "wait_limit_us", "no_pdl")]
+        + [("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("status", C.c_void_p)]
+    )
+
+
 class PeerHandle(C.Structure):
     """b200_peer_handle: plain bytes, safe to pickle with bytes(handle) and rebuild with from_buffer_copy."""
     _fields_ = [
@@ -163,6 +174,11 @@ EXPORTS = (
     "b200_gemm_a8w8_launch",
     "b200_gemm_a8w8_release",
     "b200_gemm_quantize_a8",
+    "b200_gemm_moe_a16w16",
+    "b200_gemm_moe_workspace_bytes",
+    "b200_gemm_moe_prepare",
+    "b200_gemm_moe_launch",
+    "b200_gemm_moe_release",
     "b200_gemm_cast_bias",
     "b200_gemm_reduce_slots",
     "b200_peer_export",
@@ -230,6 +246,16 @@ def load() -> C.CDLL:
     lib.b200_gemm_a8w8_release.restype = None
     lib.b200_gemm_quantize_a8.argtypes = [C.POINTER(QuantizeArgs), C.c_void_p]
     lib.b200_gemm_quantize_a8.restype = C.c_int
+    lib.b200_gemm_moe_a16w16.argtypes = [C.POINTER(MoeArgs), C.c_void_p]
+    lib.b200_gemm_moe_a16w16.restype = C.c_int
+    lib.b200_gemm_moe_workspace_bytes.argtypes = [C.POINTER(MoeArgs)]
+    lib.b200_gemm_moe_workspace_bytes.restype = C.c_uint64
+    lib.b200_gemm_moe_prepare.argtypes = [C.POINTER(MoeArgs), C.POINTER(C.c_void_p)]
+    lib.b200_gemm_moe_prepare.restype = C.c_int
+    lib.b200_gemm_moe_launch.argtypes = [C.c_void_p, C.c_void_p]
+    lib.b200_gemm_moe_launch.restype = C.c_int
+    lib.b200_gemm_moe_release.argtypes = [C.c_void_p]
+    lib.b200_gemm_moe_release.restype = None
     lib.b200_gemm_cast_bias.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
     lib.b200_gemm_cast_bias.restype = C.c_int
     lib.b200_gemm_reduce_slots.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,

@@ -21,9 +21,9 @@ LIB_PATH = PKG_DIR / "libb200_gemm.so"
 STAMP_PATH = PKG_DIR / "libb200_gemm.so.stamp"
 
 SOURCES = [CSRC / name for name in ("gemm_api.cu", "variants_single_k128.cu", "variants_single_k64.cu", "variants_pair.cu",
-                                    "variants_loader.cu", "gemm_a8w8_api.cu", "gemm_a8w8_variants.cu")]
+                                    "variants_loader.cu", "gemm_a8w8_api.cu", "gemm_a8w8_variants.cu", "moe_api.cu")]
 HEADERS = [CSRC / "gemm_kernel.cuh", CSRC / "aux_kernels.cuh", CSRC / "variants.h", CSRC / "ptx.cuh", CSRC / "host.h",
-           CSRC / "gemm_a8w8_kernel.cuh", CSRC / "gemm_a8w8_variants.h", CSRC / "quantize_kernel.cuh", INCLUDE / "b200_gemm.h"]
+           CSRC / "gemm_a8w8_kernel.cuh", CSRC / "gemm_a8w8_variants.h", CSRC / "quantize_kernel.cuh", CSRC / "moe_kernels.cuh", INCLUDE / "b200_gemm.h"]
 OBJ_DIR = PKG_DIR / "_obj"  # object files of the translation units (not shipped, not tracked)
 
 NVCC_FLAGS = [

@@ -1,0 +1,189 @@
+// Host side of the few-token mixture-of-experts layer (b200_gemm_moe_* in include/b200_gemm.h): validation, tensor maps, the two
+// launches. No device allocation, no synchronisation.
+#include <cstring>
+#include <new>
+
+#include "../../include/b200_gemm.h"
+#include "host.h"
+#include "moe_kernels.cuh"
+
+namespace b200 {
+
+// Ring depths: as many 128-deep stages as fit 227 KB next to the exchange area.
+struct MoeVariant {
+  MoeFn up, down;
+  int up_smem, down_smem, cols;
+};
+template <int TN, int STAGES>
+static MoeVariant moe_make() {
+  static_assert(SmemMoe<TN, STAGES, true>::kDynBytes <= 227 * 1024 && SmemMoe<TN, STAGES, false>::kDynBytes <= 227 * 1024, "shared memory");
+  return {moe_a16w16_sm100_kernel<TN, STAGES, true>, moe_a16w16_sm100_kernel<TN, STAGES, false>, SmemMoe<TN, STAGES, true>::kDynBytes,
+          SmemMoe<TN, STAGES, false>::kDynBytes, TN};
+}
+static MoeVariant moe_variant(int64_t t) { return t <= 16 ? moe_make<16, 5>() : t <= 32 ? moe_make<32, 5>() : moe_make<64, 4>(); }
+
+constexpr uint64_t kMoeListBytes = 4096;  // the list of chosen experts at the start of the scratch
+
+static int moe_check(const b200_gemm_moe_args* a) {
+  if (a == nullptr || a->tokens <= 0 || a->hidden <= 0 || a->inner <= 0 || a->experts <= 0) return B200_GEMM_ERR_BAD_ARG;
+  if (a->tokens > kMoeMaxTokens || a->experts > kMoeMaxExperts || a->hidden > (1 << 24) || a->inner > (1 << 24)) return B200_GEMM_ERR_TOO_LARGE;
+  if (a->top_k < 1 || a->top_k > kMoeMaxTopK || a->top_k > a->experts) return B200_GEMM_ERR_BAD_ARG;
+  if (a->dtype != B200_GEMM_DTYPE_BF16 && a->dtype != B200_GEMM_DTYPE_FP16) return B200_GEMM_ERR_BAD_ARG;
+  if (a->logits_dtype < 1 || a->logits_dtype > 3) return B200_GEMM_ERR_BAD_ARG;
+  // TMA describes all operands: rows of whole 16-byte pieces
+  if (a->hidden % 8 != 0 || a->inner % 8 != 0) return B200_GEMM_ERR_BAD_ARG;
+  if (a->ldx < a->hidden || a->w13_row < a->hidden || a->w2_row < a->inner || a->ldo < a->hidden) return B200_GEMM_ERR_BAD_ARG;
+  if (a->ldx % 8 != 0 || a->w13_row % 8 != 0 || a->w13_expert % 8 != 0 || a->w2_row % 8 != 0 || a->w2_expert % 8 != 0) return B200_GEMM_ERR_BAD_ARG;
+  if (a->experts > 1 && (a->w13_expert < 2 * a->inner * a->w13_row - (a->w13_row - a->hidden) ||
+                         a->w2_expert < a->hidden * a->w2_row - (a->w2_row - a->inner)))
+    return B200_GEMM_ERR_BAD_ARG;
+  return 0;
+}
+
+static int64_t moe_slots(const b200_gemm_moe_args* a) {
+  const int64_t pairs = a->tokens * a->top_k;
+  return pairs < a->experts ? pairs : a->experts;
+}
+
+static int encode3(CUtensorMap* map, int dtype, const void* ptr, int64_t d0, int64_t d1, int64_t d2, int64_t s1, int64_t s2, int box1) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return B200_GEMM_ERR_DRIVER;
+  cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+  cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box1, 1}, estr[3] = {1, 1, 1};
+  const CUresult res = enc(map, dtype == B200_GEMM_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           d2 > 0 ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return res == CUDA_SUCCESS ? 0 : B200_GEMM_ERR_TENSOR_MAP;
+}
+
+}  // namespace b200
+
+struct b200_gemm_moe_handle {
+  b200::MoeParams up, down;
+  b200::MoeVariant var;
+  int grid_up, grid_down, pdl;
+};
+
+namespace b200 {
+
+static int moe_prepare(const b200_gemm_moe_args* a, b200_gemm_moe_handle* h) {
+  int rc = moe_check(a);
+  if (rc) return rc;
+  if (a->x == nullptr || a->logits == nullptr || a->w13 == nullptr || a->w2 == nullptr || a->out == nullptr) return B200_GEMM_ERR_BAD_ARG;
+  auto off = [](const void* ptr, uintptr_t to) { return (reinterpret_cast<uintptr_t>(ptr) % to) != 0; };
+  if (off(a->x, 16) || off(a->w13, 16) || off(a->w2, 16) || off(a->out, 2) || off(a->logits, a->logits_dtype == 1 ? 4 : 2))
+    return B200_GEMM_ERR_BAD_ARG;
+  if (a->workspace == nullptr || off(a->workspace, 256) || a->workspace_bytes < b200_gemm_moe_workspace_bytes(a)) return B200_GEMM_ERR_WORKSPACE;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return B200_GEMM_ERR_LAUNCH;
+  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return set_cuda_error(e);
+
+  memset(h, 0, sizeof(*h));
+  h->var = moe_variant(a->tokens);
+  const int cols = h->var.cols;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  MoeParams& u = h->up;
+  u.logits = a->logits, u.logits_row = a->logits_row, u.logits_col = a->logits_col, u.logits_dtype = a->logits_dtype;
+  u.T = (int)a->tokens, u.E = (int)a->experts, u.H = (int)a->hidden, u.I = (int)a->inner, u.top_k = a->top_k, u.renorm = a->renormalize ? 1 : 0;
+  u.dtype = a->dtype;
+  u.active = reinterpret_cast<int*>(ws);
+  u.h = reinterpret_cast<uint16_t*>(ws + kMoeListBytes);
+  u.out = a->out, u.ldo = a->ldo;
+  u.status = a->status;
+  u.wait_limit_ns = a->wait_limit_us > 0 ? (unsigned long long)a->wait_limit_us * 1000ull : kWaitLimitNs;
+  const uint32_t fmt = a->dtype == B200_GEMM_DTYPE_BF16 ? 1u : 0u;
+  u.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(cols >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+  u.desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  h->down = u;
+  const int64_t slots = moe_slots(a);
+  const int64_t one13 = a->experts > 1 ? a->w13_expert : 2 * a->inner * a->w13_row, one2 = a->experts > 1 ? a->w2_expert : a->hidden * a->w2_row;
+  rc = encode3(&h->up.tmap_u, a->dtype, a->w13, a->hidden, 2 * a->inner, a->experts, a->w13_row, one13, 64);
+  if (!rc) rc = encode3(&h->up.tmap_v, a->dtype, a->x, a->hidden, a->tokens, 0, a->ldx, 0, cols);
+  if (!rc) rc = encode3(&h->down.tmap_u, a->dtype, a->w2, a->inner, a->hidden, a->experts, a->w2_row, one2, 128);
+  if (!rc) rc = encode3(&h->down.tmap_v, a->dtype, u.h, a->inner, a->tokens, slots, a->inner, a->tokens * a->inner, cols);
+  if (rc) return rc;
+
+  const int64_t units = slots * ((a->inner + 63) / 64);
+  h->grid_up = (int)(units < sms ? units : sms);
+  // the down product's K axis over as many CTAs of a cluster as keep the grid within the SMs; each finishes some columns
+  const int64_t row_tiles = (a->hidden + 127) / 128;
+  int s = 1;
+  while (s < 16 && s * 2 <= cols && row_tiles * s * 2 <= sms && s * 2 <= slots * ((a->inner + kMoeTK - 1) / kMoeTK)) s *= 2;
+  h->down.cluster_split = s;
+  h->grid_down = (int)(row_tiles * s);
+  h->pdl = a->no_pdl ? 0 : 1;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(h->var.up), cudaFuncAttributeMaxDynamicSharedMemorySize, h->var.up_smem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(h->var.down), cudaFuncAttributeMaxDynamicSharedMemorySize, h->var.down_smem);
+  if (e == cudaSuccess && s > 8)
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(h->var.down), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e == cudaSuccess ? 0 : set_cuda_error(e);
+}
+
+static int moe_run(const b200_gemm_moe_handle* h, cudaStream_t stream) {
+  for (int second = 0; second < 2; ++second) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(second ? h->grid_down : h->grid_up, 1, 1);
+    cfg.blockDim = dim3(kMoeThreads, 1, 1);
+    cfg.dynamicSmemBytes = second ? h->var.down_smem : h->var.up_smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (second && h->down.cluster_split > 1) {
+      attr[n].id = cudaLaunchAttributeClusterDimension;
+      attr[n].val.clusterDim.x = h->down.cluster_split, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
+      ++n;
+    }
+    if (h->pdl) {
+      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[n].val.programmaticStreamSerializationAllowed = 1;
+      ++n;
+    }
+    cfg.attrs = n ? attr : nullptr;
+    cfg.numAttrs = n;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, second ? h->var.down : h->var.up, second ? h->down : h->up);
+    if (e != cudaSuccess) return set_cuda_error(e);
+  }
+  return 0;
+}
+
+}  // namespace b200
+
+extern "C" {
+
+uint64_t b200_gemm_moe_workspace_bytes(const b200_gemm_moe_args* args) {
+  if (b200::moe_check(args) != 0) return 0;
+  return b200::kMoeListBytes + (uint64_t)(b200::moe_slots(args) * args->tokens * args->inner) * 2;
+}
+
+int b200_gemm_moe_a16w16(const b200_gemm_moe_args* args, void* cuda_stream) {
+  b200_gemm_moe_handle h;
+  const int rc = b200::moe_prepare(args, &h);
+  return rc ? rc : b200::moe_run(&h, reinterpret_cast<cudaStream_t>(cuda_stream));
+}
+
+int b200_gemm_moe_prepare(const b200_gemm_moe_args* args, b200_gemm_moe_handle** out) {
+  if (out == nullptr) return B200_GEMM_ERR_BAD_ARG;
+  *out = nullptr;
+  b200_gemm_moe_handle* h = new (std::nothrow) b200_gemm_moe_handle;
+  if (h == nullptr) return B200_GEMM_ERR_BAD_ARG;
+  const int rc = b200::moe_prepare(args, h);
+  if (rc) {
+    delete h;
+    return rc;
+  }
+  *out = h;
+  return 0;
+}
+
+int b200_gemm_moe_launch(const b200_gemm_moe_handle* handle, void* cuda_stream) {
+  if (handle == nullptr) return B200_GEMM_ERR_BAD_ARG;
+  return b200::moe_run(handle, reinterpret_cast<cudaStream_t>(cuda_stream));
+}
+
+void b200_gemm_moe_release(b200_gemm_moe_handle* handle) { delete handle; }
+
+}  // extern "C"

@@ -307,6 +307,41 @@ typedef struct b200_gemm_quantize_args {
 } b200_gemm_quantize_args;
 int b200_gemm_quantize_a8(const b200_gemm_quantize_args* args, void* cuda_stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * A mixture-of-experts layer for a few tokens, in two kernels.
+ *   p = softmax(logits[t, :]); the top_k experts of each token, ties to the lowest index; weights divided by their sum when
+ *   `renormalize`; out[t] = sum over them of p * W2[e] (silu(G) * U), [G; U] = W13[e] x[t], rounded once.
+ * 16-bit x, weights and output (all `dtype`); sums, softmax and SiLU in fp32; p * silu(G) * U is rounded to `dtype` once, as
+ * the operand of the second product (so in fp16 it has to stay below 65504). An expert whose weight is zero (a logit of -inf)
+ * is not evaluated; a token whose logits are all -inf gets zeros; a NaN logit makes its token's output NaN. Each chosen
+ * expert's weights are read once for all tokens; non-finite values in them reach every token of the call.
+ * Limits: 1 ... 64 tokens, up to 512 experts, top_k up to 16; hidden and inner multiples of 8; x and the weights on 16-byte
+ * boundaries with strides that are multiples of 8 elements. Anything else is refused. */
+typedef struct b200_gemm_moe_args {
+  const void* x;      /* [tokens, hidden], row stride ldx                                                            */
+  const void* logits; /* router's output [tokens, experts], any strides                                              */
+  const void* w13;    /* [experts, 2 * inner, hidden]: gate rows, then up rows; strides w13_expert, w13_row           */
+  const void* w2;     /* [experts, hidden, inner]; strides w2_expert, w2_row                                         */
+  void* out;          /* [tokens, hidden], row stride ldo                                                            */
+  int64_t tokens, hidden, inner, experts;
+  int64_t ldx, logits_row, logits_col, w13_expert, w13_row, w2_expert, w2_row, ldo; /* elements                       */
+  int32_t top_k, renormalize;
+  int32_t dtype, logits_dtype; /* BF16 or FP16; FP32, BF16 or FP16                                                    */
+  int32_t wait_limit_us, no_pdl; /* as in b200_gemm_policy                                                            */
+  void* workspace;             /* b200_gemm_moe_workspace_bytes(), 256-byte aligned; needs no initialisation. Calls that share
+                                  one must be ordered on the device                                                  */
+  uint64_t workspace_bytes;
+  int32_t* status; /* as in b200_gemm_args                                                                              */
+} b200_gemm_moe_args;
+
+int b200_gemm_moe_a16w16(const b200_gemm_moe_args* args, void* cuda_stream);
+uint64_t b200_gemm_moe_workspace_bytes(const b200_gemm_moe_args* args); /* 0 for arguments that are refused */
+/* Plan once, launch many times: as b200_gemm_prepare / launch / release. */
+typedef struct b200_gemm_moe_handle b200_gemm_moe_handle;
+int b200_gemm_moe_prepare(const b200_gemm_moe_args* args, b200_gemm_moe_handle** handle);
+int b200_gemm_moe_launch(const b200_gemm_moe_handle* handle, void* cuda_stream);
+void b200_gemm_moe_release(b200_gemm_moe_handle* handle);
+
 /* Text for an error code; for B200_GEMM_ERR_LAUNCH the last CUDA error string seen by this thread. */
 const char* b200_gemm_strerror(int code);
 
