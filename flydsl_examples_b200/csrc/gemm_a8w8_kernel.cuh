@@ -73,7 +73,7 @@ struct Smem8 {
   static constexpr int kScaleBytes = k8ScaleStages * kScaleVals * 4;
   static constexpr int kBufs = TILE_Q > 128 ? 2 : 4;  // accumulators in TMEM
   static constexpr int kBarOff = kScaleOff + kScaleBytes;
-  static constexpr int kNumBars = 2 * STAGES + 2 * k8ScaleStages + 2 * kBufs;
+  static constexpr int kNumBars = 2 * STAGES + 2 * k8ScaleStages + kBufs;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kTotal = kMiscOff + 16;
   static constexpr int kDynBytes = kTotal + 1024;  // slack for manual 1024-byte alignment
@@ -169,6 +169,16 @@ __device__ __forceinline__ void raster8(const Gemm8Params& p, int tile, int& tp,
   }
 }
 
+// Both barriers' phases, the whole warp with one verdict. The two probes are in flight together; nothing else is on the path
+// of a warp that finds them complete.
+__device__ __forceinline__ bool wait_two(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag,
+                                         unsigned long long limit) {
+  const bool a = mbar_try_wait(bar0, parity0), b = mbar_try_wait(bar1, parity1);
+  if (__all_sync(0xffffffffu, a && b)) return true;
+  const bool good = mbar_wait(bar0, parity0, abort_flag, limit) && mbar_wait(bar1, parity1, abort_flag, limit);
+  return __all_sync(0xffffffffu, good);
+}
+
 template <int TILE_Q, int STAGES, int CG, bool VVEC>
 __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __grid_constant__ Gemm8Params p) {
   using L = Smem8<TILE_Q, STAGES, CG, VVEC>;
@@ -188,11 +198,13 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
   uint8_t* sm = smem_raw + (base - raw);
   const uint32_t bar0 = base + L::kBarOff;
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  // The MMAs of the K block in stage s are done: the stage may be loaded again, and the block's accumulator may be read. One
+  // commit per block serves both: an accumulator is read before its stage can have come round again (kBufs < STAGES).
+  auto done_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto sfull_bar = [&](int s) { return bar0 + 8u * (2 * STAGES + s); };
   auto sempty_bar = [&](int s) { return bar0 + 8u * (2 * STAGES + k8ScaleStages + s); };
-  auto accf_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 * k8ScaleStages + b); };
-  auto acce_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 * k8ScaleStages + kBufs + b); };
+  auto acce_bar = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 * k8ScaleStages + b); };
+  static_assert(kBufs <= STAGES, "an accumulator is read before its stage is loaded again");
   volatile uint32_t* tmem_ptr_s = reinterpret_cast<volatile uint32_t*>(sm + L::kMiscOff);
   volatile int* abort_s = reinterpret_cast<volatile int*>(sm + L::kMiscOff + 4);
   const unsigned long long wait_limit = p.wait_limit_ns;
@@ -213,16 +225,13 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(done_bar(s), 1);
     }
     for (int s = 0; s < k8ScaleStages; ++s) {
       mbar_init(sfull_bar(s), 64);
       mbar_init(sempty_bar(s), 8);
     }
-    for (int b = 0; b < kBufs; ++b) {
-      mbar_init(accf_bar(b), 1);
-      mbar_init(acce_bar(b), 8 * CG);
-    }
+    for (int b = 0; b < kBufs; ++b) mbar_init(acce_bar(b), 8 * CG);
     *abort_s = 0;
     fence_mbar_init();
     prefetch_tmap(&p.tmap_u);
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
         for (int kb = kb0; kb < p.kb_total; kb += kbstep) {
           if (issued >= STAGES) {
             int good = 1;
-            if (lane == 0) good = mbar_wait<CG == 2>(empty_bar(stage), phase ^ 1u, abort_s, wait_limit) ? 1 : 0;
+            if (lane == 0) good = mbar_wait(done_bar(stage), phase ^ 1u, abort_s, wait_limit) ? 1 : 0;
             good = __shfl_sync(0xffffffffu, good, 0);
             if (!good) {
               if (lane == 0) report_abort8(p.status, 0, tile);
@@ -309,7 +318,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA issuer (the pair's leader only)
       if (prank == 0) {
-        int stage = 0, ready = 0;
+        int stage = 0;
         uint32_t phase = 0;
         int g = 0;  // K blocks so far; each has an accumulator of its own
         bool ok = true;
@@ -318,22 +327,12 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
 #pragma unroll 1
           for (int kb = kb0; kb < p.kb_total; kb += kbstep, ++g) {
             const int buf = g % kBufs;
-            int good = 1;
-            if (lane == 0) {
-              good = mbar_wait<CG == 2>(acce_bar(buf), ((g / kBufs) & 1) ^ 1u, abort_s, wait_limit) ? 1 : 0;
-              if (good && !ready) good = mbar_wait<CG == 2>(full_bar(stage), phase, abort_s, wait_limit) ? 1 : 0;
-            }
-            good = __shfl_sync(0xffffffffu, good, 0);
-            if (!good) {
+            if (!wait_two(acce_bar(buf), ((g / kBufs) & 1) ^ 1u, full_bar(stage), phase, abort_s, wait_limit)) {
               if (lane == 0) report_abort8(p.status, 1, tile);
               ok = false;
               break;
             }
             tc_fence_after();
-            const int nstage = stage + 1 == STAGES ? 0 : stage + 1;
-            const uint32_t nphase = stage + 1 == STAGES ? phase ^ 1u : phase;
-            int next_ready = 0;
-            if (lane == 0) next_ready = (CG == 2 ? mbar_try_wait_cluster(full_bar(nstage), nphase) : mbar_try_wait(full_bar(nstage), nphase)) ? 1 : 0;
             if (elect_one()) {
               const uint32_t su = base + stage * L::kStageBytes, sv = su + k8UBytes;
               const uint64_t du = (uint64_t(p.u_desc_hi) << 32) | uint64_t(p.u_desc_lo | ((su >> 4) & 0x3fffu));
@@ -342,19 +341,13 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
 #pragma unroll
               for (int j = 0; j < k8TK / 32; ++j)
                 umma_f8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), p.idesc, j != 0 ? 1u : 0u);
-              if constexpr (CG == 2) {
-                umma_commit_pair(mapa_cluster(empty_bar(stage), 0));
-                umma_commit_pair(mapa_cluster(empty_bar(stage), 1));
-                umma_commit_pair(mapa_cluster(accf_bar(buf), 0));
-                umma_commit_pair(mapa_cluster(accf_bar(buf), 1));
-              } else {
-                umma_commit(empty_bar(stage));
-                umma_commit(accf_bar(buf));
-              }
+              if constexpr (CG == 2)
+                umma_commit_both(done_bar(stage));
+              else
+                umma_commit(done_bar(stage));
             }
-            ready = __shfl_sync(0xffffffffu, next_ready, 0);
-            stage = nstage;
-            phase = nphase;
+            __syncwarp();
+            if (++stage == STAGES) stage = 0, phase ^= 1u;
           }
         }
       }
@@ -416,31 +409,28 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
     const int row = quarter * 32 + lane;
     const float* ring = reinterpret_cast<const float*>(sm + L::kScaleOff);
     const uint32_t image = base + L::kOutOff + (uint32_t)(warp - 4) * 4096u;
-    int g = 0;
+    int g = 0, stage = 0;
+    uint32_t phase = 0;
 #pragma unroll 1
     for (int tile = tile0; tile < p.num_tiles; tile += tile_step) {
       int tp, tq;
       raster8(p, tile, tp, tq);
       const int prow = (tp * CG + prank) * k8TileP + row;
       const int qbase = tq * TILE_Q + half * HC;
-      float acc[HC];
+      uint64_t acc2[HC / 2];  // two neighbouring columns each: fma.rn.f32x2 does both in one issue slot
 #pragma unroll
-      for (int i = 0; i < HC; ++i) acc[i] = 0.f;
+      for (int i = 0; i < HC / 2; ++i) acc2[i] = 0;
+      auto acc = [&](int i) { return __uint_as_float((uint32_t)(i & 1 ? acc2[i >> 1] >> 32 : acc2[i >> 1])); };
       bool ok = true;
 #pragma unroll 1
       for (int kb = kb0; kb < p.kb_total; kb += kbstep, ++g) {
         const int buf = g % kBufs, ss = g % k8ScaleStages;
         // The verdict is the warp's: tcgen05.ld needs all its lanes.
-        bool good = mbar_wait(sfull_bar(ss), (g / k8ScaleStages) & 1, abort_s, wait_limit);
-        good = good && mbar_wait<CG == 2>(accf_bar(buf), (g / kBufs) & 1, abort_s, wait_limit);
-        if (!__all_sync(0xffffffffu, good)) {
+        if (!wait_two(sfull_bar(ss), (g / k8ScaleStages) & 1, done_bar(stage), phase, abort_s, wait_limit)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const float* sc = ring + ss * L::kScaleVals;
-        const float su = VVEC ? sc[row] : sc[row] * sc[k8TileP + half];
-        const float* sv = sc + k8TileP + half * HC;
         const uint32_t t_acc = tmem_base + buf * TILE_Q + half * HC + (uint32_t(quarter * 32) << 16);
         uint32_t ra[32], rb[32];
         auto load_chunk = [&](uint32_t(&r)[32], int c) {
@@ -451,46 +441,49 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
           else
             tmem_ld_32x8(t_acc + c * CW, r);
         };
+        load_chunk(ra, 0);
+        if (NCH > 1) load_chunk(rb, 1);
+        const float* sc = ring + ss * L::kScaleVals;
+        const float su = VVEC ? sc[row] : sc[row] * sc[k8TileP + half];
+        const float* sv = sc + k8TileP + half * HC;
+        const uint64_t su2 = pack_f32x2(su, su);
         auto add_chunk = [&](const uint32_t(&r)[32], int c) {
 #pragma unroll
           for (int i = 0; i < CW; i += 4) {
+            uint64_t s0 = su2, s1 = su2;
             if constexpr (VVEC) {
               const float4 v4 = *reinterpret_cast<const float4*>(sv + c * CW + i);
-              acc[c * CW + i] = fmaf(__uint_as_float(r[i]), su * v4.x, acc[c * CW + i]);
-              acc[c * CW + i + 1] = fmaf(__uint_as_float(r[i + 1]), su * v4.y, acc[c * CW + i + 1]);
-              acc[c * CW + i + 2] = fmaf(__uint_as_float(r[i + 2]), su * v4.z, acc[c * CW + i + 2]);
-              acc[c * CW + i + 3] = fmaf(__uint_as_float(r[i + 3]), su * v4.w, acc[c * CW + i + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[c * CW + i + j] = fmaf(__uint_as_float(r[i + j]), su, acc[c * CW + i + j]);
+              s0 = mul_f32x2(su2, pack_f32x2(v4.x, v4.y));
+              s1 = mul_f32x2(su2, pack_f32x2(v4.z, v4.w));
             }
+            uint64_t* a = acc2 + (c * CW + i) / 2;
+            a[0] = fma_f32x2(pack_u32x2(r[i], r[i + 1]), s0, a[0]);
+            a[1] = fma_f32x2(pack_u32x2(r[i + 2], r[i + 3]), s1, a[1]);
           }
         };
-        load_chunk(ra, 0);
-        tmem_ld_wait();
+        auto release = [&]() {  // the accumulator has been read: it may be written again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2 && prank != 0)
+              mbar_arrive_remote(acce_bar(buf), 0);
+            else
+              mbar_arrive(acce_bar(buf));
+          }
+        };
+        // Two loads travel together and each buffer is refilled as soon as its values are added.
 #pragma unroll
         for (int c = 0; c < NCH; c += 2) {
-          if (c + 1 < NCH) {
-            load_chunk(rb, c + 1);
-            add_chunk(ra, c);
-            tmem_ld_wait();
-            if (c + 2 < NCH) load_chunk(ra, c + 2);
-            add_chunk(rb, c + 1);
-            if (c + 2 < NCH) tmem_ld_wait();
-          } else {
-            add_chunk(ra, c);
-          }
+          tmem_ld_wait();
+          if (c + 2 >= NCH) release();
+          add_chunk(ra, c);
+          if (c + 2 < NCH) load_chunk(ra, c + 2);
+          if (c + 1 < NCH) add_chunk(rb, c + 1);
+          if (c + 3 < NCH) load_chunk(rb, c + 3);
         }
-        // accumulator and scales are in registers: hand both back
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(sempty_bar(ss));
-          if (CG == 2 && prank != 0)
-            mbar_arrive_cluster(acce_bar(buf), 0);
-          else
-            mbar_arrive(acce_bar(buf));
-        }
+        if (lane == 0) mbar_arrive(sempty_bar(ss));  // the scales are read
+        if (++stage == STAGES) stage = 0, phase ^= 1u;
       }
       if (!ok) {
         if (lane == 0) report_abort8(p.status, 3, tile);
@@ -511,7 +504,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
           const int c = half * HC + i;
           const uint32_t dst = mapa_cluster(recv + (uint32_t)(((rank << own_log2) + (c & ((1 << own_log2) - 1))) * k8TileP) * 4u,
                                             (uint32_t)(c >> own_log2));
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(acc[i]) : "memory");
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(acc(i)) : "memory");
         }
       } else if (p.swap_out) {
         // D^T: the lanes of a warp write neighbouring addresses
@@ -519,7 +512,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
           const float b = p.bias != nullptr ? load_as_float(p.bias, prow, p.bias_dtype) : 0.f;
 #pragma unroll
           for (int i = 0; i < HC; ++i)
-            if (qbase + i < p.Q) store_one(p.out, (long long)(qbase + i) * p.ldo + prow, acc[i] + b, p.out_dtype);
+            if (qbase + i < p.Q) store_one(p.out, (long long)(qbase + i) * p.ldo + prow, acc(i) + b, p.out_dtype);
         }
       } else if (HC >= 64 && p.tma_store) {
         // One 128-byte row segment per lane into the warp's swizzled image (16-byte piece j of row t at j ^ (t % 8)), which
@@ -546,7 +539,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
             for (int j = 0; j < 4; ++j) {
               float v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = acc[f * 32 + j * 8 + i];
+              for (int i = 0; i < 8; ++i) v[i] = acc(f * 32 + j * 8 + i);
               add_bias8(p, v, qbase + f * 32 + j * 8);
 #pragma unroll
               for (int h = 0; h < 2; ++h)
@@ -564,7 +557,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
             for (int j = 0; j < 8; ++j) {
               float v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = acc[f * 64 + j * 8 + i];
+              for (int i = 0; i < 8; ++i) v[i] = acc(f * 64 + j * 8 + i);
               add_bias8(p, v, qbase + f * 64 + j * 8);
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_base + (uint32_t)((j ^ (lane & 7)) << 4)),
                            "r"(pack16(v[0], v[1], p.out_dtype)), "r"(pack16(v[2], v[3], p.out_dtype)),
@@ -579,7 +572,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
         for (int j = 0; j < HC / 8; ++j) {
           float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = acc[j * 8 + i];
+          for (int i = 0; i < 8; ++i) v[i] = acc(j * 8 + i);
           add_bias8(p, v, qbase + j * 8);
           store_row8(p, v, prow, qbase + j * 8);
         }
