@@ -170,15 +170,9 @@ EXPORTS = (
     "b200_gemm_describe_variant",
     "b200_gemm_a8w8",
     "b200_gemm_a8w8_plan_query",
-    "b200_gemm_a8w8_prepare",
-    "b200_gemm_a8w8_launch",
-    "b200_gemm_a8w8_release",
     "b200_gemm_quantize_a8",
     "b200_gemm_moe_a16w16",
     "b200_gemm_moe_workspace_bytes",
-    "b200_gemm_moe_prepare",
-    "b200_gemm_moe_launch",
-    "b200_gemm_moe_release",
     "b200_gemm_cast_bias",
     "b200_gemm_reduce_slots",
     "b200_peer_export",
@@ -238,24 +232,12 @@ def load() -> C.CDLL:
     lib.b200_gemm_a8w8.restype = C.c_int
     lib.b200_gemm_a8w8_plan_query.argtypes = [C.POINTER(Args8), C.POINTER(Plan)]
     lib.b200_gemm_a8w8_plan_query.restype = C.c_int
-    lib.b200_gemm_a8w8_prepare.argtypes = [C.POINTER(Args8), C.POINTER(C.c_void_p)]
-    lib.b200_gemm_a8w8_prepare.restype = C.c_int
-    lib.b200_gemm_a8w8_launch.argtypes = [C.c_void_p, C.c_void_p]
-    lib.b200_gemm_a8w8_launch.restype = C.c_int
-    lib.b200_gemm_a8w8_release.argtypes = [C.c_void_p]
-    lib.b200_gemm_a8w8_release.restype = None
     lib.b200_gemm_quantize_a8.argtypes = [C.POINTER(QuantizeArgs), C.c_void_p]
     lib.b200_gemm_quantize_a8.restype = C.c_int
     lib.b200_gemm_moe_a16w16.argtypes = [C.POINTER(MoeArgs), C.c_void_p]
     lib.b200_gemm_moe_a16w16.restype = C.c_int
     lib.b200_gemm_moe_workspace_bytes.argtypes = [C.POINTER(MoeArgs)]
     lib.b200_gemm_moe_workspace_bytes.restype = C.c_uint64
-    lib.b200_gemm_moe_prepare.argtypes = [C.POINTER(MoeArgs), C.POINTER(C.c_void_p)]
-    lib.b200_gemm_moe_prepare.restype = C.c_int
-    lib.b200_gemm_moe_launch.argtypes = [C.c_void_p, C.c_void_p]
-    lib.b200_gemm_moe_launch.restype = C.c_int
-    lib.b200_gemm_moe_release.argtypes = [C.c_void_p]
-    lib.b200_gemm_moe_release.restype = None
     lib.b200_gemm_cast_bias.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
     lib.b200_gemm_cast_bias.restype = C.c_int
     lib.b200_gemm_reduce_slots.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
@@ -277,6 +259,18 @@ def load() -> C.CDLL:
     lib.b200_gemm_version.restype = C.c_char_p
     _lib = lib
     return lib
+
+
+_fast: dict = {}
+
+
+def fast(name: str):
+    """The entry point `int name(const args*, stream)` taking its argument block as bytes: filling a ctypes structure member by
+    member costs more than the launch it describes."""
+    fn = _fast.get(name)
+    if fn is None:
+        fn = _fast[name] = C.CFUNCTYPE(C.c_int, C.c_char_p, C.c_void_p)((name, load()))
+    return fn
 
 
 def strerror(code: int) -> str:

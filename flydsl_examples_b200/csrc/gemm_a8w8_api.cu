@@ -1,21 +1,19 @@
 // Host side of the 8-bit block-scaled GEMM and its quantizer: validation, plan, tensor maps, launch. Exports the
 // b200_gemm_a8w8_* and b200_gemm_quantize_a8 entry points of include/b200_gemm.h. No device allocation, no synchronisation.
 #include <cstring>
-#include <mutex>
-#include <new>
 
 #include "../../include/b200_gemm.h"
 #include "gemm_a8w8_variants.h"
 #include "host.h"
 #include "quantize_kernel.cuh"
 
-struct b200_gemm_a8w8_handle {
-  b200::Gemm8Params params;
-  b200::Variant8 var;
-  int grid, device, cluster, pdl;
-};
-
 namespace b200 {
+
+struct Call8 {
+  Gemm8Params params;
+  Variant8 var;
+  int grid, cluster, pdl;
+};
 
 static bool is_fp8(int dt) { return dt == B200_GEMM_DTYPE_E4M3 || dt == B200_GEMM_DTYPE_E5M2; }
 
@@ -91,13 +89,7 @@ static void make_desc8(int mn_major, uint32_t* hi, uint32_t* lo, uint32_t* kstep
   *kstep = mn_major ? (4096 >> 4) : (32 >> 4);
 }
 
-static int device_sms(int* dev, int* sms) {
-  if (cudaGetDevice(dev) != cudaSuccess) return B200_GEMM_ERR_LAUNCH;
-  const cudaError_t e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev);
-  return e == cudaSuccess ? 0 : set_cuda_error(e);
-}
-
-static int prepare8(const b200_gemm_a8w8_args* a, b200_gemm_a8w8_handle* h) {
+static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   int dev = 0, sms = 0;
   b200_gemm_plan pl;
   Variant8 var;
@@ -111,7 +103,7 @@ static int prepare8(const b200_gemm_a8w8_args* a, b200_gemm_a8w8_handle* h) {
   if (!aligned(a->a_scale, 4) || !aligned(a->b_scale, 4) || !aligned(a->out, es)) return B200_GEMM_ERR_BAD_ARG;
   if (a->bias != nullptr && (a->bias_dtype < 1 || a->bias_dtype > 3 || !aligned(a->bias, a->bias_dtype == 1 ? 4 : 2)))
     return B200_GEMM_ERR_BAD_ARG;
-  rc = device_sms(&dev, &sms);
+  rc = current_sms(&dev, &sms);
   if (rc) return rc;
   rc = resolve8(a, sms, &pl, &var);
   if (rc) return rc;
@@ -163,16 +155,12 @@ static int prepare8(const b200_gemm_a8w8_args* a, b200_gemm_a8w8_handle* h) {
 
   h->var = var;
   h->grid = pl.grid;
-  h->device = dev;
   h->cluster = pl.cta_group == 2 ? 2 : pl.cluster_split;
   h->pdl = a->policy.no_pdl ? 0 : 1;
-  const void* fn = reinterpret_cast<const void*>(var.fn);
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, var.smem_bytes);
-  if (e == cudaSuccess && h->cluster > 8) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return e == cudaSuccess ? 0 : set_cuda_error(e);
+  return allow_launch(reinterpret_cast<const void*>(var.fn), var.smem_bytes, dev);
 }
 
-static int run8(const b200_gemm_a8w8_handle* h, cudaStream_t stream) {
+static int run8(const Call8* h, cudaStream_t stream) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(h->grid, 1, 1);
@@ -214,37 +202,16 @@ extern "C" {
 int b200_gemm_a8w8_plan_query(const b200_gemm_a8w8_args* args, b200_gemm_plan* plan) {
   if (plan == nullptr) return B200_GEMM_ERR_BAD_ARG;
   int dev = 0, sms = 0;
-  if (b200::device_sms(&dev, &sms) != 0) sms = 148;
+  if (b200::current_sms(&dev, &sms) != 0) sms = 148;
   b200::Variant8 var;
   return b200::resolve8(args, sms, plan, &var);
 }
 
 int b200_gemm_a8w8(const b200_gemm_a8w8_args* args, void* cuda_stream) {
-  b200_gemm_a8w8_handle h;
+  b200::Call8 h;
   const int rc = b200::prepare8(args, &h);
   return rc ? rc : b200::run8(&h, reinterpret_cast<cudaStream_t>(cuda_stream));
 }
-
-int b200_gemm_a8w8_prepare(const b200_gemm_a8w8_args* args, b200_gemm_a8w8_handle** out) {
-  if (out == nullptr) return B200_GEMM_ERR_BAD_ARG;
-  *out = nullptr;
-  b200_gemm_a8w8_handle* h = new (std::nothrow) b200_gemm_a8w8_handle;
-  if (h == nullptr) return B200_GEMM_ERR_BAD_ARG;
-  const int rc = b200::prepare8(args, h);
-  if (rc) {
-    delete h;
-    return rc;
-  }
-  *out = h;
-  return 0;
-}
-
-int b200_gemm_a8w8_launch(const b200_gemm_a8w8_handle* handle, void* cuda_stream) {
-  if (handle == nullptr) return B200_GEMM_ERR_BAD_ARG;
-  return b200::run8(handle, reinterpret_cast<cudaStream_t>(cuda_stream));
-}
-
-void b200_gemm_a8w8_release(b200_gemm_a8w8_handle* handle) { delete handle; }
 
 int b200_gemm_quantize_a8(const b200_gemm_quantize_args* a, void* cuda_stream) {
   if (a == nullptr || a->rows < 0 || a->cols < 0) return B200_GEMM_ERR_BAD_ARG;

@@ -340,6 +340,27 @@ int set_cuda_error(cudaError_t e) {
   return B200_GEMM_ERR_LAUNCH;
 }
 
+int current_sms(int* dev, int* sms) {
+  DeviceInfo* info = nullptr;
+  const int rc = current_device_info(&info, dev);
+  if (rc == 0) *sms = info->sm_count;
+  return rc;
+}
+
+int allow_launch(const void* fn, int smem_bytes, int dev) {
+  constexpr int kMax = 64;  // more kernels than the library has; beyond it the attributes are set at every call
+  static const void* done[kMaxDevices][kMax];
+  static int count[kMaxDevices];
+  std::lock_guard<std::mutex> lock(g_dev_mutex);
+  for (int i = 0; i < count[dev]; ++i)
+    if (done[dev][i] == fn) return 0;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return set_cuda_error(e);
+  if (count[dev] < kMax) done[dev][count[dev]++] = fn;
+  return 0;
+}
+
 // A fully resolved call: everything the launch needs, so that repeating it costs one kernel launch (two when an operand must be repacked first)
 // and no host-side planning or tensor-map encoding.
 struct RepackJob {

@@ -18,4 +18,10 @@ EncodeTiledFn get_encode_fn();
 // Keeps the error's text for b200_gemm_strerror and returns B200_GEMM_ERR_LAUNCH.
 int set_cuda_error(cudaError_t e);
 
+// The current device and its number of SMs.
+int current_sms(int* dev, int* sms);
+
+// Lets `fn` launch with `smem_bytes` of dynamic shared memory and clusters of up to 16 CTAs on device `dev`; done once for each.
+int allow_launch(const void* fn, int smem_bytes, int dev);
+
 }  // namespace b200

@@ -1,7 +1,6 @@
 // Host side of the few-token mixture-of-experts layer (b200_gemm_moe_* in include/b200_gemm.h): validation, tensor maps, the two
 // launches. No device allocation, no synchronisation.
 #include <cstring>
-#include <new>
 
 #include "../../include/b200_gemm.h"
 #include "host.h"
@@ -57,17 +56,13 @@ static int encode3(CUtensorMap* map, int dtype, const void* ptr, int64_t d0, int
   return res == CUDA_SUCCESS ? 0 : B200_GEMM_ERR_TENSOR_MAP;
 }
 
-}  // namespace b200
-
-struct b200_gemm_moe_handle {
-  b200::MoeParams up, down;
-  b200::MoeVariant var;
+struct MoeCall {
+  MoeParams up, down;
+  MoeVariant var;
   int grid_up, grid_down, pdl;
 };
 
-namespace b200 {
-
-static int moe_prepare(const b200_gemm_moe_args* a, b200_gemm_moe_handle* h) {
+static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   int rc = moe_check(a);
   if (rc) return rc;
   if (a->x == nullptr || a->logits == nullptr || a->w13 == nullptr || a->w2 == nullptr || a->out == nullptr) return B200_GEMM_ERR_BAD_ARG;
@@ -76,9 +71,8 @@ static int moe_prepare(const b200_gemm_moe_args* a, b200_gemm_moe_handle* h) {
     return B200_GEMM_ERR_BAD_ARG;
   if (a->workspace == nullptr || off(a->workspace, 256) || a->workspace_bytes < b200_gemm_moe_workspace_bytes(a)) return B200_GEMM_ERR_WORKSPACE;
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return B200_GEMM_ERR_LAUNCH;
-  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return set_cuda_error(e);
+  rc = current_sms(&dev, &sms);
+  if (rc) return rc;
 
   memset(h, 0, sizeof(*h));
   h->var = moe_variant(a->tokens);
@@ -114,15 +108,11 @@ static int moe_prepare(const b200_gemm_moe_args* a, b200_gemm_moe_handle* h) {
   h->down.cluster_split = s;
   h->grid_down = (int)(row_tiles * s);
   h->pdl = a->no_pdl ? 0 : 1;
-  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(h->var.up), cudaFuncAttributeMaxDynamicSharedMemorySize, h->var.up_smem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(h->var.down), cudaFuncAttributeMaxDynamicSharedMemorySize, h->var.down_smem);
-  if (e == cudaSuccess && s > 8)
-    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(h->var.down), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return e == cudaSuccess ? 0 : set_cuda_error(e);
+  rc = allow_launch(reinterpret_cast<const void*>(h->var.up), h->var.up_smem, dev);
+  return rc ? rc : allow_launch(reinterpret_cast<const void*>(h->var.down), h->var.down_smem, dev);
 }
 
-static int moe_run(const b200_gemm_moe_handle* h, cudaStream_t stream) {
+static int moe_run(const MoeCall* h, cudaStream_t stream) {
   for (int second = 0; second < 2; ++second) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
@@ -160,30 +150,9 @@ uint64_t b200_gemm_moe_workspace_bytes(const b200_gemm_moe_args* args) {
 }
 
 int b200_gemm_moe_a16w16(const b200_gemm_moe_args* args, void* cuda_stream) {
-  b200_gemm_moe_handle h;
+  b200::MoeCall h;
   const int rc = b200::moe_prepare(args, &h);
   return rc ? rc : b200::moe_run(&h, reinterpret_cast<cudaStream_t>(cuda_stream));
 }
-
-int b200_gemm_moe_prepare(const b200_gemm_moe_args* args, b200_gemm_moe_handle** out) {
-  if (out == nullptr) return B200_GEMM_ERR_BAD_ARG;
-  *out = nullptr;
-  b200_gemm_moe_handle* h = new (std::nothrow) b200_gemm_moe_handle;
-  if (h == nullptr) return B200_GEMM_ERR_BAD_ARG;
-  const int rc = b200::moe_prepare(args, h);
-  if (rc) {
-    delete h;
-    return rc;
-  }
-  *out = h;
-  return 0;
-}
-
-int b200_gemm_moe_launch(const b200_gemm_moe_handle* handle, void* cuda_stream) {
-  if (handle == nullptr) return B200_GEMM_ERR_BAD_ARG;
-  return b200::moe_run(handle, reinterpret_cast<cudaStream_t>(cuda_stream));
-}
-
-void b200_gemm_moe_release(b200_gemm_moe_handle* handle) { delete handle; }
 
 }  // extern "C"

@@ -16,6 +16,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
 
 namespace b200 {
@@ -57,24 +59,40 @@ __device__ __forceinline__ uint32_t pack_fp8x2(float lo, float hi, int e5m2) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
 }
 
+// Eight consecutive elements, and what the groups' maxima need: magnitudes compare like unsigned integers, so 16-bit values
+// are compared two to an instruction as they are (`Mag` = two of them), fp32 values one by one.
 template <typename T>
-struct RawRow;  // eight consecutive elements
-template <>
-struct RawRow<float> {
-  float v[8];
-  __device__ __forceinline__ float get(int i) const { return v[i]; }
-};
-template <>
-struct RawRow<__nv_bfloat16> {
-  uint32_t w[4];
-  __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
-};
-template <>
-struct RawRow<__half> {
-  uint32_t w[4];
+struct RawRow {
+  static constexpr int kWords = sizeof(T) == 4 ? 8 : 4;
+  uint32_t w[kWords];
   __device__ __forceinline__ float get(int i) const {
-    const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
-    return i & 1 ? __high2float(h) : __low2float(h);
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    } else {
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+      return i & 1 ? __high2float(h) : __low2float(h);
+    }
+  }
+};
+template <typename T>
+struct Mag {
+  static constexpr bool kWide = sizeof(T) == 4;
+  static constexpr uint32_t kAbs = kWide ? 0x7fffffffu : 0x7fff7fffu;
+  static constexpr uint32_t kInf = kWide ? 0x7f800000u : std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;  // and above: NaN
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return kWide ? max(a, b) : __vmaxu2(a, b); }
+  static __device__ __forceinline__ bool any_odd(uint32_t m) { return kWide ? m >= kInf : (m & 0xffffu) >= kInf || (m >> 16) >= kInf; }
+  static __device__ __forceinline__ uint32_t only_finite(uint32_t m) {
+    if constexpr (kWide) return m >= kInf ? 0u : m;
+    return ((m & 0xffffu) >= kInf ? 0u : m & 0xffffu) | ((m >> 16) >= kInf ? 0u : m & 0xffff0000u);
+  }
+  // the magnitude in half h of the word, as fp32
+  static __device__ __forceinline__ float value(uint32_t m, int h) {
+    if constexpr (kWide) return __uint_as_float(m);
+    const uint32_t b = h ? m >> 16 : m & 0xffffu;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(b << 16);
+    return __half2float(__ushort_as_half((unsigned short)b));
   }
 };
 
@@ -82,25 +100,20 @@ template <typename T>
 __device__ __forceinline__ RawRow<T> load_row8(const T* src, int n, bool vec) {
   RawRow<T> r;
   if (n >= 8 && vec) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src));  // read once
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
     if constexpr (sizeof(T) == 4) {
-      const uint4 b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(w[i]);
-    } else {
-      r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+      const uint4 b = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
+      r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
     }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = i < n ? __float_as_uint(src[i]) : 0u;
   } else {
-    if constexpr (sizeof(T) == 4) {
+    const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = i < n ? src[i] : 0.f;
-    } else {
-      const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        r.w[i] = (uint32_t)(2 * i < n ? s[2 * i] : 0) | ((uint32_t)(2 * i + 1 < n ? s[2 * i + 1] : 0) << 16);
-    }
+    for (int i = 0; i < 4; ++i)
+      r.w[i] = (uint32_t)(2 * i < n ? s[2 * i] : 0) | ((uint32_t)(2 * i + 1 < n ? s[2 * i + 1] : 0) << 16);
   }
   return r;
 }
@@ -131,27 +144,40 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantP
     v[i] = load_row8<T>(x + (in ? (long long)(r0 + r) * p.ldx + col : 0), in ? ncol : 0, vec);
   }
 
-  // Magnitudes of finite values; a value that is not finite counts as zero and raises a flag.
-  bool odd = false;
-  auto mag = [&](float f) {
-    const float a = fabsf(f);
-    return a < __uint_as_float(0x7f800000u) ? a : 0.f;
-  };
-  float cmax[8], rmax[kPasses];
+  // Largest magnitudes per row (over the thread's eight columns) and per column (over its eight rows).
+  using M = Mag<T>;
+  constexpr int kW = RawRow<T>::kWords;
+  uint32_t rmag[kPasses], cmag[kW];
+  auto maxima = [&](auto finite) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
+    for (int j = 0; j < kW; ++j) cmag[j] = 0;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    rmax[i] = 0.f;
+    for (int i = 0; i < kPasses; ++i) {
+      rmag[i] = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f = v[i].get(j);
-      odd |= !(fabsf(f) < __uint_as_float(0x7f800000u));
-      const float a = mag(f);
-      if (MODE & 5) rmax[i] = fmaxf(rmax[i], a);
-      if (MODE & 2) cmax[j] = fmaxf(cmax[j], a);
+      for (int j = 0; j < kW; ++j) {
+        const uint32_t m = finite(v[i].w[j] & M::kAbs);
+        if (MODE & 5) rmag[i] = M::max2(rmag[i], m);
+        if (MODE & 2) cmag[j] = M::max2(cmag[j], m);
+      }
     }
+  };
+  maxima([](uint32_t m) { return m; });
+  uint32_t all = 0;
+  if (MODE & 2) {
+#pragma unroll
+    for (int j = 0; j < kW; ++j) all = M::max2(all, cmag[j]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) all = M::max2(all, rmag[i]);
   }
+  const bool odd = M::any_odd(all);  // an infinity or a NaN among them: it counts as zero
+  if (odd) maxima([](uint32_t m) { return M::only_finite(m); });
+  float rmax[kPasses], cmax[8];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) rmax[i] = M::kWide ? M::value(rmag[i], 0) : fmaxf(M::value(rmag[i], 0), M::value(rmag[i], 1));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) cmax[j] = M::kWide ? M::value(cmag[j % kW], 0) : M::value(cmag[(j >> 1) % kW], j & 1);
   // Eight values of one row times their inverse scales, converted and stored.
   auto put = [&](uint8_t* dst, const RawRow<T>& raw, const float (&inv)[8], bool dvec) {
     uint32_t w[2];

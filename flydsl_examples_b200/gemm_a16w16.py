@@ -42,12 +42,13 @@ class _Workspace:
     4-word status block kernels write when a bounded wait gives up. Grows on demand, never shrinks.
     Takes the place of get_split_k_buffers (kernels/gemm_a16w16_gfx950.py:1277-1281)."""
 
-    __slots__ = ("buf", "status", "generation")
+    __slots__ = ("buf", "status", "status_ptr", "generation")
 
     def __init__(self, device: torch.device):
         self.buf = None
         self.generation = 0
         self.status = torch.zeros(_STATUS_WORDS, dtype=torch.int32, device=device)
+        self.status_ptr = self.status.data_ptr()
 
     def ensure(self, nbytes: int, device: torch.device, stream: torch.cuda.Stream) -> None:
         if self.buf is None or self.buf.numel() < nbytes:
@@ -57,8 +58,10 @@ class _Workspace:
             self.generation += 1  # prepared launches that point into the old buffer are stale
 
 
-def _workspace_for(device: torch.device, stream: torch.cuda.Stream) -> _Workspace:
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream.cuda_stream)
+def _workspace_for(device: torch.device, stream) -> _Workspace:
+    """The workspace of a device and a stream (a torch.cuda.Stream or its handle)."""
+    key = (device.index if device.index is not None else torch.cuda.current_device(),
+           stream if isinstance(stream, int) else stream.cuda_stream)
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None:

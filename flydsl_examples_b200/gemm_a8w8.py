@@ -11,14 +11,15 @@ libb200_gemm.so (hand-written sm_100a CUDA), there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
-import threading
-from collections import OrderedDict
+import functools
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .gemm_a16w16 import _num_sms, _workspace_for
+from ._launch import device_sms, on_device, raw_stream
+from .gemm_a16w16 import _workspace_for
 
 GROUP = 128
 _F8_ID = {torch.float8_e4m3fn: _lib.DTYPE_E4M3, torch.float8_e5m2: _lib.DTYPE_E5M2}
@@ -31,6 +32,12 @@ def _blocks(n: int) -> int:
 
 
 # ------------------------------------------------------------------------------------------------------------ policy
+@functools.lru_cache(maxsize=4096)
+def _heuristic_items(m, n, k, a_t, b_t, num_sms) -> tuple:
+    pol = heuristic_a8w8(m, n, k, a_t, b_t, num_sms)
+    return pol["tile_n"], pol["cta_group"], pol["split_k"], pol.get("group_m", 0), int(pol["swap_ab"])
+
+
 def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: bool, num_sms: int = 148) -> dict:
     """Tile, split and operand order for a call without a tiling of its own.
 
@@ -65,64 +72,38 @@ def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: boo
     return pol
 
 
-def _resolve(m, n, k, a_t, b_t, user_kwargs, num_sms) -> dict:
+def _policy(m, n, k, a_t, b_t, user_kwargs, num_sms) -> tuple:
+    """The fields of b200_gemm_policy, in its order."""
+    if not user_kwargs:
+        tile_n, cta_group, split_k, group_m, swap_ab = _heuristic_items(m, n, k, a_t, b_t, num_sms)
+        return tile_n, 0, split_k, group_m, swap_ab, cta_group, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0
     for key in user_kwargs:
         if key not in _POLICY_KEYS:
             raise ValueError(f"unknown gemm_a8w8 policy key {key!r}; expected some of {_POLICY_KEYS}")
     if "tile_n" in user_kwargs:
-        pol = {"cta_group": 1, "swap_ab": False, "split_k": 1, "group_m": 0}
+        pol = {"cta_group": 1, "swap_ab": False, "split_k": 1}
     else:
         pol = heuristic_a8w8(m, n, k, a_t, b_t, num_sms)
         for key in ("cta_group", "split_k", "swap_ab"):
             if key in user_kwargs:
                 raise ValueError(f"gemm_a8w8 policy key {key!r} needs 'tile_n' beside it")
     pol.update(user_kwargs)
-    return pol
-
-
-# ----------------------------------------------------------------------------------------------------- prepared calls
-_PREPARED_MAX = 1024
-_prepared: "OrderedDict[tuple, tuple]" = OrderedDict()
-_prepared_lock = threading.Lock()
-
-
-def clear_prepared_calls() -> None:
-    """Drop every cached launch handle."""
-    with _prepared_lock:
-        items = list(_prepared.values())
-        _prepared.clear()
-    for handle, _, _ in items:
-        _lib.load().b200_gemm_a8w8_release(handle)
-
-
-def _describe(t: Optional[torch.Tensor]):
-    return None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype)
-
-
-def _launch_cached(key, stream_ptr) -> bool:
-    """Repeat of a call seen before. The lock is held over the launch: a handle is released only after it has left the table."""
-    with _prepared_lock:
-        ent = _prepared.get(key)
-        if ent is None:
-            return False
-        handle, dev, _ = ent
-        lib = _lib.load()
-        if torch.cuda.current_device() == dev:
-            rc = lib.b200_gemm_a8w8_launch(handle, stream_ptr)
-        else:
-            with torch.cuda.device(dev):
-                rc = lib.b200_gemm_a8w8_launch(handle, stream_ptr)
-    if rc != 0:
-        raise RuntimeError(f"b200_gemm_a8w8_launch failed ({rc}): {_lib.strerror(rc)}")
-    return True
+    return (pol["tile_n"], 0, pol["split_k"], pol.get("group_m", 0), int(pol["swap_ab"]), pol["cta_group"], 0, pol.get("max_ctas", 0), 0,
+            0 if pol.get("pdl", True) else 1, 0, pol.get("wait_limit_us", 0), 0, 0, 0, 0)
 
 
 # -------------------------------------------------------------------------------------------------------------- GEMM
+_LAYOUTS = {"nn": (False, False), "nt": (False, True), "tn": (True, False), "tt": (True, True)}
+_ARGS = struct.Struct("@6P10q8i16iP")  # b200_gemm_a8w8_args
+
+
 def _check_operand(name: str, t: torch.Tensor, transposed: bool) -> int:
     """Leading stride of an operand; raises unless the contiguous dimension has stride 1 and rows start on 16 bytes."""
     rows, cols = t.shape
-    inner, lead = (t.stride(0), t.stride(1)) if transposed else (t.stride(1), t.stride(0))
-    n_inner, n_lead = (rows, cols) if transposed else (cols, rows)
+    lead, inner = t.stride()
+    n_lead, n_inner = rows, cols
+    if transposed:
+        lead, inner, n_lead, n_inner = inner, lead, n_inner, n_lead
     if n_inner == 1:
         inner = 1  # a stride of a size-1 dimension is arbitrary in torch
     if n_lead == 1:
@@ -136,56 +117,43 @@ def _check_operand(name: str, t: torch.Tensor, transposed: bool) -> int:
     return lead
 
 
-def _check_scale(name: str, s: torch.Tensor, rows: int, kb: int, device) -> int:
-    """1 when the scale is one per 128 rows, 0 when one per row; s is [rows or blocks of rows, blocks of K]."""
-    if s.ndim != 2 or s.dtype != torch.float32 or s.shape[1] != kb or s.shape[0] not in (rows, _blocks(rows)):
+def _check_scale(name: str, s: torch.Tensor, rows: int, kb: int, have_rows: int, have_kb: int) -> int:
+    """1 when the scale is one per 128 rows, 0 when one per row."""
+    if s.dtype is not torch.float32 or have_kb != kb or have_rows != rows and have_rows != _blocks(rows):
         raise ValueError(
-            f"{name} must be a float32 tensor with one scale per block of {GROUP} along K and per row or block of {GROUP} rows: "
-            f"expected {rows} or {_blocks(rows)} by {kb}, got {tuple(s.shape)} {s.dtype}"
+            f"{name} must be a float32 tensor with one scale per block of {GROUP} along K and per row (column) or block of {GROUP}: "
+            f"expected {rows} or {_blocks(rows)} and {kb}, got shape {tuple(s.shape)}, {s.dtype}"
         )
-    if s.device != device:
-        raise ValueError(f"{name} is on {s.device}, the operands are on {device}")
-    return 0 if s.shape[0] == rows else 1
+    return 0 if have_rows == rows else 1
 
 
-def _fill_args(a, a_scale, b, b_scale, out, bias, a_t, b_t, pol) -> _lib.Args8:
+def _arguments(a, a_scale, b, b_scale, out_ptr, out_dtype, bias, layout, user_kwargs, num_sms, status) -> bytes:
+    """Checks the operands and packs a b200_gemm_a8w8_args."""
+    a_t, b_t = _LAYOUTS[layout]
     m, k = a.shape
     n = b.shape[1]
     kb = _blocks(k)
-    args = _lib.Args8()
-    args.lda = _check_operand("A", a, a_t)
-    args.ldb = _check_operand("B", b, b_t)
-    args.a_block = _check_scale("a_scale", a_scale, m, kb, a.device)
-    args.b_block = _check_scale("b_scale (transposed)", b_scale.t(), n, kb, a.device)
-    args.a, args.b, args.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
-    args.a_scale, args.b_scale = a_scale.data_ptr(), b_scale.data_ptr()
-    args.bias = None if bias is None else bias.data_ptr()
-    args.m, args.n, args.k, args.ldo = m, n, k, n
-    args.sa_row, args.sa_kb = a_scale.stride()
-    args.sb_kb, args.sb_col = b_scale.stride()
-    args.a_trans, args.b_trans = int(a_t), int(b_t)
-    args.a_dtype, args.b_dtype = _F8_ID[a.dtype], _F8_ID[b.dtype]
-    args.out_dtype = _F_ID[out.dtype]
-    args.bias_dtype = 0 if bias is None else _F_ID[bias.dtype]
-    p = args.policy
-    p.tile_n, p.cta_group, p.split_k = pol["tile_n"], pol["cta_group"], pol["split_k"]
-    p.swap_ab, p.group_m = int(pol["swap_ab"]), pol.get("group_m", 0)
-    p.max_ctas, p.wait_limit_us = pol.get("max_ctas", 0), pol.get("wait_limit_us", 0)
-    p.no_pdl = 0 if pol.get("pdl", True) else 1
-    return args
-
-
-def _validate(a, a_scale, b, b_scale, layout):
-    layout = layout.lower()
-    if layout not in ("nn", "nt", "tn", "tt"):
-        raise ValueError(f"unsupported GEMM layout: {layout!r}; expected 'nn', 'nt', 'tn', or 'tt'")
-    assert a.ndim == 2 and b.ndim == 2
-    assert b.shape[0] == a.shape[1], f"A is {tuple(a.shape)}, B is {tuple(b.shape)}"
     if a.dtype not in _F8_ID or b.dtype not in _F8_ID:
         raise ValueError(f"gemm_a8w8 takes float8_e4m3fn or float8_e5m2 operands, got {a.dtype} and {b.dtype}")
-    assert a.device == b.device
-    assert b_scale.ndim == 2, f"b_scale has {b_scale.ndim} dimensions"
-    return layout[0] == "t", layout[1] == "t"
+    lda, ldb = _check_operand("A", a, a_t), _check_operand("B", b, b_t)
+    sa_rows, sa_kbs = a_scale.shape
+    sb_kbs, sb_cols = b_scale.shape
+    a_block = _check_scale("a_scale", a_scale, m, kb, sa_rows, sa_kbs)
+    b_block = _check_scale("b_scale", b_scale, n, kb, sb_cols, sb_kbs)
+    sa_row, sa_kb = a_scale.stride()
+    sb_kb, sb_col = b_scale.stride()
+    return _ARGS.pack(
+        a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), out_ptr, 0 if bias is None else bias.data_ptr(),
+        m, n, k, lda, ldb, n, sa_row, sa_kb, sb_col, sb_kb,
+        a_t, b_t, _F8_ID[a.dtype], _F8_ID[b.dtype], a_block, b_block, _F_ID[out_dtype], 0 if bias is None else _F_ID[bias.dtype],
+        *_policy(m, n, k, a_t, b_t, user_kwargs, num_sms), status)
+
+
+def _layout(layout: str) -> str:
+    low = layout.lower()
+    if low not in _LAYOUTS:
+        raise ValueError(f"unsupported GEMM layout: {layout!r}; expected 'nn', 'nt', 'tn', or 'tt'")
+    return low
 
 
 def gemm_a8w8(
@@ -210,19 +178,14 @@ def gemm_a8w8(
 
     user_kwargs: tile_n (16, 32, 64, 128; with cta_group 2: 128, 256), cta_group, split_k (K blocks of a tile over the CTAs of a
     cluster), swap_ab, group_m, max_ctas, pdl, wait_limit_us; without tile_n the tiling is chosen by `heuristic_a8w8`."""
-    key = None
-    if out is not None and a.is_cuda:
-        stream_ptr = (torch.cuda.current_stream(a.device) if stream is None else stream).cuda_stream
-        key = (_describe(a), _describe(a_scale), _describe(b), _describe(b_scale), _describe(out), _describe(bias),
-               tuple(sorted(user_kwargs.items())) if user_kwargs else (), stream_ptr, layout, out_dtype, a.get_device(),
-               a_scale.get_device(), b.get_device(), b_scale.get_device(), out.get_device())
-        if _launch_cached(key, stream_ptr):
-            return out.view(-1, b.shape[1])
-
-    a_t, b_t = _validate(a, a_scale, b, b_scale, layout)
+    layout = _layout(layout)
+    assert a.ndim == 2 and b.ndim == 2 and a_scale.ndim == 2 and b_scale.ndim == 2, "operands and scales are matrices"
     m, k = a.shape
     n = b.shape[1]
+    assert b.shape[0] == k, f"A is {tuple(a.shape)}, B is {tuple(b.shape)}"
     device = a.device
+    if b.device != device or a_scale.device != device or b_scale.device != device:
+        raise ValueError(f"operands and scales are on different devices: {device}, {b.device}, {a_scale.device}, {b_scale.device}")
     if out_dtype is None:
         out_dtype = torch.bfloat16 if out is None else out.dtype
     if out_dtype not in _F_ID:
@@ -231,66 +194,40 @@ def gemm_a8w8(
         if bias.dtype not in _F_ID:
             raise ValueError(f"unsupported bias dtype {bias.dtype}; expected float32, bfloat16 or float16")
         assert bias.ndim == 1 and bias.shape[0] == n and bias.device == device
-    out_in, bias_in = out, bias
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=device)
-    else:
+    if out is not None:
         assert out.dtype == out_dtype
         assert out.device == device
         assert out.is_contiguous()
         assert out.numel() == m * n, f"out has {out.numel()} elements, the product {m * n}"
-    out = out.view(m, n)
-    pol = _resolve(m, n, k, a_t, b_t, user_kwargs, _num_sms(device) if a.is_cuda else 148)
-    if m and n and k:
-        args = _fill_args(a, a_scale, b, b_scale, out, bias, a_t, b_t, pol)
-    assert a.is_cuda, "gemm_a8w8 runs on CUDA tensors only (there is no CPU path)"
-    if stream is None:
-        stream = torch.cuda.current_stream(device)
-    if m == 0 or n == 0:
-        return out
-    if k == 0:
-        with torch.cuda.stream(stream):
-            if bias is None:
-                out.zero_()
-            else:
-                out.copy_(bias.to(out.dtype).expand(m, n))
-        return out
-    args.status = _workspace_for(device, stream).status.data_ptr()
-    lib = _lib.load()
-    handle = C.c_void_p()
-    with torch.cuda.device(device):
-        rc = lib.b200_gemm_a8w8_prepare(C.byref(args), C.byref(handle))
-        if rc != 0:
-            raise RuntimeError(f"b200_gemm_a8w8_prepare failed ({rc}): {_lib.strerror(rc)}")
-        rc = lib.b200_gemm_a8w8_launch(handle, stream.cuda_stream)
+    if not a.is_cuda:
+        _arguments(a, a_scale, b, b_scale, 0, out_dtype, bias, layout, user_kwargs, 148, 0)
+        raise AssertionError("gemm_a8w8 runs on CUDA tensors only (there is no CPU path)")
+    index = device.index
+    with on_device(index, stream):
+        if out is None:
+            out = torch.empty((m, n), dtype=out_dtype, device=device)
+        elif out.shape != (m, n):
+            out = out.view(m, n)
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        if m == 0 or n == 0:
+            return out
+        if k == 0:
+            return out.zero_() if bias is None else out.copy_(bias.expand(m, n))
+        stream_ptr = raw_stream(index)
+        args = _arguments(a, a_scale, b, b_scale, out.data_ptr(), out_dtype, bias, layout, user_kwargs, device_sms(index),
+                          _workspace_for(device, stream_ptr).status_ptr)
+        rc = _lib.fast("b200_gemm_a8w8")(args, stream_ptr)
     if rc != 0:
-        lib.b200_gemm_a8w8_release(handle)
-        raise RuntimeError(f"b200_gemm_a8w8_launch failed ({rc}): {_lib.strerror(rc)}")
-    if key is not None and bias is bias_in and out_in is not None:
-        evicted = []
-        with _prepared_lock:
-            old = _prepared.pop(key, None)
-            if old is not None:
-                evicted.append(old)
-            _prepared[key] = (handle, a.get_device(), n)
-            while len(_prepared) > _PREPARED_MAX:
-                evicted.append(_prepared.popitem(last=False)[1])
-        for h, _, _ in evicted:
-            lib.b200_gemm_a8w8_release(h)
-    else:
-        lib.b200_gemm_a8w8_release(handle)
+        raise RuntimeError(f"b200_gemm_a8w8 failed ({rc}): {_lib.strerror(rc)}")
     return out
 
 
 def plan(a, a_scale, b, b_scale, layout="nt", user_kwargs: dict = {}, out_dtype=torch.bfloat16) -> dict:
     """What a call with these arguments would launch (tile, cluster split, grid, shared memory)."""
-    a_t, b_t = _validate(a, a_scale, b, b_scale, layout)
-    pol = _resolve(a.shape[0], b.shape[1], a.shape[1], a_t, b_t, user_kwargs, 148)
-    args = _fill_args(a, a_scale, b, b_scale, torch.empty(0, dtype=out_dtype), None, a_t, b_t, pol)
+    raw = _arguments(a, a_scale, b, b_scale, 0, out_dtype, None, _layout(layout), user_kwargs, 148, 0)
     pl = _lib.Plan()
-    rc = _lib.load().b200_gemm_a8w8_plan_query(C.byref(args), C.byref(pl))
+    rc = _lib.load().b200_gemm_a8w8_plan_query(C.byref(_lib.Args8.from_buffer_copy(raw)), C.byref(pl))
     if rc != 0:
         raise RuntimeError(f"b200_gemm_a8w8_plan_query failed ({rc}): {_lib.strerror(rc)}")
     return pl.as_dict()
@@ -299,9 +236,9 @@ def plan(a, a_scale, b, b_scale, layout="nt", user_kwargs: dict = {}, out_dtype=
 # --------------------------------------------------------------------------------------------------------- quantizer
 def _pitched(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
     """[rows, cols] with rows that start on 16-byte boundaries."""
-    pitch = -(-cols // 16) * 16
-    buf = torch.empty((rows, pitch), dtype=dtype, device=device)
-    return buf if pitch == cols else buf[:, :cols]
+    if cols % 16 == 0:
+        return torch.empty((rows, cols), dtype=dtype, device=device)
+    return torch.empty((rows, -(-cols // 16) * 16), dtype=dtype, device=device)[:, :cols]
 
 
 def _is_row_major(x: torch.Tensor) -> bool:
@@ -313,6 +250,7 @@ def _row_major(x: torch.Tensor) -> torch.Tensor:
     return x if _is_row_major(x) else x.contiguous()
 
 
+_QUANT_ARGS = struct.Struct("@P3q4i" + "PqP2q" * 2 + "Pq")  # b200_gemm_quantize_args
 _GROUPS = {"row": 1, "col": 2, "both": 3, "block": 4}
 
 
@@ -329,32 +267,31 @@ def _quantize(x, group, dtype, stream, want_colsum=False):
         raise ValueError(f"x must be row-major: expected stride(1) == 1; got shape={tuple(x.shape)} and stride={x.stride()}")
     assert x.is_cuda, "quantize_a8 runs on CUDA tensors only (there is no CPU path)"
     device = x.device
-    if stream is None:
-        stream = torch.cuda.current_stream(device)
+    index = device.index
     mode = _GROUPS[group]
-    args = _lib.QuantizeArgs()
-    args.x, args.rows, args.cols, args.ldx = x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols
-    args.in_dtype, args.out_dtype, args.mode = _F_ID[x.dtype], _F8_ID[dtype], mode
     got = []
-    with torch.cuda.device(device), torch.cuda.stream(stream):
+    row = col = (0, 0, 0, 0, 0)
+    sums = (0, 0)
+    with on_device(index, stream):
         if mode != 2:
             q = _pitched(rows, cols, dtype, device)
             # the product reads the scales of 128 rows at a time: rows are the contiguous dimension
-            s = torch.empty((_blocks(cols), _blocks(rows) if mode == 4 else rows), dtype=torch.float32, device=device).t()
-            args.q_row, args.ldq_row, args.s_row = q.data_ptr(), max(q.stride(0), cols), s.data_ptr()
-            args.sr_row, args.sr_group = s.stride()
-            got += [q, s]
-        if mode in (2, 3):
+            n_rows = _blocks(rows) if mode == 4 else rows
+            s = torch.empty((_blocks(cols), n_rows), dtype=torch.float32, device=device)
+            row = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), 1, n_rows)
+            got += [q, s.t()]
+        if mode == 2 or mode == 3:
             q = _pitched(rows, cols, dtype, device)
             s = torch.empty((_blocks(rows), cols), dtype=torch.float32, device=device)
-            args.q_col, args.ldq_col, args.s_col = q.data_ptr(), max(q.stride(0), cols), s.data_ptr()
-            args.sc_group, args.sc_col = s.stride()
+            col = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), cols, 1)
             got += [q, s]
         if want_colsum:
-            sums = torch.empty((_blocks(rows), -(-cols // 4) * 4), dtype=torch.float32, device=device)
-            args.colsum, args.colsum_ld = sums.data_ptr(), sums.shape[1]
-            got.append(sums)
-        rc = _lib.load().b200_gemm_quantize_a8(C.byref(args), stream.cuda_stream)
+            part = torch.empty((_blocks(rows), -(-cols // 4) * 4), dtype=torch.float32, device=device)
+            sums = (part.data_ptr(), part.shape[1])
+            got.append(part)
+        args = _QUANT_ARGS.pack(x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, _F_ID[x.dtype], _F8_ID[dtype], mode, 0,
+                                *row, *col, *sums)
+        rc = _lib.fast("b200_gemm_quantize_a8")(args, raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
     return tuple(got)
@@ -420,9 +357,10 @@ def _sum_rows(parts: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
     out = torch.empty(pitch, dtype=dtype, device=parts.device)
     if parts.shape[0] == 0:
         return out.zero_()[:n]
-    with torch.cuda.device(parts.device):
+    index = parts.get_device()
+    with on_device(index, None):
         rc = _lib.load().b200_gemm_reduce_slots(parts.data_ptr(), pitch, parts.shape[0], out.data_ptr(), None, 1, pitch, _F_ID[dtype], 0,
-                                                torch.cuda.current_stream(parts.device).cuda_stream)
+                                                raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"b200_gemm_reduce_slots failed ({rc}): {_lib.strerror(rc)}")
     return out[:n]

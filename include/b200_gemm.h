@@ -277,11 +277,6 @@ typedef struct b200_gemm_a8w8_args {
 int b200_gemm_a8w8(const b200_gemm_a8w8_args* args, void* cuda_stream);
 /* What the call would launch (fields of the 16-bit GEMM that have no meaning here are 0); no workspace is needed. */
 int b200_gemm_a8w8_plan_query(const b200_gemm_a8w8_args* args, b200_gemm_plan* plan);
-/* Plan once, launch many times: as b200_gemm_prepare / launch / release. */
-typedef struct b200_gemm_a8w8_handle b200_gemm_a8w8_handle;
-int b200_gemm_a8w8_prepare(const b200_gemm_a8w8_args* args, b200_gemm_a8w8_handle** handle);
-int b200_gemm_a8w8_launch(const b200_gemm_a8w8_handle* handle, void* cuda_stream);
-void b200_gemm_a8w8_release(b200_gemm_a8w8_handle* handle);
 
 /* The quantizer that makes such operands: x[rows, cols] (fp32, bf16 or fp16; columns contiguous, row stride ldx) in groups of
  * 128. The scale of a group is the smallest power of two, at least 2^-126, that brings its largest finite magnitude to the
@@ -336,11 +331,6 @@ typedef struct b200_gemm_moe_args {
 
 int b200_gemm_moe_a16w16(const b200_gemm_moe_args* args, void* cuda_stream);
 uint64_t b200_gemm_moe_workspace_bytes(const b200_gemm_moe_args* args); /* 0 for arguments that are refused */
-/* Plan once, launch many times: as b200_gemm_prepare / launch / release. */
-typedef struct b200_gemm_moe_handle b200_gemm_moe_handle;
-int b200_gemm_moe_prepare(const b200_gemm_moe_args* args, b200_gemm_moe_handle** handle);
-int b200_gemm_moe_launch(const b200_gemm_moe_handle* handle, void* cuda_stream);
-void b200_gemm_moe_release(b200_gemm_moe_handle* handle);
 
 /* Text for an error code; for B200_GEMM_ERR_LAUNCH the last CUDA error string seen by this thread. */
 const char* b200_gemm_strerror(int code);

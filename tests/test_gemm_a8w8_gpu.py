@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from flydsl_examples_b200.gemm_a16w16 import check_status
-from flydsl_examples_b200.gemm_a8w8 import clear_prepared_calls, gemm_a8w8, linear_a8w8, plan, quantize_a8
+from flydsl_examples_b200.gemm_a8w8 import gemm_a8w8, linear_a8w8, plan, quantize_a8
 
 pytestmark = pytest.mark.gpu
 
@@ -203,7 +203,6 @@ def test_other_stream_graph_and_two_callers():
     torch.cuda.synchronize()
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], want.flip(0))
     check_status()
-    clear_prepared_calls()
 
 
 # --------------------------------------------------------------------------------------------------------- quantizer

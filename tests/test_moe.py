@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from flydsl_examples_b200 import _lib
-from flydsl_examples_b200.moe_a16w16 import moe_a16w16
+from flydsl_examples_b200.moe_a16w16 import _ARGS, _scratch_bytes, moe_a16w16
 
 
 def args(**kw):
@@ -30,8 +30,7 @@ def test_entry_points_refuse_before_any_device_work():
         assert lib.b200_gemm_moe_workspace_bytes(C.byref(args(**bad))) == 0
     for bad in (dict(x=None), dict(logits=None), dict(w13=None), dict(w2=None), dict(out=None), dict(x=4104), dict(w13=4104), dict(w2=4098),
                 dict(out=4097), dict(logits=4098)):
-        h = C.c_void_p()
-        assert lib.b200_gemm_moe_prepare(C.byref(args(**bad)), C.byref(h)) == -1 and not h.value, bad
+        assert lib.b200_gemm_moe_a16w16(C.byref(args(**bad)), None) == -1, bad
     for big in (dict(tokens=65), dict(experts=513)):
         assert lib.b200_gemm_moe_a16w16(C.byref(args(**big)), None) == -7
     for ws in (dict(workspace=None), dict(workspace=4100), dict(workspace_bytes=4096)):
@@ -39,9 +38,11 @@ def test_entry_points_refuse_before_any_device_work():
     # a list of experts, and h for every expert that four tokens can choose
     assert lib.b200_gemm_moe_workspace_bytes(C.byref(args())) == 4096 + 8 * 4 * 32 * 2
     assert lib.b200_gemm_moe_workspace_bytes(C.byref(args(tokens=1))) == 4096 + 2 * 1 * 32 * 2
-    assert lib.b200_gemm_moe_a16w16(None, None) == -1 and lib.b200_gemm_moe_launch(None, None) == -1
-    assert lib.b200_gemm_moe_prepare(C.byref(args()), None) == -1
-    lib.b200_gemm_moe_release(None)
+    assert lib.b200_gemm_moe_a16w16(None, None) == -1
+    for t, i, e, k in ((4, 32, 8, 2), (1, 32, 8, 2), (64, 2048, 512, 16)):  # the Python call's own sum
+        assert _scratch_bytes(t, i, e, k) == lib.b200_gemm_moe_workspace_bytes(C.byref(args(
+            tokens=t, inner=i, w2_row=i, w2_expert=64 * i, w13_expert=128 * i, experts=e, top_k=k)))
+    assert _ARGS.size == C.sizeof(_lib.MoeArgs)
 
 
 def test_structure_matches_the_header(tmp_path):

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from flydsl_examples_b200.gemm_a16w16 import check_status, gemm_a16w16
-from flydsl_examples_b200.moe_a16w16 import clear_prepared_calls, moe_a16w16
+from flydsl_examples_b200.moe_a16w16 import moe_a16w16
 
 pytestmark = pytest.mark.gpu
 
@@ -210,7 +210,6 @@ def test_repeats_streams_and_two_graphs():
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want.flip(0)) and torch.equal(out, want)
     check_status()
-    clear_prepared_calls()
 
 
 def test_growing_workspace_and_no_tokens():
