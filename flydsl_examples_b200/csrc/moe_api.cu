@@ -1,6 +1,7 @@
 // Host side of the few-token mixture-of-experts layer (b200_gemm_moe_* in include/b200_gemm.h): validation, tensor maps, the two
 // launches. No device allocation, no synchronisation.
 #include <cstring>
+#include <mutex>
 
 #include "../../include/b200_gemm.h"
 #include "host.h"
@@ -13,13 +14,16 @@ struct MoeVariant {
   MoeFn up, down;
   int up_smem, down_smem, cols;
 };
-template <int TN, int STAGES>
+template <int TN, int UP_STAGES, int DOWN_STAGES>
 static MoeVariant moe_make() {
-  static_assert(SmemMoe<TN, STAGES, true>::kDynBytes <= 227 * 1024 && SmemMoe<TN, STAGES, false>::kDynBytes <= 227 * 1024, "shared memory");
-  return {moe_a16w16_sm100_kernel<TN, STAGES, true>, moe_a16w16_sm100_kernel<TN, STAGES, false>, SmemMoe<TN, STAGES, true>::kDynBytes,
-          SmemMoe<TN, STAGES, false>::kDynBytes, TN};
+  using Up = SmemMoe<TN, UP_STAGES, true>;
+  using Down = SmemMoe<TN, DOWN_STAGES, false>;
+  static_assert(Up::kDynBytes <= 227 * 1024 && Down::kDynBytes <= 227 * 1024, "shared memory");
+  return {moe_a16w16_sm100_kernel<TN, UP_STAGES, true>, moe_a16w16_sm100_kernel<TN, DOWN_STAGES, false>, Up::kDynBytes, Down::kDynBytes, TN};
 }
-static MoeVariant moe_variant(int64_t t) { return t <= 16 ? moe_make<16, 5>() : t <= 32 ? moe_make<32, 5>() : moe_make<64, 4>(); }
+static MoeVariant moe_variant(int64_t t) {
+  return t <= 16 ? moe_make<16, 5, 5>() : t <= 32 ? moe_make<32, 5, 4>() : moe_make<64, 4, 3>();
+}
 
 constexpr uint64_t kMoeListBytes = 4096;  // the list of chosen experts at the start of the scratch
 
@@ -62,6 +66,30 @@ struct MoeCall {
   int grid_up, grid_down, pdl;
 };
 
+// Clusters of `size` CTAs of the second kernel that the device holds at once; asked once for each kernel and size.
+static int max_clusters(const MoeVariant& var, int size, int dev) {
+  static std::mutex mutex;
+  static int known[kMaxDevices][3][17];  // 0: not asked yet
+  int& n = known[dev][var.cols == 16 ? 0 : var.cols == 32 ? 1 : 2][size];
+  std::lock_guard<std::mutex> lock(mutex);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(size, 1, 1), cfg.blockDim = dim3(kMoeThreads, 1, 1), cfg.dynamicSmemBytes = var.down_smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, reinterpret_cast<const void*>(var.down), &cfg) != cudaSuccess) {
+      cudaGetLastError();  // not a launch error: this size is not used
+      got = 0;
+    }
+    n = got > 0 ? got : -1;
+  }
+  return n;
+}
+
 static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   int rc = moe_check(a);
   if (rc) return rc;
@@ -77,13 +105,12 @@ static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   memset(h, 0, sizeof(*h));
   h->var = moe_variant(a->tokens);
   const int cols = h->var.cols;
-  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   MoeParams& u = h->up;
   u.logits = a->logits, u.logits_row = a->logits_row, u.logits_col = a->logits_col, u.logits_dtype = a->logits_dtype;
   u.T = (int)a->tokens, u.E = (int)a->experts, u.H = (int)a->hidden, u.I = (int)a->inner, u.top_k = a->top_k, u.renorm = a->renormalize ? 1 : 0;
   u.dtype = a->dtype;
-  u.active = reinterpret_cast<int*>(ws);
-  u.h = reinterpret_cast<uint16_t*>(ws + kMoeListBytes);
+  u.list = static_cast<int*>(a->workspace);
+  u.h = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a->workspace) + kMoeListBytes);
   u.out = a->out, u.ldo = a->ldo;
   u.status = a->status;
   u.wait_limit_ns = a->wait_limit_us > 0 ? (unsigned long long)a->wait_limit_us * 1000ull : kWaitLimitNs;
@@ -101,15 +128,21 @@ static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
 
   const int64_t units = slots * ((a->inner + 63) / 64);
   h->grid_up = (int)(units < sms ? units : sms);
-  // the down product's K axis over as many CTAs of a cluster as keep the grid within the SMs; each finishes some columns
-  const int64_t row_tiles = (a->hidden + 127) / 128;
-  int s = 1;
-  while (s < 16 && s * 2 <= cols && row_tiles * s * 2 <= sms && s * 2 <= slots * ((a->inner + kMoeTK - 1) / kMoeTK)) s *= 2;
-  h->down.cluster_split = s;
-  h->grid_down = (int)(row_tiles * s);
-  h->pdl = a->no_pdl ? 0 : 1;
   rc = allow_launch(reinterpret_cast<const void*>(h->var.up), h->var.up_smem, dev);
-  return rc ? rc : allow_launch(reinterpret_cast<const void*>(h->var.down), h->var.down_smem, dev);
+  if (!rc) rc = allow_launch(reinterpret_cast<const void*>(h->var.down), h->var.down_smem, dev);
+  if (rc) return rc;
+  // The down product's K axis goes over the CTAs of clusters, as large as still fit the GPU all at once (how many do depends
+  // on how its SMs are grouped: 16 clusters of 8 have been seen to take two turns); no CTA without a K block or a token's
+  // column to finish.
+  const int row_tiles = (int)((a->hidden + 127) / 128);
+  const int64_t blocks = slots * ((a->inner + kMoeTK - 1) / kMoeTK);
+  int s = 16;
+  if (s > blocks) s = (int)blocks;
+  while (s > 1 && (row_tiles * s > sms || max_clusters(h->var, s, dev) < row_tiles)) --s;
+  h->down.cluster_split = s;
+  h->grid_down = row_tiles * s;
+  h->pdl = a->no_pdl ? 0 : 1;
+  return 0;
 }
 
 static int moe_run(const MoeCall* h, cudaStream_t stream) {

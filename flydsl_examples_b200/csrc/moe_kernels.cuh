@@ -8,10 +8,13 @@
 //  * Weights sit on the 128-row side of tcgen05.mma, tokens on its N axis (16, 32 or 64 columns). All tokens take part in
 //    every expert's product and the epilogue keeps the pairs that the router chose: no gather, and the tensor core has
 //    the time (64 columns need a quarter of what the weights' bytes take).
-//  * First kernel: every block routes for itself (a warp per token, top_k rounds of a warp-wide maximum; the logits are a
-//    few kilobytes), so no launch and no pass of its own. A tile is 64 gate rows over 64 up rows of one expert; its
-//    epilogue writes h[slot][t][i] = round16(p * silu(gate) * up), zero for pairs that were not chosen. The weight of the
-//    pair is folded in before the one rounding that the second product's 16-bit operand needs.
+//  * Every block of the first kernel routes for itself (the logits are a few kilobytes), so routing has no launch and no pass
+//    of its own; the list of chosen experts goes to the second kernel. (The second kernel routing again, in order to fill
+//    its ring with weights while the first one's last tiles run, took 26.2 instead of 24.4 us for one token of 8 / 128
+//    experts, 169 instead of 171 us for 8 tokens of 2 / 16: its blocks mostly start when the first kernel's end.)
+//  * First kernel: a tile is 64 gate rows over 64 up rows of one expert; its epilogue writes h[slot][t][i] =
+//    round16(p * silu(gate) * up), zero for pairs that were not chosen. The weight of the pair is folded in before the one
+//    rounding that the second product's 16-bit operand needs.
 //  * Second kernel: the sum over experts is the K axis of one product, y[h, t] = sum over (slot, i) of W2 * h, accumulated
 //    in TMEM. K is cut into contiguous spans over the CTAs of a cluster, which add up through distributed shared
 //    memory in rank order: no atomics, the same bits every time.
@@ -24,7 +27,7 @@
 
 namespace b200 {
 
-constexpr int kMoeThreads = 192;  // warp 0 TMA producer, warp 1 TMEM and MMA, warps 2-5 epilogue
+constexpr int kMoeThreads = 384;  // warp 0 TMA producer, warp 1 TMEM and MMA, warps 2-5 epilogue; 6-11 only help to route
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
 constexpr int kMoeTK = 128;       // K elements per stage: two 64-element swizzle spans
 constexpr int kMoeUBytes = 128 * kMoeTK * 2;
@@ -38,7 +41,7 @@ struct alignas(64) MoeParams {
   int T, E, H, I, top_k, renorm;
   int dtype;         // 2 bf16, 3 fp16
   uint16_t* h;       // [slot][T][I]
-  int* active;       // [0] = number of experts chosen by any token, then their indices in increasing order
+  int* list;         // [0] = number of experts that a token chose, [16..] = their indices in increasing order
   void* out;
   long long ldo;
   int cluster_split;
@@ -51,13 +54,16 @@ template <int TN, int STAGES, bool UP>
 struct SmemMoe {
   static constexpr int kVBox = TN * 128;
   static constexpr int kStageBytes = kMoeUBytes + 2 * kVBox;
-  static constexpr int kXOff = STAGES * kStageBytes;                 // UP: the up half's sums [TN][64]; otherwise recv[src][col][128]
-  static constexpr int kXBytes = UP ? TN * 64 * 4 : TN * 128 * 4;
-  static constexpr int kRouteOff = kXOff + kXBytes;                  // ids, weights [64][16]; active list; weights of one expert
-  static constexpr int kRouteBytes = UP ? kMoeMaxTokens * kMoeMaxTopK * 8 + (kMoeMaxExperts + 16 + kMoeMaxExperts / 32 + kMoeMaxTokens) * 4 : 0;
+  static constexpr int kXOff = STAGES * kStageBytes;                 // UP: the up half's sums [TN][64]; otherwise recv[t / S][source][128], t / S <= (TN - 1) / S
+  static constexpr int kXBytes = UP ? TN * 64 * 4 : (TN + 15) * 128 * 4;
+  static constexpr int kRouteOff = kXOff + kXBytes;
+  // the list of experts; first kernel: their bits, one expert's weights, and ids and weights [TN][16]
+  static constexpr int kPairs = TN * kMoeMaxTopK;
+  static constexpr int kRouteBytes = (kMoeMaxExperts + 16) * 4 + (UP ? (kMoeMaxExperts / 32 + kMoeMaxTokens) * 4 + kPairs * 8 : 0);
   static constexpr int kBarOff = (kRouteOff + kRouteBytes + 7) / 8 * 8;
   static constexpr int kMiscOff = kBarOff + (2 * STAGES + 4) * 8;
   static constexpr int kTotal = kMiscOff + 16;
+  static_assert(!UP || STAGES * kStageBytes >= TN * (kMoeMaxExperts + 4) * 4, "the ring holds all logits while routing");
   static constexpr int kDynBytes = kTotal + 1024;
 };
 
@@ -71,73 +77,135 @@ __device__ __forceinline__ void report_abort_moe(int* status, int role, int unit
 
 // Order-preserving integer of a logit; NaN above everything, the two zeros alike.
 __device__ __forceinline__ uint32_t logit_key(float f) {
-  if (f != f) return 0xffffffffu;
+  if (f != f) return 0xfffffffeu;  // one below the largest integer: ranks add 1 to keys
   const uint32_t b = __float_as_uint(f + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ float load_logit(const MoeParams& p, int t, int e) {
-  const long long i = (long long)t * p.logits_row + (long long)e * p.logits_col;
-  if (p.logits_dtype == 1) return reinterpret_cast<const float*>(p.logits)[i];
-  if (p.logits_dtype == 2) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.logits)[i]);
-  return __half2float(reinterpret_cast<const __half*>(p.logits)[i]);
+__device__ __forceinline__ float logit_of_key(uint32_t k) {
+  return k == 0xfffffffeu ? __uint_as_float(0x7fffffffu) : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// One warp routes token t: ids[0..top_k), weights[0..top_k) (a weight of zero: not chosen), and the experts' bits in `mask`.
-__device__ __forceinline__ void route_token(const MoeParams& p, int t, int lane, int* ids, float* weights, uint32_t* mask) {
-  constexpr int kPer = kMoeMaxExperts / 32;
-  uint32_t key[kPer];  // 0: no expert, or taken already (no logit maps to 0)
-  float top = -INFINITY, total = 0.f;
+// Logits as keys into shared memory; 0 marks no expert, or one taken already (no logit maps to 0). Four loads of a thread travel
+// together: one by one, each costs an L2 round trip of 0.4 us.
+template <typename T>
+__device__ __forceinline__ void stage_logits(const MoeParams& p, const T* logits, uint32_t* keys, int e4, int stride) {
+  const int total = p.T * e4;
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < total; i0 += 4 * kMoeThreads) {
+    T raw[4];
+    int at[4];
+    bool in[4];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    key[j] = 0;
-    if (j * 32 < p.E) {
-      const int e = j * 32 + lane;
-      if (e < p.E) key[j] = logit_key(load_logit(p, t, e));
+    for (int n = 0; n < 4; ++n) {
+      const int i = i0 + n * kMoeThreads, t = i / e4, e = i - t * e4;
+      at[n] = i < total ? t * stride + e : -1;
+      in[n] = i < total && e < p.E;
+      raw[n] = logits[in[n] ? t * p.logits_row + e * p.logits_col : 0];
     }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (at[n] >= 0) keys[at[n]] = in[n] ? logit_key((float)raw[n]) : 0u;
   }
-  auto value = [](uint32_t k) {  // the logit of a key
-    return k == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-  };
-  float mine = 0.f;  // lane r holds the r-th chosen logit and index
-  int my_id = 0;
-  for (int r = 0; r < p.top_k; ++r) {
-    uint32_t best = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (j * 32 < p.E) best = max(best, key[j]);
-    best = __reduce_max_sync(0xffffffffu, best);
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int j = kPer - 1; j >= 0; --j)
-      if (j * 32 < p.E && key[j] == best) at = j * 32 + lane;
-    at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
-    if (r == 0) {
-      top = value(best);
-      if (!p.renorm) {  // the softmax's sum over all experts
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (j * 32 + lane < p.E) total += expf(value(key[j]) - top);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+}
+
+// The whole block routes all tokens: ids[t][r], weights[t][r] for r < top_k (-1 and zero: not chosen), the chosen experts' bits
+// in `mask`. `keys` is scratch for T * stride integers.
+//
+// This code runs once per launch and its instructions come from L2 meanwhile, about 30 cycles each by the counters, so it is
+// written for few instructions and not for few cycles: logits as ordered integers in shared memory, rolled loops. (With
+// logits in unrolled registers routing took 3 us for one token and 16 us for 64, with them it takes XX and XX.)
+__device__ __forceinline__ void route_all(const MoeParams& p, uint32_t* keys, int* ids, float* weights, uint32_t* mask) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int e4 = (p.E + 3) & ~3, stride = e4 + 4;  // rows of 16-byte pieces, on different banks
+  if (p.logits_dtype == 1)
+    stage_logits(p, reinterpret_cast<const float*>(p.logits), keys, e4, stride);
+  else if (p.logits_dtype == 2)
+    stage_logits(p, reinterpret_cast<const __nv_bfloat16*>(p.logits), keys, e4, stride);
+  else
+    stage_logits(p, reinterpret_cast<const __half*>(p.logits), keys, e4, stride);
+  __syncthreads();
+  const int G = p.E <= 128 ? 4 : 16;  // lanes to a token where tokens share warps
+  if (p.T * p.E <= kMoeThreads && p.E <= 128) {
+    // A thread per (token, expert): its rank is the number of experts ahead of it (larger, or equal with a lower index).
+    const int t = tid / p.E, e = tid - t * p.E;
+    uint32_t* row = keys + t * stride;
+    int rank = p.top_k;
+    if (t < p.T) {
+      const uint32_t mine = row[e];
+      rank = 0;
+#pragma unroll 2
+      for (int o = 0; o < e4; o += 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(row + o);
+        rank += (k.x + (o < e) > mine) + (k.y + (o + 1 < e) > mine) + (k.z + (o + 2 < e) > mine) + (k.w + (o + 3 < e) > mine);
+      }
+      if (rank < p.top_k) {
+        ids[t * kMoeMaxTopK + rank] = e;
+        weights[t * kMoeMaxTopK + rank] = logit_of_key(mine);
       }
     }
-    if (lane == r) mine = value(best), my_id = at;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (j * 32 + lane == at) key[j] = 0;
+    __syncthreads();
+    if (rank < p.top_k) row[e] = 0;
+  } else {
+    // More pairs of experts than threads to compare them: top_k rounds per token, each taking out the largest.
+    const int sub = lane & (G - 1);
+#pragma unroll 1
+    for (int t0 = 0; t0 < p.T; t0 += kMoeThreads / G) {
+      const int t = t0 + tid / G;
+      uint32_t* row = keys + min(t, p.T - 1) * stride;
+#pragma unroll 1
+      for (int r = 0; r < p.top_k; ++r) {
+        uint32_t best = 0;
+        int at = 0x7fffffff;
+#pragma unroll 2
+        for (int e = 4 * sub; e < e4; e += 4 * G) {
+          const uint4 k = *reinterpret_cast<const uint4*>(row + e);
+          if (k.x > best) best = k.x, at = e;
+          if (k.y > best) best = k.y, at = e + 1;
+          if (k.z > best) best = k.z, at = e + 2;
+          if (k.w > best) best = k.w, at = e + 3;
+        }
+        for (int o = G >> 1; o > 0; o >>= 1) {
+          const uint32_t k2 = __shfl_xor_sync(0xffffffffu, best, o);
+          const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+          if (k2 > best || (k2 == best && a2 < at)) best = k2, at = a2;
+        }
+        __syncwarp();
+        if (t < p.T && sub == 0) {
+          row[at] = 0;
+          ids[t * kMoeMaxTopK + r] = at;
+          weights[t * kMoeMaxTopK + r] = logit_of_key(best);
+        }
+        __syncwarp();
+      }
+    }
   }
-  float w = lane < p.top_k ? expf(mine - top) : 0.f;
-  if (p.renorm) {
-    total = w;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  w = top == -INFINITY ? 0.f : w / total;  // a token whose logits are all -inf goes nowhere
-  if (lane < p.top_k) {
-    ids[lane] = w == 0.f ? -1 : my_id;
-    weights[lane] = w;
-    if (w != 0.f) atomicOr(mask + (my_id >> 5), 1u << (my_id & 31));
+  __syncthreads();
+  // softmax over the chosen logits, with the others' share of the sum unless the weights are renormalised
+  const int WG = p.T <= kMoeThreads / 32 ? 32 : G, sub = lane & (WG - 1);
+#pragma unroll 1
+  for (int t0 = 0; t0 < p.T; t0 += kMoeThreads / WG) {
+    const int t = t0 + tid / WG, at = min(t, p.T - 1);
+    int* id = ids + at * kMoeMaxTopK;
+    float* weight = weights + at * kMoeMaxTopK;
+    const float top = weight[0];
+    float total = 0.f;
+    if (!p.renorm)
+      for (int e = sub; e < p.E; e += WG)
+        if (keys[at * stride + e] != 0) total += expf(logit_of_key(keys[at * stride + e]) - top);
+    for (int r = sub; r < p.top_k; r += WG) total += expf(weight[r] - top);
+    for (int o = WG >> 1; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    __syncwarp();  // every lane has read weight[0]
+    if (t < p.T)
+      for (int r = sub; r < p.top_k; r += WG) {
+        // a token whose logits are all -inf goes nowhere
+        const float w = top == -INFINITY ? 0.f : expf(weight[r] - top) / total;
+        weight[r] = w;
+        if (w != 0.f)
+          atomicOr(mask + (id[r] >> 5), 1u << (id[r] & 31));
+        else
+          id[r] = -1;
+      }
   }
 }
 
@@ -158,11 +226,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
   volatile uint32_t* tmem_ptr_s = reinterpret_cast<volatile uint32_t*>(sm + L::kMiscOff);
   volatile int* abort_s = reinterpret_cast<volatile int*>(sm + L::kMiscOff + 4);
   volatile int* epi_abort_s = reinterpret_cast<volatile int*>(sm + L::kMiscOff + 8);
-  int* ids = reinterpret_cast<int*>(sm + L::kRouteOff);
-  float* weights = reinterpret_cast<float*>(ids + kMoeMaxTokens * kMoeMaxTopK);
-  int* list = reinterpret_cast<int*>(weights + kMoeMaxTokens * kMoeMaxTopK);  // [0] = count, [16..] = experts
+  int* list = reinterpret_cast<int*>(sm + L::kRouteOff);  // [0] = number of experts that a token chose, [16..] = their indices
   uint32_t* mask = reinterpret_cast<uint32_t*>(list + 16 + kMoeMaxExperts);
   float* pair_w = reinterpret_cast<float*>(mask + kMoeMaxExperts / 32);
+  int* ids = reinterpret_cast<int*>(pair_w + kMoeMaxTokens);
+  float* weights = reinterpret_cast<float*>(ids + L::kPairs);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool cluster_mode = !UP && p.cluster_split > 1;
@@ -197,40 +265,38 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
   }
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr_s;
+  // The logits are on the critical path and often no longer (or not yet) in L2: ask for them ahead of the wait. L2 is where
+  // all writes meet, so a line that is written after this is still read right.
+  if (UP && blockIdx.x == 0) {
+    const int es = p.logits_dtype == 1 ? 4 : 2;
+    for (int i = threadIdx.x; i < p.T * ((p.E * es + 127) / 128 + 1); i += kMoeThreads) {
+      const int t = i % p.T, e = min((i / p.T) * (128 / es), p.E - 1);
+      prefetch_l2(reinterpret_cast<const char*>(p.logits) + ((long long)t * p.logits_row + (long long)e * p.logits_col) * es);
+    }
+  }
   grid_dependency_wait();
   grid_launch_dependents();
-
-  int n_active;
-  const int* experts;
   if constexpr (UP) {
-    for (int t = warp; t < p.T; t += kMoeThreads / 32) route_token(p, t, lane, ids + t * kMoeMaxTopK, weights + t * kMoeMaxTopK, mask);
+    route_all(p, reinterpret_cast<uint32_t*>(sm), ids, weights, mask);  // the ring is free until the first load
+    fence_proxy_async_smem();
     __syncthreads();
-    if (warp == 0) {  // the chosen experts in increasing order
-      uint32_t m = lane < kMoeMaxExperts / 32 ? mask[lane] : 0;
-      int before = __popc(m);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-      }
-      if (lane == 31) list[0] = before;
-      int at = before - __popc(m);
-      while (m) {
-        list[16 + at++] = lane * 32 + __ffs(m) - 1;
-        m &= m - 1;
-      }
+    // the chosen experts in increasing order
+    for (int e = threadIdx.x; e < kMoeMaxExperts; e += kMoeThreads) {
+      const int w = e >> 5;
+      int at = __popc(mask[w] & ((1u << (e & 31)) - 1u));
+      for (int j = 0; j < w; ++j) at += __popc(mask[j]);
+      if (mask[w] >> (e & 31) & 1u) list[16 + at] = e;
+      if (e == kMoeMaxExperts - 1) list[0] = at + (int)(mask[w] >> 31);
     }
     __syncthreads();
-    n_active = list[0];
-    experts = list + 16;
-    if (blockIdx.x == 0) {  // for the second kernel
-      for (int i = threadIdx.x; i < n_active; i += kMoeThreads) p.active[16 + i] = experts[i];
-      if (threadIdx.x == 0) p.active[0] = n_active;
-    }
+    if (blockIdx.x == 0)  // for the second kernel
+      for (int i = threadIdx.x; i < 16 + list[0]; i += kMoeThreads) p.list[i] = list[i];
   } else {
-    n_active = *reinterpret_cast<volatile int*>(p.active);
-    experts = p.active + 16;
+    for (int i = threadIdx.x; i < 16 + min(p.E, p.T * p.top_k); i += kMoeThreads) list[i] = p.list[i];
+    __syncthreads();
   }
+  const int n_active = list[0];
+  const int* experts = list + 16;
 
   // UP: unit = (slot, 64 gate rows), K = H. Otherwise one unit per CTA: 128 rows of H, a span of the K axis (slot, I).
   const int k_blocks = UP ? (p.H + kMoeTK - 1) / kMoeTK : (p.I + kMoeTK - 1) / kMoeTK;
@@ -250,15 +316,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
 #pragma unroll 1
     for (int u = u_first; ok && u < u_end; u += u_step) {
       const int slot0 = UP ? u / tiles : 0, i0 = UP ? (u - slot0 * tiles) * 64 : 0;
-      int expert = UP ? experts[slot0] : 0, slot = UP ? slot0 : -1;
 #pragma unroll 1
       for (int b = b_first; b < b_end; ++b) {
-        int kb = b;
-        if constexpr (!UP) {
-          const int s = b / k_blocks;
-          kb = b - s * k_blocks;
-          if (s != slot) slot = s, expert = experts[s];
-        }
         if (issued >= STAGES) {
           int good = 1;
           if (lane == 0) good = mbar_wait(empty_bar(stage), phase ^ 1u, abort_s, p.wait_limit_ns) ? 1 : 0;
@@ -270,8 +329,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
           }
         }
         if (elect_one()) {
-          const uint32_t fb = full_bar(stage);
-          const uint32_t su = base + stage * L::kStageBytes, sv = su + kMoeUBytes;
+          const uint32_t fb = full_bar(stage), su = base + stage * L::kStageBytes, sv = su + kMoeUBytes;
+          const int s = UP ? slot0 : b / k_blocks, kb = UP ? b : b - s * k_blocks;
+          const int expert = experts[s];
           mbar_arrive_expect_tx(fb, L::kStageBytes);
 #pragma unroll
           for (int sub = 0; sub < 2; ++sub) {
@@ -282,7 +342,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
               tma_load_2d(sv + sub * L::kVBox, &p.tmap_v, k0, 0, fb);
             } else {
               tma_load_3d(su + sub * 16384, &p.tmap_u, k0, row_tile * 128, expert, fb);
-              tma_load_3d(sv + sub * L::kVBox, &p.tmap_v, k0, 0, slot, fb);
+              tma_load_3d(sv + sub * L::kVBox, &p.tmap_v, k0, 0, s, fb);
             }
           }
         }
@@ -340,7 +400,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
         if (++stage == STAGES) stage = 0, phase ^= 1u;
       }
     }
-  } else {
+  } else if (warp < 6) {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
     const int quarter = warp & 3, row = quarter * 32 + lane, et = threadIdx.x - 64;
     float* xs = reinterpret_cast<float*>(sm + L::kXOff);
@@ -388,21 +448,25 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
         for (int i = 0; i < TN; ++i) v[i] = 0.f;
       }
       if constexpr (UP) {
-        // lanes 64..127 hold the up rows of the gate rows in lanes 0..63
-        if (row >= 64) {
+        // Lanes 64..127 hold the up rows of the gate rows in lanes 0..63: the halves swap sums through shared memory, so that
+        // the first finishes the first half of the tokens and the second the others.
+        const bool is_gate = row < 64;
+        const int r64 = row & 63;
 #pragma unroll
-          for (int t = 0; t < TN; ++t) xs[t * 64 + row - 64] = v[t];
-        }
+        for (int t = 0; t < TN; ++t)
+          if ((t < TN / 2) != is_gate) xs[t * 64 + r64] = v[t];
         named_bar_sync(2, 128);
-        const int i = (u - slot * tiles) * 64 + row;
-        if (row < 64 && i < p.I) {
+        const int i = (u - slot * tiles) * 64 + r64;
+        if (i < p.I) {
           uint16_t* dst = p.h + ((size_t)slot * p.T) * p.I + i;
 #pragma unroll
-          for (int t = 0; t < TN; ++t) {
+          for (int j = 0; j < TN / 2; ++j) {
+            const int t = is_gate ? j : TN / 2 + j;
             if (t < p.T) {
-              const float w = pair_w[t], g = v[t];
+              const float w = pair_w[t], other = xs[t * 64 + r64], own = is_gate ? v[j] : v[TN / 2 + j];
+              const float g = is_gate ? own : other, up = is_gate ? other : own;
               // a pair that was not chosen is zero whatever its sums are
-              const float a = w == 0.f ? 0.f : w * (g / (1.f + __expf(-g))) * xs[t * 64 + row];
+              const float a = w == 0.f ? 0.f : w * __fdividef(g, 1.f + __expf(-g)) * up;
               uint16_t bits;
               if (p.dtype == 2) {
                 const __nv_bfloat16 h = __float2bfloat16_rn(a);
@@ -417,17 +481,20 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
         }
         named_bar_sync(1, 128);  // xs and pair_w may be rewritten
       } else if (cluster_mode) {
-        // Column t belongs to CTA t / (TN / S): a warp's 32 rows are 128 contiguous bytes of recv[source][own column][row].
+        // Column t belongs to CTA t % S: a warp's 32 rows are 128 contiguous bytes of recv[t / S][source][row].
         if (cluster_wait_due) {
           cluster_wait();
           cluster_wait_due = false;
         }
-        const int own_log2 = __ffs(TN / S) - 1;
         const uint32_t recv = base + L::kXOff + (uint32_t)row * 4u;
+        int slab = 0, owner = 0;
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
-          const uint32_t dst = mapa_cluster(recv + (uint32_t)(((rank << own_log2) + (t & ((1 << own_log2) - 1))) * 128) * 4u, (uint32_t)(t >> own_log2));
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v[t]) : "memory");
+          if (t < p.T) {
+            const uint32_t dst = mapa_cluster(recv + (uint32_t)((slab + rank) * 128) * 4u, (uint32_t)owner);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v[t]) : "memory");
+            if (++owner == S) owner = 0, slab += S;
+          }
         }
       } else {
         const int hrow = row_tile * 128 + row;
@@ -452,15 +519,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
   if (cluster_mode) {
     cluster_arrive();
     cluster_wait();
-    if (warp >= 2) {
-      const int own = TN / S, row = threadIdx.x - 64, hrow = row_tile * 128 + row;
+    if (warp >= 2 && warp < 6) {
+      const int row = threadIdx.x - 64, hrow = row_tile * 128 + row;
       const float* recv = reinterpret_cast<const float*>(sm + L::kXOff) + row;
       if (hrow < p.H) {
-        for (int c = 0; c < own; ++c) {
-          const int t = rank * own + c;
-          if (t >= p.T) break;
+        for (int t = rank; t < p.T; t += S, recv += S * 128) {
           float x = 0.f;
-          for (int src = 0; src < S; ++src) x += recv[(src * own + c) * 128];
+          for (int src = 0; src < S; ++src) x += recv[src * 128];  // in rank order
           if (p.dtype == 2)
             reinterpret_cast<__nv_bfloat16*>(p.out)[(long long)t * p.ldo + hrow] = __float2bfloat16_rn(x);
           else

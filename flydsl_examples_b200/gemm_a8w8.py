@@ -205,7 +205,7 @@ def gemm_a8w8(
     index = device.index
     with on_device(index, stream):
         if out is None:
-            out = torch.empty((m, n), dtype=out_dtype, device=device)
+            out = torch.empty(m, n, dtype=out_dtype, device=device)
         elif out.shape != (m, n):
             out = out.view(m, n)
         if bias is not None and not bias.is_contiguous():
@@ -237,8 +237,8 @@ def plan(a, a_scale, b, b_scale, layout="nt", user_kwargs: dict = {}, out_dtype=
 def _pitched(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
     """[rows, cols] with rows that start on 16-byte boundaries."""
     if cols % 16 == 0:
-        return torch.empty((rows, cols), dtype=dtype, device=device)
-    return torch.empty((rows, -(-cols // 16) * 16), dtype=dtype, device=device)[:, :cols]
+        return torch.empty(rows, cols, dtype=dtype, device=device)
+    return torch.empty(rows, -(-cols // 16) * 16, dtype=dtype, device=device)[:, :cols]
 
 
 def _is_row_major(x: torch.Tensor) -> bool:
@@ -277,12 +277,12 @@ def _quantize(x, group, dtype, stream, want_colsum=False):
             q = _pitched(rows, cols, dtype, device)
             # the product reads the scales of 128 rows at a time: rows are the contiguous dimension
             n_rows = _blocks(rows) if mode == 4 else rows
-            s = torch.empty((_blocks(cols), n_rows), dtype=torch.float32, device=device)
+            s = torch.empty_strided((n_rows, _blocks(cols)), (1, n_rows), dtype=torch.float32, device=device)
             row = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), 1, n_rows)
-            got += [q, s.t()]
+            got += [q, s]
         if mode == 2 or mode == 3:
             q = _pitched(rows, cols, dtype, device)
-            s = torch.empty((_blocks(rows), cols), dtype=torch.float32, device=device)
+            s = torch.empty(_blocks(rows), cols, dtype=torch.float32, device=device)
             col = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), cols, 1)
             got += [q, s]
         if want_colsum:
