@@ -43,8 +43,7 @@ def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: boo
 
     Up to 64 rows of A the product streams the weights: B takes the 128-row side (swap_ab), the tokens fill a tile of 16 to
     64 columns, and a cluster splits K until the CTAs fill the SMs. Above that the time of a call is taken as whole waves
-    times the cycles of a K block (the longer of the tensor time and the operands' way into the SM at 64 bytes a cycle),
-    and the cheapest of the tiles is used."""
+    times the measured cycles of a K block, and the cheapest of the tiles is used."""
     kb = _blocks(k)
     if m <= 64 and not a_transposed:
         tile = 16 if m <= 16 else 32 if m <= 32 else 64
@@ -54,17 +53,17 @@ def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: boo
             split *= 2
         return {"tile_n": tile, "cta_group": 1, "swap_ab": True, "split_k": split}
     best = None
-    for tile, cg in ((256, 2), (128, 2), (128, 1)):
+    # cycles of a K block and of a cluster's reduction, measured at 256 ... 8192 rows
+    for tile, cg, cycles, reduction in ((256, 2, 830, 0), (128, 2, 640, 0), (128, 1, 560, 8500), (64, 1, 400, 3000)):
         if not b_transposed and tile // cg != 128:
             continue  # a row-contiguous B arrives in boxes of 128 columns per CTA
         tiles = -(-m // (128 * cg)) * -(-n // tile)
         slots = num_sms // cg
-        cycles = max(tile * 2, (16384 + 128 * tile // cg) / 64)  # 128 x tile x 128 at 8192 products a cycle; bytes in
         for split in (1, 2, 4, 8) if cg == 1 else (1,):
             if split > 1 and (tiles * split > slots or kb < 4 * split):
                 continue
             waves = -(-tiles * split // slots)
-            cost = waves * (-(-kb // split) * cycles + 1500 + (2000 if split > 1 else 0))
+            cost = waves * (-(-kb // split) * cycles + 1500) + (reduction if split > 1 else 0)
             if best is None or cost < best[0]:
                 best = (cost, {"tile_n": tile, "cta_group": cg, "swap_ab": False, "split_k": split})
     pol = best[1]
@@ -254,7 +253,7 @@ _QUANT_ARGS = struct.Struct("@P3q4i" + "PqP2q" * 2 + "Pq")  # b200_gemm_quantize
 _GROUPS = {"row": 1, "col": 2, "both": 3, "block": 4}
 
 
-def _quantize(x, group, dtype, stream, want_colsum=False):
+def _quantize(x, group, dtype, stream):
     if group not in _GROUPS:
         raise ValueError(f"unknown group {group!r}; expected one of {tuple(_GROUPS)}")
     if dtype not in _F8_ID:
@@ -271,7 +270,6 @@ def _quantize(x, group, dtype, stream, want_colsum=False):
     mode = _GROUPS[group]
     got = []
     row = col = (0, 0, 0, 0, 0)
-    sums = (0, 0)
     with on_device(index, stream):
         if mode != 2:
             q = _pitched(rows, cols, dtype, device)
@@ -285,12 +283,8 @@ def _quantize(x, group, dtype, stream, want_colsum=False):
             s = torch.empty(_blocks(rows), cols, dtype=torch.float32, device=device)
             col = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), cols, 1)
             got += [q, s]
-        if want_colsum:
-            part = torch.empty((_blocks(rows), -(-cols // 4) * 4), dtype=torch.float32, device=device)
-            sums = (part.data_ptr(), part.shape[1])
-            got.append(part)
         args = _QUANT_ARGS.pack(x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, _F_ID[x.dtype], _F8_ID[dtype], mode, 0,
-                                *row, *col, *sums)
+                                *row, *col, 0, 0)
         rc = _lib.fast("b200_gemm_quantize_a8")(args, raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
@@ -312,58 +306,145 @@ def quantize_a8(x: torch.Tensor, group: str = "row", dtype: torch.dtype = torch.
 
 
 # ------------------------------------------------------------------------------------------------------ linear layer
+# A step of the layer is eight launches, and a launch through the public calls costs the host more than the GPU needs for it at
+# ordinary sizes. The layer checks its tensors once, keeps each pass's operands in one buffer and packs the argument blocks
+# itself.
+def _up(n: int, to: int) -> int:
+    return -(-n // to) * to
+
+
+class _Buffer:
+    """Offsets of the pieces of one allocation, each on a 256-byte boundary."""
+
+    __slots__ = ("at", "size")
+
+    def __init__(self, *sizes: int):
+        self.at, self.size = [], 0
+        for n in sizes:
+            self.at.append(self.size)
+            self.size += _up(n, 256)
+
+
+@functools.lru_cache(maxsize=1024)
+def _quantized(rows: int, cols: int, row: bool, col: bool, block: bool) -> _Buffer:
+    """Values (pitch a multiple of 16) and scales of each kind that is asked for, in this order."""
+    values, sizes = rows * _up(cols, 16), []
+    if row:
+        sizes += [values, 4 * rows * _blocks(cols)]
+    if col:
+        sizes += [values, 4 * _blocks(rows) * cols]
+    if block:
+        sizes += [values, 4 * _blocks(rows) * _blocks(cols)]
+    return _Buffer(*sizes)
+
+
+def _check(rc: int, name: str) -> None:
+    if rc != 0:
+        raise RuntimeError(f"{name} failed ({rc}): {_lib.strerror(rc)}")
+
+
+def _quantize_at(x, f8_id, row_at, col_at, block_at, sums, stream) -> None:
+    """Quantizes a row-major matrix to device addresses (0: not wanted), laid out as `_quantized` has them."""
+    rows, cols = x.shape
+    if rows == 0 or cols == 0:
+        return
+    pitch = _up(cols, 16)
+    mode = 4 if block_at else (1 if row_at else 0) + (2 if col_at else 0)
+    q = rows * pitch
+    row = (block_at or row_at, pitch, (block_at or row_at) + _up(q, 256), 1, _blocks(rows) if block_at else rows) if mode != 2 else (0,) * 5
+    col = (col_at, pitch, col_at + _up(q, 256), cols, 1) if mode in (2, 3) else (0,) * 5
+    args = _QUANT_ARGS.pack(x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, _F_ID[x.dtype], f8_id, mode, 0, *row, *col, *sums)
+    _check(_lib.fast("b200_gemm_quantize_a8")(args, stream), "b200_gemm_quantize_a8")
+
+
+def _gemm_at(pointers, m, n, k, lda, ldb, scale_strides, a_t, b_t, a_id, b_id, b_block, out_id, bias_id, index, status, stream) -> None:
+    """b200_gemm_a8w8 on device addresses; pointers: a, b, a_scale, b_scale, out, bias."""
+    if m == 0 or n == 0:
+        return
+    args = _ARGS.pack(*pointers, m, n, k, lda, ldb, n, *scale_strides, a_t, b_t, a_id, b_id, 0, b_block, out_id, bias_id,
+                      *_policy(m, n, k, a_t, b_t, {}, device_sms(index)), status)
+    _check(_lib.fast("b200_gemm_a8w8")(args, stream), "b200_gemm_a8w8")
+
+
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, grad_dtype):
-        x2 = _row_major(x.reshape(-1, x.shape[-1]))
-        need_dw = weight.requires_grad
-        f8 = torch.float8_e4m3fn
-        if need_dw:
-            xr, sxr, xc, sxc = _quantize(x2, "both", f8, None)
-        else:
-            xr, sxr = _quantize(x2, "row", f8, None)
-            xc = sxc = None
-        wq, sw = _quantize(_row_major(weight), "block", f8, None)
-        y = gemm_a8w8(xr, sxr, wq.t(), sw.t(), bias=bias, layout="nt", out_dtype=x.dtype)
-        ctx.save_for_backward(xc, sxc, wq if x.requires_grad else None, sw if x.requires_grad else None)
-        ctx.meta = (x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype, grad_dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        k, n = x.shape[-1], weight.shape[0]
+        x2, w2 = _row_major(x.reshape(-1, k)), _row_major(weight)
+        m = x2.shape[0]
+        need_x, need_w = ctx.needs_input_grad[:2]
+        index, device, e4 = x.get_device(), x.device, _lib.DTYPE_E4M3
+        kp, mb, nb, kb = _up(k, 16), _blocks(m), _blocks(n), _blocks(k)
+        with on_device(index, None):
+            stream = raw_stream(index)
+            y = torch.empty(m, n, dtype=x.dtype, device=device)
+            rows, cols, blocks = _quantized(m, k, True, False, False), _quantized(m, k, False, True, False), _quantized(n, k, False, False, True)
+            # what the backward pass reads: x by columns and the weight, as far as they are needed
+            keep = _Buffer(cols.size if need_w else 0, blocks.size if need_x else 0)
+            temp = torch.empty(rows.size + (0 if need_x else blocks.size), dtype=torch.uint8, device=device)
+            saved = torch.empty(keep.size, dtype=torch.uint8, device=device)
+            xr = temp.data_ptr()
+            xc = saved.data_ptr() if need_w else 0
+            wq = saved.data_ptr() + keep.at[1] if need_x else xr + rows.size
+            if k == 0:
+                y.copy_(0 if bias is None else bias.expand(m, n))
+            else:
+                _quantize_at(x2, e4, xr, xc, 0, (0, 0), stream)
+                _quantize_at(w2, e4, 0, 0, wq, (0, 0), stream)
+                _gemm_at((xr, wq, xr + rows.at[1], wq + blocks.at[1], y.data_ptr(), 0 if bias is None else bias.data_ptr()), m, n, k, kp, kp,
+                         (1, m, 1, nb), False, True, e4, e4, 1, _F_ID[x.dtype], 0 if bias is None else _F_ID[bias.dtype], index,
+                         _workspace_for(device, stream).status_ptr, stream)
+        ctx.save_for_backward(saved)
+        ctx.meta = (x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype, _F8_ID[grad_dtype], m, n, k, keep, cols, blocks)
+        return y.view(*x.shape[:-1], n)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xc, sxc, wq, sw = ctx.saved_tensors
-        shape, x_dtype, w_dtype, b_dtype, f8 = ctx.meta
+        (saved,) = ctx.saved_tensors
+        shape, x_dtype, w_dtype, b_dtype, g_id, m, n, k, keep, cols, blocks = ctx.meta
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        g = _row_major(dy.reshape(-1, dy.shape[-1]))  # an expanded gradient (of a sum) is spread out here
+        g = _row_major(dy.reshape(m, n))  # an expanded gradient (of a sum) is spread out here
+        index, device, e4 = dy.get_device(), dy.device, _lib.DTYPE_E4M3
+        np_, kp, mb, nb = _up(n, 16), _up(k, 16), _blocks(m), _blocks(n)
+        by_col = need_w or need_b
         dx = dw = db = None
-        col = need_w or need_b
-        got = list(_quantize(g, "both" if need_x and col else "col" if col else "row", f8, None, want_colsum=need_b))
-        if need_x:
-            gr, sgr = got[:2]
-            got = got[2:]
-            dx = gemm_a8w8(gr, sgr, wq, sw, layout="nn", out_dtype=x_dtype).view(shape)
-        if need_w:
-            gc, sgc = got[:2]
-            dw = gemm_a8w8(gc.t(), sgc.t(), xc, sxc, layout="tn", out_dtype=w_dtype)
-        if need_b:
-            db = _sum_rows(got[-1], g.shape[1], b_dtype)
+        with on_device(index, None):
+            stream = raw_stream(index)
+            status = _workspace_for(device, stream).status_ptr
+            grows, gcols = _quantized(m, n, True, False, False), _quantized(m, n, False, True, False)
+            pitch = _up(n, 4)
+            parts = _Buffer(grows.size if need_x else 0, gcols.size if by_col else 0, 4 * mb * pitch if need_b else 0)
+            temp = torch.empty(parts.size, dtype=torch.uint8, device=device)
+            gr, gc, sums = (temp.data_ptr() + at for at in parts.at)
+            if by_col or need_x:
+                _quantize_at(g, g_id, gr if need_x else 0, gc if by_col else 0, 0, (sums, pitch) if need_b else (0, 0), stream)
+            if need_x:
+                dx = torch.empty(m, k, dtype=x_dtype, device=device)
+                if n == 0:
+                    dx.zero_()
+                elif k:
+                    wq = saved.data_ptr() + keep.at[1]
+                    _gemm_at((gr, wq, gr + grows.at[1], wq + blocks.at[1], dx.data_ptr(), 0), m, k, n, np_, kp, (1, m, nb, 1), False, False,
+                             g_id, e4, 1, _F_ID[x_dtype], 0, index, status, stream)
+                dx = dx.view(shape)
+            if need_w:
+                dw = torch.empty(n, k, dtype=w_dtype, device=device)
+                if m == 0:
+                    dw.zero_()
+                elif k:
+                    xc = saved.data_ptr()
+                    _gemm_at((gc, xc, gc + gcols.at[1], xc + cols.at[1], dw.data_ptr(), 0), n, k, m, np_, kp, (1, n, 1, k), True, False,
+                             g_id, e4, 0, _F_ID[w_dtype], 0, index, status, stream)
+            if need_b:
+                db = torch.empty(pitch, dtype=b_dtype, device=device)
+                if m == 0:
+                    db.zero_()
+                elif n:  # the columns' sums over each 128 rows, added in order
+                    _check(_lib.load().b200_gemm_reduce_slots(sums, pitch, mb, db.data_ptr(), None, 1, pitch, _F_ID[b_dtype], 0, stream),
+                           "b200_gemm_reduce_slots")
+                db = db[:n]
         return dx, dw, db, None
-
-
-def _sum_rows(parts: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
-    """Sum over the first dimension of fp32 [parts, pitch], in order, rounded once; the first n columns."""
-    pitch = parts.shape[1]
-    out = torch.empty(pitch, dtype=dtype, device=parts.device)
-    if parts.shape[0] == 0:
-        return out.zero_()[:n]
-    index = parts.get_device()
-    with on_device(index, None):
-        rc = _lib.load().b200_gemm_reduce_slots(parts.data_ptr(), pitch, parts.shape[0], out.data_ptr(), None, 1, pitch, _F_ID[dtype], 0,
-                                                raw_stream(index))
-    if rc != 0:
-        raise RuntimeError(f"b200_gemm_reduce_slots failed ({rc}): {_lib.strerror(rc)}")
-    return out[:n]
 
 
 def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -376,10 +457,14 @@ def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     quantized along the rows in the forward pass); dbias is the sum of the unquantized gradient in fp32, in a fixed order.
     Gradients have their tensor's type."""
     assert weight.ndim == 2 and x.ndim >= 1 and x.shape[-1] == weight.shape[1], f"x is {tuple(x.shape)}, weight {tuple(weight.shape)}"
-    assert x.is_cuda, "linear_a8w8 runs on CUDA tensors only (there is no CPU path)"
-    assert x.device == weight.device
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype not in _F_ID:
+            raise ValueError(f"linear_a8w8 takes float32, bfloat16 or float16; {name} is {t.dtype}")
     if grad_dtype not in _F8_ID:
         raise ValueError(f"grad_dtype must be float8_e4m3fn or float8_e5m2, not {grad_dtype}")
+    assert x.is_cuda, "linear_a8w8 runs on CUDA tensors only (there is no CPU path)"
+    assert x.device == weight.device
     if bias is not None:
         assert bias.shape == (weight.shape[0],) and bias.device == x.device
+        bias = bias.contiguous()
     return _Linear8.apply(x, weight, bias, grad_dtype)
