@@ -65,7 +65,7 @@ struct Smem8 {
   static constexpr int kVBytes = kVRows * k8TK;
   static constexpr int kStageBytes = k8UBytes + kVBytes;
   static constexpr int kOutOff = STAGES * kStageBytes;
-  static constexpr int kStagingBytes = TILE_Q >= 128 ? 8 * 4096 : 0;      // one swizzled 32 x 128-byte image per epilogue warp
+  static constexpr int kStagingBytes = TILE_Q >= 64 ? 8 * 4096 : 0;       // one swizzled 32 x 128-byte image per epilogue warp
   static constexpr int kRecvBytes = CG == 1 ? k8TileP * TILE_Q * 4 : 0;   // cluster split: [source][own column][128] fp32
   static constexpr int kOutBytes = kRecvBytes > kStagingBytes ? kRecvBytes : kStagingBytes;
   static constexpr int kScaleOff = kOutOff + kOutBytes;
@@ -514,22 +514,45 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
           for (int i = 0; i < HC; ++i)
             if (qbase + i < p.Q) store_one(p.out, (long long)(qbase + i) * p.ldo + prow, acc(i) + b, p.out_dtype);
         }
-      } else if (HC >= 64 && p.tma_store) {
-        // One 128-byte row segment per lane into the warp's swizzled image (16-byte piece j of row t at j ^ (t % 8)), which
-        // leaves by TMA and is clipped at the matrix's edges.
+      } else if constexpr (HC >= 32) {
+        // One 128-byte row segment per lane into the warp's swizzled image (16-byte piece j of row t at j ^ (t % 8)). The image
+        // leaves by TMA, clipped at the matrix's edges; where C's rows do not start on 16 bytes the warp writes it row by
+        // row, neighbouring lanes neighbouring values (a lane per row would touch 32 sectors for every value).
         const int row0 = (tp * CG + prank) * k8TileP + quarter * 32;
         const uint32_t row_base = image + (uint32_t)lane * 128u;
         auto acquire = [&]() {
           if (lane == 0) tma_store_wait_read<0>();
           __syncwarp();
         };
-        auto flush = [&](int col0) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (row0 < p.P && col0 < p.Q) tma_store_2d(&p.tmap_out, col0, row0, image);
-            tma_store_commit();
+        auto flush = [&](int col0, int ncols) {  // ncols: columns of this segment inside the tile
+          if (p.tma_store) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (row0 < p.P && col0 < p.Q) tma_store_2d(&p.tmap_out, col0, row0, image);
+              tma_store_commit();
+            }
+            return;
           }
+          __syncwarp();
+          const int rows = min(32, p.P - row0), cols = min(ncols, p.Q - col0);
+          if (p.out_dtype == 1) {
+            float* dst = reinterpret_cast<float*>(p.out) + (long long)row0 * p.ldo + col0 + lane;
+            for (int t = 0; t < rows; ++t, dst += p.ldo)
+              if (lane < cols) *dst = *reinterpret_cast<const float*>(sm + (image - base) + t * 128 + ((((lane >> 2) ^ (t & 7)) << 4) | ((lane & 3) << 2)));
+          } else {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (long long)row0 * p.ldo + col0;
+            for (int t = 0; t < rows; ++t, dst += p.ldo) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(sm + (image - base) + t * 128 + ((((lane >> 2) ^ (t & 7)) << 4) | ((lane & 3) << 2)));
+              if (2 * lane + 1 < cols && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+                reinterpret_cast<uint32_t*>(dst)[lane] = w;
+              } else {
+                if (2 * lane < cols) dst[2 * lane] = (uint16_t)w;
+                if (2 * lane + 1 < cols) dst[2 * lane + 1] = (uint16_t)(w >> 16);
+              }
+            }
+          }
+          __syncwarp();  // the image may be rewritten
         };
         if (p.out_dtype == 1) {
 #pragma unroll
@@ -547,24 +570,25 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
                              "f"(v[4 * h]), "f"(v[4 * h + 1]), "f"(v[4 * h + 2]), "f"(v[4 * h + 3])
                              : "memory");
             }
-            flush(qbase + f * 32);
+            flush(qbase + f * 32, 32);
           }
         } else {
+          constexpr int FC = HC < 64 ? HC : 64;  // columns of a row segment
 #pragma unroll
-          for (int f = 0; f < HC / 64; ++f) {
+          for (int f = 0; f < HC / FC; ++f) {
             acquire();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < FC / 8; ++j) {
               float v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = acc(f * 64 + j * 8 + i);
-              add_bias8(p, v, qbase + f * 64 + j * 8);
+              for (int i = 0; i < 8; ++i) v[i] = acc(f * FC + j * 8 + i);
+              add_bias8(p, v, qbase + f * FC + j * 8);
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_base + (uint32_t)((j ^ (lane & 7)) << 4)),
                            "r"(pack16(v[0], v[1], p.out_dtype)), "r"(pack16(v[2], v[3], p.out_dtype)),
                            "r"(pack16(v[4], v[5], p.out_dtype)), "r"(pack16(v[6], v[7], p.out_dtype))
                            : "memory");
             }
-            flush(qbase + f * 64);
+            flush(qbase + f * FC, FC);
           }
         }
       } else if (prow < p.P) {
