@@ -185,14 +185,18 @@ static int run8(const Call8* h, cudaStream_t stream) {
   return e == cudaSuccess ? 0 : set_cuda_error(e);
 }
 
-template <typename T>
+template <typename T, bool E5M2>
 static void* quant_fn(int mode) {
   switch (mode) {
-    case 1: return reinterpret_cast<void*>(quantize_a8_kernel<T, 1>);
-    case 2: return reinterpret_cast<void*>(quantize_a8_kernel<T, 2>);
-    case 3: return reinterpret_cast<void*>(quantize_a8_kernel<T, 3>);
-    default: return reinterpret_cast<void*>(quantize_a8_kernel<T, 4>);
+    case 1: return reinterpret_cast<void*>(quantize_a8_kernel<T, 1, E5M2>);
+    case 2: return reinterpret_cast<void*>(quantize_a8_kernel<T, 2, E5M2>);
+    case 3: return reinterpret_cast<void*>(quantize_a8_kernel<T, 3, E5M2>);
+    default: return reinterpret_cast<void*>(quantize_a8_kernel<T, 4, E5M2>);
   }
+}
+template <typename T>
+static void* quant_fn(int mode, bool e5m2) {
+  return e5m2 ? quant_fn<T, true>(mode) : quant_fn<T, false>(mode);
 }
 
 }  // namespace b200
@@ -230,13 +234,13 @@ int b200_gemm_quantize_a8(const b200_gemm_quantize_args* a, void* cuda_stream) {
   b200::QuantParams p;
   memset(&p, 0, sizeof(p));
   p.x = a->x, p.ldx = a->ldx, p.rows = (int)a->rows, p.cols = (int)a->cols;
-  p.e5m2 = a->out_dtype == B200_GEMM_DTYPE_E5M2;
   p.q_row = static_cast<uint8_t*>(a->q_row), p.ldq_row = a->ldq_row, p.s_row = a->s_row, p.sr_row = a->sr_row, p.sr_group = a->sr_group;
   p.q_col = static_cast<uint8_t*>(a->q_col), p.ldq_col = a->ldq_col, p.s_col = a->s_col, p.sc_group = a->sc_group, p.sc_col = a->sc_col;
   p.colsum = a->colsum, p.colsum_ld = a->colsum_ld;
-  void* fn = a->in_dtype == B200_GEMM_DTYPE_FP32   ? b200::quant_fn<float>(a->mode)
-             : a->in_dtype == B200_GEMM_DTYPE_BF16 ? b200::quant_fn<__nv_bfloat16>(a->mode)
-                                                    : b200::quant_fn<__half>(a->mode);
+  const bool e5m2 = a->out_dtype == B200_GEMM_DTYPE_E5M2;
+  void* fn = a->in_dtype == B200_GEMM_DTYPE_FP32   ? b200::quant_fn<float>(a->mode, e5m2)
+             : a->in_dtype == B200_GEMM_DTYPE_BF16 ? b200::quant_fn<__nv_bfloat16>(a->mode, e5m2)
+                                                    : b200::quant_fn<__half>(a->mode, e5m2);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)tiles, 1, 1);

@@ -13,7 +13,6 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -28,7 +27,6 @@ struct QuantParams {
   const void* x;
   long long ldx;  // elements between rows of x (columns are contiguous)
   int rows, cols;
-  int e5m2;
   uint8_t* q_row;  // groups along a row (and 128 x 128 blocks, in block mode)
   long long ldq_row;
   float* s_row;
@@ -55,8 +53,25 @@ __device__ __forceinline__ uint32_t scale_bits(float amax, int n) {
 // 1 / s for a power of two s = 2^(b - 127), as fp32 bits; b is between 1 and 247, so the result is normal.
 __device__ __forceinline__ float inverse_of_scale(uint32_t bits) { return __uint_as_float((254u << 23) - bits); }
 
-__device__ __forceinline__ uint32_t pack_fp8x2(float lo, float hi, int e5m2) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+// Four values to the format, to nearest even (beyond its range: its largest value; NaN: NaN), the first in the lowest byte.
+template <bool E5M2>
+__device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {
+  uint32_t r;
+  if constexpr (E5M2)
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+  else
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
 }
 
 // Eight consecutive elements, and what the groups' maxima need: magnitudes compare like unsigned integers, so 16-bit values
@@ -81,7 +96,17 @@ struct Mag {
   static constexpr bool kWide = sizeof(T) == 4;
   static constexpr uint32_t kAbs = kWide ? 0x7fffffffu : 0x7fff7fffu;
   static constexpr uint32_t kInf = kWide ? 0x7f800000u : std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;  // and above: NaN
-  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return kWide ? max(a, b) : __vmaxu2(a, b); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    if constexpr (kWide) return max(a, b);
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  // an infinity of either sign to a NaN (both halves of a word)
+  static __device__ __forceinline__ uint32_t no_inf(uint32_t w) {
+    if constexpr (kWide) return (w & kAbs) == kInf ? w | 1u : w;
+    return w | ((w & 0x7fffu) == kInf ? 1u : 0u) | ((w >> 16 & 0x7fffu) == kInf ? 0x10000u : 0u);
+  }
   static __device__ __forceinline__ bool any_odd(uint32_t m) { return kWide ? m >= kInf : (m & 0xffffu) >= kInf || (m >> 16) >= kInf; }
   static __device__ __forceinline__ uint32_t only_finite(uint32_t m) {
     if constexpr (kWide) return m >= kInf ? 0u : m;
@@ -96,17 +121,12 @@ struct Mag {
   }
 };
 
+// The rows and columns at a ragged edge, or off 16-byte boundaries: element by element. Not inlined: the kernel's straight path is
+// long as it is, and waits for instructions where it outgrows the cache.
 template <typename T>
-__device__ __forceinline__ RawRow<T> load_row8(const T* src, int n, bool vec) {
+__device__ __noinline__ RawRow<T> load_row8_slow(const T* src, int n) {
   RawRow<T> r;
-  if (n >= 8 && vec) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src));  // read once
-    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
-    if constexpr (sizeof(T) == 4) {
-      const uint4 b = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
-      r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
-    }
-  } else if constexpr (sizeof(T) == 4) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.w[i] = i < n ? __float_as_uint(src[i]) : 0u;
   } else {
@@ -117,10 +137,27 @@ __device__ __forceinline__ RawRow<T> load_row8(const T* src, int n, bool vec) {
   }
   return r;
 }
+template <typename T>
+__device__ __forceinline__ RawRow<T> load_row8(const T* src, int n, bool vec) {
+  if (!(n >= 8 && vec)) return load_row8_slow(src, n);
+  RawRow<T> r;
+  const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src));  // read once
+  r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+  if constexpr (sizeof(T) == 4) {
+    const uint4 b = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
+    r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+  }
+  return r;
+}
+static __device__ __noinline__ void store_row8_slow(uint8_t* dst, uint32_t lo, uint32_t hi, int n) {
+  const uint64_t v = (uint64_t(hi) << 32) | lo;
+#pragma unroll 1
+  for (int j = 0; j < min(n, 8); ++j) dst[j] = (uint8_t)(v >> (8 * j));
+}
 
 // MODE: 1 = groups along rows, 2 = along columns, 4 = 128 x 128 blocks (written through the row members).
-template <typename T, int MODE>
-__global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantParams p) {
+template <typename T, int MODE, bool E5M2>
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantize_a8_kernel(const QuantParams p) {
   constexpr int kPasses = 8;  // rows per thread: ty, ty + 16, ...
   __shared__ float red[8][128];
   __shared__ float red2[8][128];
@@ -132,16 +169,17 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantP
   const int nrow = min(128, p.rows - r0);
   const T* x = reinterpret_cast<const T*>(p.x);
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ((p.ldx * (long long)sizeof(T)) & 15) == 0;
-  const int n = p.e5m2 ? 15 : 8;
+  constexpr int n = E5M2 ? 15 : 8;
 
   grid_dependency_wait();
   grid_launch_dependents();
   RawRow<T> v[kPasses];
+  const T* src = x + (long long)(r0 + ty) * p.ldx + col;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
-    const int r = ty + 16 * i;
-    const bool in = r < nrow && ncol > 0;
-    v[i] = load_row8<T>(x + (in ? (long long)(r0 + r) * p.ldx + col : 0), in ? ncol : 0, vec);
+    const bool in = ty + 16 * i < nrow && ncol > 0;
+    v[i] = load_row8<T>(in ? src : x, in ? ncol : 0, vec);
+    src += 16 * p.ldx;
   }
 
   // Largest magnitudes per row (over the thread's eight columns) and per column (over its eight rows).
@@ -172,7 +210,15 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantP
     for (int i = 0; i < kPasses; ++i) all = M::max2(all, rmag[i]);
   }
   const bool odd = M::any_odd(all);  // an infinity or a NaN among them: it counts as zero
-  if (odd) maxima([](uint32_t m) { return M::only_finite(m); });
+  if (odd) {
+    maxima([](uint32_t m) { return M::only_finite(m); });
+    if constexpr (!E5M2) {  // the conversion clamps infinities, e4m3 has none
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int j = 0; j < kW; ++j) v[i].w[j] = M::no_inf(v[i].w[j]);
+    }
+  }
   float rmax[kPasses], cmax[8];
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) rmax[i] = M::kWide ? M::value(rmag[i], 0) : fmaxf(M::value(rmag[i], 0), M::value(rmag[i], 1));
@@ -182,45 +228,52 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantP
   auto put = [&](uint8_t* dst, const RawRow<T>& raw, const float (&inv)[8], bool dvec) {
     uint32_t w[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t lo = pack_fp8x2(raw.get(4 * h) * inv[4 * h], raw.get(4 * h + 1) * inv[4 * h + 1], p.e5m2);
-      const uint32_t hi = pack_fp8x2(raw.get(4 * h + 2) * inv[4 * h + 2], raw.get(4 * h + 3) * inv[4 * h + 3], p.e5m2);
-      w[h] = lo | (hi << 16);
-    }
-    if (odd) {  // the conversion clamps infinities to the largest value
+    for (int h = 0; h < 2; ++h)
+      w[h] = pack_fp8x4<E5M2>(raw.get(4 * h) * inv[4 * h], raw.get(4 * h + 1) * inv[4 * h + 1], raw.get(4 * h + 2) * inv[4 * h + 2],
+                              raw.get(4 * h + 3) * inv[4 * h + 3]);
+    if constexpr (E5M2) {
+      if (odd) {  // the conversion clamps infinities to the largest value
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(raw.get(j));
-        if ((b & 0x7fffffffu) == 0x7f800000u) {
-          const uint32_t code = p.e5m2 ? 0x7cu | ((b >> 24) & 0x80u) : 0x7fu;
-          w[j >> 2] = (w[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (code << (8 * (j & 3)));
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __float_as_uint(raw.get(j));
+          if ((b & 0x7fffffffu) == 0x7f800000u) {
+            const uint32_t code = 0x7cu | ((b >> 24) & 0x80u);
+            w[j >> 2] = (w[j >> 2] & ~(0xffu << (8 * (j & 3)))) | (code << (8 * (j & 3)));
+          }
         }
       }
     }
-    if (dvec && ncol >= 8) {
+    if (dvec && ncol >= 8)
       *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < ncol) dst[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-    }
+    else
+      store_row8_slow(dst, w[0], w[1], ncol);
   };
   const bool rvec = (reinterpret_cast<uintptr_t>(p.q_row) & 7) == 0 && (p.ldq_row & 7) == 0;
   const bool cvec = (reinterpret_cast<uintptr_t>(p.q_col) & 7) == 0 && (p.ldq_col & 7) == 0;
 
   if constexpr (MODE & 1) {
+    // Eight rows over 16 lanes: each exchange halves the rows a lane answers for, so that eight shuffles (instead of 32) leave
+    // lane tx with the maximum of row ty + 16 * (tx / 2, its three bits) and one scale to work out.
+#pragma unroll
+    for (int h = 4; h > 0; h >>= 1) {
+      const bool up = tx & (2 * h);
+#pragma unroll
+      for (int j = 0; j < h; ++j) {
+        const float mine = up ? rmax[j + h] : rmax[j], other = up ? rmax[j] : rmax[j + h];
+        rmax[j] = fmaxf(mine, __shfl_xor_sync(0xffffffffu, other, 2 * h));
+      }
+    }
+    const uint32_t sb = scale_bits(fmaxf(rmax[0], __shfl_xor_sync(0xffffffffu, rmax[0], 1)), n);
+    const int own = ty + 16 * (tx >> 1);
+    if ((tx & 1) == 0 && own < nrow) p.s_row[(long long)(r0 + own) * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+    const float own_inv = inverse_of_scale(sb);
+    uint8_t* dst = p.q_row + (long long)(r0 + ty) * p.ldq_row + col;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
-      const int r = ty + 16 * i;
-      const uint32_t sb = scale_bits(rmax[i], n);
-      const float s = inverse_of_scale(sb);
+      const float s = __shfl_sync(0xffffffffu, own_inv, 2 * i, 16);
       const float inv[8] = {s, s, s, s, s, s, s, s};
-      if (r < nrow) {
-        if (ncol > 0) put(p.q_row + (long long)(r0 + r) * p.ldq_row + col, v[i], inv, rvec);
-        if (tx == 0) p.s_row[(long long)(r0 + r) * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
-      }
+      if (ty + 16 * i < nrow && ncol > 0) put(dst, v[i], inv, rvec);
+      dst += 16 * p.ldq_row;
     }
   }
   if constexpr (MODE & 2) {
@@ -267,10 +320,11 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantP
       float inv[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) inv[j] = red[0][tx * 8 + j];
+      uint8_t* dst = p.q_col + (long long)(r0 + ty) * p.ldq_col + col;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
-        const int r = ty + 16 * i;
-        if (r < nrow) put(p.q_col + (long long)(r0 + r) * p.ldq_col + col, v[i], inv, cvec);
+        if (ty + 16 * i < nrow) put(dst, v[i], inv, cvec);
+        dst += 16 * p.ldq_col;
       }
     }
   }
@@ -289,10 +343,11 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_a8_kernel(const QuantP
     const float s = inverse_of_scale(sb);
     const float inv[8] = {s, s, s, s, s, s, s, s};
     if (ncol > 0) {
+      uint8_t* dst = p.q_row + (long long)(r0 + ty) * p.ldq_row + col;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
-        const int r = ty + 16 * i;
-        if (r < nrow) put(p.q_row + (long long)(r0 + r) * p.ldq_row + col, v[i], inv, rvec);
+        if (ty + 16 * i < nrow) put(dst, v[i], inv, rvec);
+        dst += 16 * p.ldq_row;
       }
     }
   }
