@@ -9,20 +9,21 @@
 
 namespace b200 {
 
-// Ring depths: as many 128-deep stages as fit 227 KB next to the exchange area.
+// Ring depths: as many stages (128 deep, the widest second kernel's 64) as fit 227 KB next to the exchange area.
 struct MoeVariant {
   MoeFn up, down;
-  int up_smem, down_smem, cols;
+  int up_smem, down_smem, cols, down_k;
 };
-template <int TN, int UP_STAGES, int DOWN_STAGES>
+template <int TN, int UP_STAGES, int DOWN_STAGES, int DOWN_SUBS>
 static MoeVariant moe_make() {
-  using Up = SmemMoe<TN, UP_STAGES, true>;
-  using Down = SmemMoe<TN, DOWN_STAGES, false>;
+  using Up = SmemMoe<TN, UP_STAGES, 2, true>;
+  using Down = SmemMoe<TN, DOWN_STAGES, DOWN_SUBS, false>;
   static_assert(Up::kDynBytes <= 227 * 1024 && Down::kDynBytes <= 227 * 1024, "shared memory");
-  return {moe_a16w16_sm100_kernel<TN, UP_STAGES, true>, moe_a16w16_sm100_kernel<TN, DOWN_STAGES, false>, Up::kDynBytes, Down::kDynBytes, TN};
+  return {moe_a16w16_sm100_kernel<TN, UP_STAGES, 2, true>, moe_a16w16_sm100_kernel<TN, DOWN_STAGES, DOWN_SUBS, false>, Up::kDynBytes,
+          Down::kDynBytes, TN, 64 * DOWN_SUBS};
 }
 static MoeVariant moe_variant(int64_t t) {
-  return t <= 16 ? moe_make<16, 5, 5>() : t <= 32 ? moe_make<32, 5, 4>() : moe_make<64, 4, 3>();
+  return t <= 16 ? moe_make<16, 5, 5, 2>() : t <= 32 ? moe_make<32, 5, 4, 2>() : moe_make<64, 4, 5, 1>();
 }
 
 constexpr uint64_t kMoeListBytes = 4096;  // the list of chosen experts at the start of the scratch
@@ -115,15 +116,16 @@ static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   u.status = a->status;
   u.wait_limit_ns = a->wait_limit_us > 0 ? (unsigned long long)a->wait_limit_us * 1000ull : kWaitLimitNs;
   const uint32_t fmt = a->dtype == B200_GEMM_DTYPE_BF16 ? 1u : 0u;
-  u.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(cols >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+  u.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(cols >> 3) << 17) | (uint32_t(128 >> 4) << 24);  // N = the tokens' rows
   u.desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
   h->down = u;
+  h->down.idesc = (u.idesc & ~(0x3fu << 17)) | (uint32_t(2 * cols >> 3) << 17);
   const int64_t slots = moe_slots(a);
   const int64_t one13 = a->experts > 1 ? a->w13_expert : 2 * a->inner * a->w13_row, one2 = a->experts > 1 ? a->w2_expert : a->hidden * a->w2_row;
   rc = encode3(&h->up.tmap_u, a->dtype, a->w13, a->hidden, 2 * a->inner, a->experts, a->w13_row, one13, 64);
   if (!rc) rc = encode3(&h->up.tmap_v, a->dtype, a->x, a->hidden, a->tokens, 0, a->ldx, 0, cols);
   if (!rc) rc = encode3(&h->down.tmap_u, a->dtype, a->w2, a->inner, a->hidden, a->experts, a->w2_row, one2, 128);
-  if (!rc) rc = encode3(&h->down.tmap_v, a->dtype, u.h, a->inner, a->tokens, slots, a->inner, a->tokens * a->inner, cols);
+  if (!rc) rc = encode3(&h->down.tmap_v, a->dtype, u.h, a->inner, a->tokens, 2 * slots, a->inner, a->tokens * a->inner, cols);
   if (rc) return rc;
 
   const int64_t units = slots * ((a->inner + 63) / 64);
@@ -135,7 +137,7 @@ static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   // on how its SMs are grouped: 16 clusters of 8 have been seen to take two turns); no CTA without a K block or a token's
   // column to finish.
   const int row_tiles = (int)((a->hidden + 127) / 128);
-  const int64_t blocks = slots * ((a->inner + kMoeTK - 1) / kMoeTK);
+  const int64_t blocks = slots * ((a->inner + h->var.down_k - 1) / h->var.down_k);
   int s = 16;
   if (s > blocks) s = (int)blocks;
   while (s > 1 && (row_tiles * s > sms || max_clusters(h->var, s, dev) < row_tiles)) --s;
@@ -179,7 +181,7 @@ extern "C" {
 
 uint64_t b200_gemm_moe_workspace_bytes(const b200_gemm_moe_args* args) {
   if (b200::moe_check(args) != 0) return 0;
-  return b200::kMoeListBytes + (uint64_t)(b200::moe_slots(args) * args->tokens * args->inner) * 2;
+  return b200::kMoeListBytes + (uint64_t)(b200::moe_slots(args) * args->tokens * args->inner) * 4;
 }
 
 int b200_gemm_moe_a16w16(const b200_gemm_moe_args* args, void* cuda_stream) {

@@ -12,9 +12,10 @@
 //    of its own; the list of chosen experts goes to the second kernel. (The second kernel routing again, in order to fill
 //    its ring with weights while the first one's last tiles run, took 26.2 instead of 24.4 us for one token of 8 / 128
 //    experts, 169 instead of 171 us for 8 tokens of 2 / 16: its blocks mostly start when the first kernel's end.)
-//  * First kernel: a tile is 64 gate rows over 64 up rows of one expert; its epilogue writes h[slot][t][i] =
-//    round16(p * silu(gate) * up), zero for pairs that were not chosen. The weight of the pair is folded in before the one
-//    rounding that the second product's 16-bit operand needs.
+//  * First kernel: a tile is 64 gate rows over 64 up rows of one expert; its epilogue computes h[slot][t][i] = p * silu(gate) *
+//    up, zero for pairs that were not chosen, with the weight of the pair folded in. h is the second product's 16-bit
+//    operand; it is stored as two of them, the rounded value and the rounded remainder, which cost that product columns
+//    (2 TN instead of TN) that it has to spare. Rounded once, h would put as much error into y as y's own rounding does.
 //  * Second kernel: the sum over experts is the K axis of one product, y[h, t] = sum over (slot, i) of W2 * h, accumulated
 //    in TMEM. K is cut into contiguous spans over the CTAs of a cluster, which add up through distributed shared
 //    memory in rank order: no atomics, the same bits every time.
@@ -29,18 +30,16 @@ namespace b200 {
 
 constexpr int kMoeThreads = 384;  // warp 0 TMA producer, warp 1 TMEM and MMA, warps 2-5 epilogue; 6-11 only help to route
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
-constexpr int kMoeTK = 128;       // K elements per stage: two 64-element swizzle spans
-constexpr int kMoeUBytes = 128 * kMoeTK * 2;
 
 struct alignas(64) MoeParams {
   CUtensorMap tmap_u;  // W13 as {H, 2I, E}, box {64, 64, 1}; or W2 as {I, H, E}, box {64, 128, 1}
-  CUtensorMap tmap_v;  // x as {H, T}, box {64, TN}; or h as {I, T, slots}, box {64, TN, 1}
+  CUtensorMap tmap_v;  // x as {H, T}, box {64, TN}; or h as {I, T, 2 slots}, box {64, TN, 1}
   const void* logits;
   long long logits_row, logits_col;
   int logits_dtype;  // 1 fp32, 2 bf16, 3 fp16
   int T, E, H, I, top_k, renorm;
   int dtype;         // 2 bf16, 3 fp16
-  uint16_t* h;       // [slot][T][I]
+  uint16_t* h;       // [slot][value, remainder][T][I]
   int* list;         // [0] = number of experts that a token chose, [16..] = their indices in increasing order
   void* out;
   long long ldo;
@@ -50,10 +49,14 @@ struct alignas(64) MoeParams {
   unsigned long long wait_limit_ns;
 };
 
-template <int TN, int STAGES, bool UP>
+// A stage holds SUBS swizzle spans (64 K elements) of 128 weight rows and of the tokens' rows (the second kernel's twice: value
+// and remainder).
+template <int TN, int STAGES, int SUBS, bool UP>
 struct SmemMoe {
-  static constexpr int kVBox = TN * 128;
-  static constexpr int kStageBytes = kMoeUBytes + 2 * kVBox;
+  static constexpr int kVRows = UP ? TN : 2 * TN;
+  static constexpr int kVBox = kVRows * 128;
+  static constexpr int kUBytes = SUBS * 16384;
+  static constexpr int kStageBytes = kUBytes + SUBS * kVBox;
   static constexpr int kXOff = STAGES * kStageBytes;                 // UP: the up half's sums [TN][64]; otherwise recv[t / S][source][128], t / S <= (TN - 1) / S
   static constexpr int kXBytes = UP ? TN * 64 * 4 : (TN + 15) * 128 * 4;
   static constexpr int kRouteOff = kXOff + kXBytes;
@@ -112,9 +115,9 @@ __device__ __forceinline__ void stage_logits(const MoeParams& p, const T* logits
 // The whole block routes all tokens: ids[t][r], weights[t][r] for r < top_k (-1 and zero: not chosen), the chosen experts' bits
 // in `mask`. `keys` is scratch for T * stride integers.
 //
-// This code runs once per launch and its instructions come from L2 meanwhile, about 30 cycles each by the counters, so it is
-// written for few instructions and not for few cycles: logits as ordered integers in shared memory, rolled loops. (With
-// logits in unrolled registers routing took 3 us for one token and 16 us for 64, with them it takes XX and XX.)
+// A single token has latencies to pay one after the other, many tokens have instructions to issue; both are kept few: logits
+// as ordered integers in shared memory, loads in batches, short rolled loops. One token of 128 experts takes 3 us (1 us of
+// it for its logits to come), 32 of 32 5.4 us, 64 of 64 8 us.
 __device__ __forceinline__ void route_all(const MoeParams& p, uint32_t* keys, int* ids, float* weights, uint32_t* mask) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int e4 = (p.E + 3) & ~3, stride = e4 + 4;  // rows of 16-byte pieces, on different banks
@@ -129,23 +132,21 @@ __device__ __forceinline__ void route_all(const MoeParams& p, uint32_t* keys, in
   if (p.T * p.E <= kMoeThreads && p.E <= 128) {
     // A thread per (token, expert): its rank is the number of experts ahead of it (larger, or equal with a lower index).
     const int t = tid / p.E, e = tid - t * p.E;
-    uint32_t* row = keys + t * stride;
-    int rank = p.top_k;
-    if (t < p.T) {
-      const uint32_t mine = row[e];
-      rank = 0;
+    uint32_t* row = keys + min(t, p.T - 1) * stride;
+    const uint32_t mine = row[e];
+    int rank = 0;
 #pragma unroll 2
-      for (int o = 0; o < e4; o += 4) {
-        const uint4 k = *reinterpret_cast<const uint4*>(row + o);
-        rank += (k.x + (o < e) > mine) + (k.y + (o + 1 < e) > mine) + (k.z + (o + 2 < e) > mine) + (k.w + (o + 3 < e) > mine);
-      }
-      if (rank < p.top_k) {
-        ids[t * kMoeMaxTopK + rank] = e;
-        weights[t * kMoeMaxTopK + rank] = logit_of_key(mine);
-      }
+    for (int o = 0; o < e4; o += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(row + o);
+      rank += (k.x + (o < e) > mine) + (k.y + (o + 1 < e) > mine) + (k.z + (o + 2 < e) > mine) + (k.w + (o + 3 < e) > mine);
+    }
+    const bool chosen = t < p.T && rank < p.top_k;
+    if (chosen) {
+      ids[t * kMoeMaxTopK + rank] = e;
+      weights[t * kMoeMaxTopK + rank] = logit_of_key(mine);
     }
     __syncthreads();
-    if (rank < p.top_k) row[e] = 0;
+    if (chosen) row[e] = 0;
   } else {
     // More pairs of experts than threads to compare them: top_k rounds per token, each taking out the largest.
     const int sub = lane & (G - 1);
@@ -210,10 +211,12 @@ __device__ __forceinline__ void route_all(const MoeParams& p, uint32_t* keys, in
 }
 
 // UP: the first kernel (gate and up products, SiLU), otherwise the second (down product and sum).
-template <int TN, int STAGES, bool UP>
+template <int TN, int STAGES, int SUBS, bool UP>
 __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const __grid_constant__ MoeParams p) {
-  using L = SmemMoe<TN, STAGES, UP>;
-  constexpr uint32_t kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
+  using L = SmemMoe<TN, STAGES, SUBS, UP>;
+  constexpr int kTK = 64 * SUBS;
+  constexpr int NC = L::kVRows;  // accumulator columns
+  constexpr uint32_t kTmemCols = 2 * NC < 32 ? 32 : 2 * NC;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
   const int* experts = list + 16;
 
   // UP: unit = (slot, 64 gate rows), K = H. Otherwise one unit per CTA: 128 rows of H, a span of the K axis (slot, I).
-  const int k_blocks = UP ? (p.H + kMoeTK - 1) / kMoeTK : (p.I + kMoeTK - 1) / kMoeTK;
+  const int k_blocks = ((UP ? p.H : p.I) + kTK - 1) / kTK;
   const int tiles = UP ? (p.I + 63) / 64 : 1;
   const int S = cluster_mode ? p.cluster_split : 1;
   const long long span = (long long)n_active * k_blocks;
@@ -329,20 +332,21 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
           }
         }
         if (elect_one()) {
-          const uint32_t fb = full_bar(stage), su = base + stage * L::kStageBytes, sv = su + kMoeUBytes;
+          const uint32_t fb = full_bar(stage), su = base + stage * L::kStageBytes, sv = su + L::kUBytes;
           const int s = UP ? slot0 : b / k_blocks, kb = UP ? b : b - s * k_blocks;
           const int expert = experts[s];
           mbar_arrive_expect_tx(fb, L::kStageBytes);
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-            const int k0 = kb * kMoeTK + sub * 64;
+          for (int sub = 0; sub < SUBS; ++sub) {
+            const int k0 = kb * kTK + sub * 64;
             if constexpr (UP) {
               tma_load_3d(su + sub * 16384, &p.tmap_u, k0, i0, expert, fb);
               tma_load_3d(su + sub * 16384 + 8192, &p.tmap_u, k0, p.I + i0, expert, fb);
               tma_load_2d(sv + sub * L::kVBox, &p.tmap_v, k0, 0, fb);
             } else {
               tma_load_3d(su + sub * 16384, &p.tmap_u, k0, row_tile * 128, expert, fb);
-              tma_load_3d(sv + sub * L::kVBox, &p.tmap_v, k0, 0, s, fb);
+              tma_load_3d(sv + sub * L::kVBox, &p.tmap_v, k0, 0, 2 * s, fb);
+              tma_load_3d(sv + sub * L::kVBox + TN * 128, &p.tmap_v, k0, 0, 2 * s + 1, fb);
             }
           }
         }
@@ -383,15 +387,15 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
         }
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t su = base + stage * L::kStageBytes, sv = su + kMoeUBytes;
+          const uint32_t su = base + stage * L::kStageBytes, sv = su + L::kUBytes;
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
+          for (int sub = 0; sub < SUBS; ++sub) {
             // K-major rows of 128 swizzled bytes, groups of eight 1024 bytes apart
             const uint64_t du = (uint64_t(p.desc_hi) << 32) | uint64_t((1u << 16) | (((su + sub * 16384) >> 4) & 0x3fffu));
             const uint64_t dv = (uint64_t(p.desc_hi) << 32) | uint64_t((1u << 16) | (((sv + sub * L::kVBox) >> 4) & 0x3fffu));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              umma_f16<1>(tmem_base + buf * TN, du + uint64_t(2 * j), dv + uint64_t(2 * j), p.idesc, (b != b_first || sub || j) ? 1u : 0u);
+              umma_f16<1>(tmem_base + buf * NC, du + uint64_t(2 * j), dv + uint64_t(2 * j), p.idesc, (b != b_first || sub || j) ? 1u : 0u);
           }
           umma_commit(empty_bar(stage));
           if (b + 1 == b_end) umma_commit(accf_bar(buf));
@@ -428,17 +432,22 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
           break;
         }
         tc_fence_after();
-        const uint32_t t_acc = tmem_base + buf * TN + (uint32_t(quarter * 32) << 16);
+        const uint32_t t_acc = tmem_base + buf * NC + (uint32_t(quarter * 32) << 16);
         uint32_t r[32];
 #pragma unroll
-        for (int c = 0; c < TN; c += 32) {
+        for (int c = 0; c < NC; c += TN < 32 ? TN : 32) {
           if constexpr (TN >= 32)
             tmem_ld_32x32(t_acc + c, r);
           else
             tmem_ld_32x16(t_acc + c, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < (TN < 32 ? TN : 32); ++i) v[c + i] = __uint_as_float(r[i]);
+          for (int i = 0; i < (TN < 32 ? TN : 32); ++i) {
+            if (c < TN)
+              v[c + i] = __uint_as_float(r[i]);
+            else
+              v[c - TN + i] += __uint_as_float(r[i]);  // the remainders' part
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -458,7 +467,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
         named_bar_sync(2, 128);
         const int i = (u - slot * tiles) * 64 + r64;
         if (i < p.I) {
-          uint16_t* dst = p.h + ((size_t)slot * p.T) * p.I + i;
+          const size_t plane = (size_t)p.T * p.I;
+          uint16_t* dst = p.h + 2 * slot * plane + i;
 #pragma unroll
           for (int j = 0; j < TN / 2; ++j) {
             const int t = is_gate ? j : TN / 2 + j;
@@ -467,15 +477,17 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
               const float g = is_gate ? own : other, up = is_gate ? other : own;
               // a pair that was not chosen is zero whatever its sums are
               const float a = w == 0.f ? 0.f : w * __fdividef(g, 1.f + __expf(-g)) * up;
-              uint16_t bits;
+              uint16_t bits, rest;
               if (p.dtype == 2) {
-                const __nv_bfloat16 h = __float2bfloat16_rn(a);
-                bits = *reinterpret_cast<const uint16_t*>(&h);
+                const __nv_bfloat16 h = __float2bfloat16_rn(a), l = __float2bfloat16_rn(a - __bfloat162float(h));
+                bits = __bfloat16_as_ushort(h), rest = __bfloat16_as_ushort(l);
               } else {
-                const __half h = __float2half_rn(a);
-                bits = *reinterpret_cast<const uint16_t*>(&h);
+                const __half h = __float2half_rn(a), l = __float2half_rn(a - __half2float(h));
+                bits = __half_as_ushort(h), rest = __half_as_ushort(l);
               }
+              if ((p.dtype == 2 ? bits & 0x7f80u : bits & 0x7c00u) == (p.dtype == 2 ? 0x7f80u : 0x7c00u)) rest = 0;  // infinite or NaN
               dst[(size_t)t * p.I] = bits;
+              dst[plane + (size_t)t * p.I] = rest;
             }
           }
         }

@@ -37,7 +37,7 @@ def _check_matrix(name: str, t: torch.Tensor, shape: tuple) -> None:
 
 def _scratch_bytes(t: int, i: int, e: int, top_k: int) -> int:
     """b200_gemm_moe_workspace_bytes: the list of chosen experts, and h for each that t tokens can choose."""
-    return 4096 + 2 * min(t * top_k, e) * t * i
+    return 4096 + 4 * min(t * top_k, e) * t * i
 
 
 def _arguments(x, logits, w13, w2, top_k, out, renormalize, user_kwargs, workspace, workspace_bytes, status) -> bytes:
@@ -92,7 +92,8 @@ def moe_a16w16(
     x [T, H] with 1 to 64 tokens (0: nothing is done), logits [T, E] of the router (float32, bfloat16 or float16, any strides),
     w13 [E, 2 I, H] (gate rows, then up rows), w2 [E, H, I]; x, weights and `out` [T, H] are all bfloat16 or all float16. p is the
     softmax over all experts, ties go to the lowest index, and with `renormalize` the chosen weights are divided by their sum.
-    Sums, softmax and SiLU are fp32; p * silu(g) * u is rounded to the 16-bit type as the second product's operand.
+    Sums, softmax and SiLU are fp32; p * silu(g) * u, the second product's operand, is carried as a 16-bit value and a 16-bit
+    remainder.
 
     An expert of weight zero (a logit of -inf) is not evaluated, a token whose logits are all -inf gets zeros, a NaN logit
     makes its token's row NaN. Non-finite values in a chosen expert's weights reach every token of the call.

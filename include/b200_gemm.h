@@ -306,8 +306,8 @@ int b200_gemm_quantize_a8(const b200_gemm_quantize_args* args, void* cuda_stream
  * A mixture-of-experts layer for a few tokens, in two kernels.
  *   p = softmax(logits[t, :]); the top_k experts of each token, ties to the lowest index; weights divided by their sum when
  *   `renormalize`; out[t] = sum over them of p * W2[e] (silu(G) * U), [G; U] = W13[e] x[t], rounded once.
- * 16-bit x, weights and output (all `dtype`); sums, softmax and SiLU in fp32; p * silu(G) * U is rounded to `dtype` once, as
- * the operand of the second product (so in fp16 it has to stay below 65504). An expert whose weight is zero (a logit of -inf)
+ * 16-bit x, weights and output (all `dtype`); sums, softmax and SiLU in fp32; p * silu(G) * U, the operand of the second
+ * product, is carried as a value and a remainder of `dtype` (so in fp16 it has to stay below 65504). An expert whose weight is zero (a logit of -inf)
  * is not evaluated; a token whose logits are all -inf gets zeros; a NaN logit makes its token's output NaN. Each chosen
  * expert's weights are read once for all tokens; non-finite values in them reach every token of the call.
  * Limits: 1 ... 64 tokens, up to 512 experts, top_k up to 16; hidden and inner multiples of 8; x and the weights on 16-byte

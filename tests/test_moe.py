@@ -36,8 +36,8 @@ def test_entry_points_refuse_before_any_device_work():
     for ws in (dict(workspace=None), dict(workspace=4100), dict(workspace_bytes=4096)):
         assert lib.b200_gemm_moe_a16w16(C.byref(args(**ws)), None) == -3
     # a list of experts, and h for every expert that four tokens can choose
-    assert lib.b200_gemm_moe_workspace_bytes(C.byref(args())) == 4096 + 8 * 4 * 32 * 2
-    assert lib.b200_gemm_moe_workspace_bytes(C.byref(args(tokens=1))) == 4096 + 2 * 1 * 32 * 2
+    assert lib.b200_gemm_moe_workspace_bytes(C.byref(args())) == 4096 + 8 * 4 * 32 * 4
+    assert lib.b200_gemm_moe_workspace_bytes(C.byref(args(tokens=1))) == 4096 + 2 * 1 * 32 * 4
     assert lib.b200_gemm_moe_a16w16(None, None) == -1
     for t, i, e, k in ((4, 32, 8, 2), (1, 32, 8, 2), (64, 2048, 512, 16)):  # the Python call's own sum
         assert _scratch_bytes(t, i, e, k) == lib.b200_gemm_moe_workspace_bytes(C.byref(args(

@@ -1,8 +1,9 @@
 """The few-token mixture-of-experts layer against its formula in 64 bits.
 
 Bounds, from the roundings that happen: the first product's fp32 sums (H / 16 accumulating instructions, 2^-23 of the sum of
-magnitudes each), the exponentials and the softmax (32 units of 2^-23, and 2 |g| more for the SiLU's), half a step of the
-16-bit type for each h, the second product's fp32 sums, and half a step for the result. They are propagated entry by entry.
+magnitudes each), the exponentials and the softmax (32 units of 2^-23, and 2 |g| more for the SiLU's), half a step of half a
+step of the 16-bit type for each h (a value and a remainder), the second product's fp32 sums, and half a step for the
+result. They are propagated entry by entry.
 """
 import pytest
 import torch
@@ -56,7 +57,7 @@ def reference(x, logits, w13, w2, top_k, renorm):
             silu = g / (1 + torch.exp(-g))
             hv = p * silu * u
             d = p * (1.1 * u.abs() * s[:i_n] + (silu.abs() + 1.1 * s[:i_n]) * s[i_n:]) + hv.abs() * (32 + 2 * g.abs()) * U23
-            d = d + (hv.abs() + d) * eps + tiny
+            d = d + (hv.abs() + d) * eps * eps + tiny
             y[t] += b @ hv
             err[t] += b.abs() @ d
             mag[t] += b.abs() @ (hv.abs() + d)
