@@ -65,7 +65,10 @@ struct Smem8 {
   static constexpr int kVBytes = kVRows * k8TK;
   static constexpr int kStageBytes = k8UBytes + kVBytes;
   static constexpr int kOutOff = STAGES * kStageBytes;
-  static constexpr int kStagingBytes = TILE_Q >= 64 ? 8 * 4096 : 0;       // one swizzled 32 x 128-byte image per epilogue warp
+  // swizzled 32 x 128-byte images of the epilogue warps on their way out: two each where a warp has two or more segments to
+  // send (2 % on 256 columns; the fifth ring stage that they displace gained nothing), else one
+  static constexpr int kImages = TILE_Q >= 256 ? 2 : 1;
+  static constexpr int kStagingBytes = TILE_Q >= 64 ? 8 * kImages * 4096 : 0;
   static constexpr int kRecvBytes = CG == 1 ? k8TileP * TILE_Q * 4 : 0;   // cluster split: [source][own column][128] fp32
   static constexpr int kOutBytes = kRecvBytes > kStagingBytes ? kRecvBytes : kStagingBytes;
   static constexpr int kScaleOff = kOutOff + kOutBytes;
@@ -408,7 +411,8 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
     const int half = (warp - 4) >> 2;
     const int row = quarter * 32 + lane;
     const float* ring = reinterpret_cast<const float*>(sm + L::kScaleOff);
-    const uint32_t image = base + L::kOutOff + (uint32_t)(warp - 4) * 4096u;
+    const uint32_t image0 = base + L::kOutOff + (uint32_t)((warp - 4) * L::kImages) * 4096u;
+    uint32_t image = image0;
     int g = 0, stage = 0;
     uint32_t phase = 0;
 #pragma unroll 1
@@ -519,10 +523,14 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
         // leaves by TMA, clipped at the matrix's edges; where C's rows do not start on 16 bytes the warp writes it row by
         // row, neighbouring lanes neighbouring values (a lane per row would touch 32 sectors for every value).
         const int row0 = (tp * CG + prank) * k8TileP + quarter * 32;
-        const uint32_t row_base = image + (uint32_t)lane * 128u;
-        auto acquire = [&]() {
-          if (lane == 0) tma_store_wait_read<0>();
+        uint32_t row_base = image + (uint32_t)lane * 128u;
+        auto acquire = [&]() {  // the store that last read the next image is done with it
+          if (lane == 0) tma_store_wait_read<L::kImages - 1>();
           __syncwarp();
+          if (L::kImages > 1) {
+            image = image0 + ((image - image0) ^ 4096u);
+            row_base = image + (uint32_t)lane * 128u;
+          }
         };
         auto flush = [&](int col0, int ncols) {  // ncols: columns of this segment inside the tile
           if (p.tma_store) {

@@ -27,7 +27,7 @@ bool variant8(int tile_q, int cta_group, int v_vector, Variant8* out) {
   if (cta_group == 1 && tile_q == 64) return *out = make<64, 7, 1>(v_vector), true;
   if (cta_group == 1 && tile_q == 128) return *out = make<128, 4, 1>(v_vector), true;
   if (cta_group == 2 && tile_q == 128) return *out = make<128, 7, 2>(v_vector), true;
-  if (cta_group == 2 && tile_q == 256) return *out = make<256, 5, 2>(v_vector), true;
+  if (cta_group == 2 && tile_q == 256) return *out = make<256, 4, 2>(v_vector), true;
   return false;
 }
 
