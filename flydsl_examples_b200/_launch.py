@@ -21,7 +21,11 @@ def on_device(index: int, stream: Optional[torch.cuda.Stream]):
         if stream.device_index != index:
             raise ValueError(f"the stream belongs to cuda:{stream.device_index}, the tensors are on cuda:{index}")
         return torch.cuda.stream(stream)  # also makes the stream's device the current one
-    return _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _NOTHING if is_current(index) else torch.cuda.device(index)
+
+
+def is_current(index: int) -> bool:
+    return torch._C._cuda_getDevice() == index
 
 
 @functools.lru_cache(maxsize=None)

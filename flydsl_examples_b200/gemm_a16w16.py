@@ -42,13 +42,14 @@ class _Workspace:
     4-word status block kernels write when a bounded wait gives up. Grows on demand, never shrinks.
     Takes the place of get_split_k_buffers (kernels/gemm_a16w16_gfx950.py:1277-1281)."""
 
-    __slots__ = ("buf", "status", "status_ptr", "generation")
+    __slots__ = ("buf", "status", "status_ptr", "status_bytes", "generation")
 
     def __init__(self, device: torch.device):
         self.buf = None
         self.generation = 0
         self.status = torch.zeros(_STATUS_WORDS, dtype=torch.int32, device=device)
         self.status_ptr = self.status.data_ptr()
+        self.status_bytes = self.status_ptr.to_bytes(8, "little")  # as the last member of an argument block
 
     def ensure(self, nbytes: int, device: torch.device, stream: torch.cuda.Stream) -> None:
         if self.buf is None or self.buf.numel() < nbytes:

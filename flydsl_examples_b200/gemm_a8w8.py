@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._launch import device_sms, on_device, raw_stream
+from ._launch import device_sms, is_current, on_device, raw_stream
 from .gemm_a16w16 import _workspace_for
 
 GROUP = 128
@@ -94,65 +94,94 @@ def _policy(m, n, k, a_t, b_t, user_kwargs, num_sms) -> tuple:
 # -------------------------------------------------------------------------------------------------------------- GEMM
 _LAYOUTS = {"nn": (False, False), "nt": (False, True), "tn": (True, False), "tt": (True, True)}
 _ARGS = struct.Struct("@6P10q8i16iP")  # b200_gemm_a8w8_args
+_POINTERS, _SIZES = struct.Struct("@6P"), struct.Struct("@10q8i16i")  # the same in parts; the last member is the status address
 
 
-def _check_operand(name: str, t: torch.Tensor, transposed: bool) -> int:
+def _leading(name: str, shape, stride, transposed: bool) -> int:
     """Leading stride of an operand; raises unless the contiguous dimension has stride 1 and rows start on 16 bytes."""
-    rows, cols = t.shape
-    lead, inner = t.stride()
-    n_lead, n_inner = rows, cols
+    n_lead, n_inner = shape
+    lead, inner = stride
     if transposed:
         lead, inner, n_lead, n_inner = inner, lead, n_inner, n_lead
     if n_inner == 1:
         inner = 1  # a stride of a size-1 dimension is arbitrary in torch
     if n_lead == 1:
         lead = max(-(-n_inner // 16) * 16, 16)
-    if inner != 1 or lead % 16 != 0 or lead < n_inner or t.data_ptr() % 16 != 0:
+    if inner != 1 or lead % 16 != 0 or lead < n_inner:
         raise ValueError(
             f"{name} does not satisfy the layout requirements for a {'column' if transposed else 'row'}-major input: expected "
             f"stride({0 if transposed else 1}) == 1 and a 16-byte-aligned data pointer and leading stride; "
-            f"got shape={tuple(t.shape)} and stride={t.stride()}"
+            f"got shape={tuple(shape)} and stride={stride}"
         )
     return lead
 
 
-def _check_scale(name: str, s: torch.Tensor, rows: int, kb: int, have_rows: int, have_kb: int) -> int:
+def _check_scale(name: str, dtype, have_rows: int, have_kb: int, rows: int, kb: int) -> int:
     """1 when the scale is one per 128 rows, 0 when one per row."""
-    if s.dtype is not torch.float32 or have_kb != kb or have_rows != rows and have_rows != _blocks(rows):
+    if dtype is not torch.float32 or have_kb != kb or have_rows != rows and have_rows != _blocks(rows):
         raise ValueError(
             f"{name} must be a float32 tensor with one scale per block of {GROUP} along K and per row (column) or block of {GROUP}: "
-            f"expected {rows} or {_blocks(rows)} and {kb}, got shape {tuple(s.shape)}, {s.dtype}"
+            f"expected {rows} or {_blocks(rows)} and {kb}, got {have_rows} and {have_kb}, {dtype}"
         )
     return 0 if have_rows == rows else 1
 
 
-def _arguments(a, a_scale, b, b_scale, out_ptr, out_dtype, bias, layout, user_kwargs, num_sms, status) -> bytes:
-    """Checks the operands and packs a b200_gemm_a8w8_args."""
-    a_t, b_t = _LAYOUTS[layout]
-    m, k = a.shape
-    n = b.shape[1]
-    kb = _blocks(k)
-    if a.dtype not in _F8_ID or b.dtype not in _F8_ID:
-        raise ValueError(f"gemm_a8w8 takes float8_e4m3fn or float8_e5m2 operands, got {a.dtype} and {b.dtype}")
-    lda, ldb = _check_operand("A", a, a_t), _check_operand("B", b, b_t)
-    sa_rows, sa_kbs = a_scale.shape
-    sb_kbs, sb_cols = b_scale.shape
-    a_block = _check_scale("a_scale", a_scale, m, kb, sa_rows, sa_kbs)
-    b_block = _check_scale("b_scale", b_scale, n, kb, sb_cols, sb_kbs)
-    sa_row, sa_kb = a_scale.stride()
-    sb_kb, sb_col = b_scale.stride()
-    return _ARGS.pack(
-        a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), out_ptr, 0 if bias is None else bias.data_ptr(),
-        m, n, k, lda, ldb, n, sa_row, sa_kb, sb_col, sb_kb,
-        a_t, b_t, _F8_ID[a.dtype], _F8_ID[b.dtype], a_block, b_block, _F_ID[out_dtype], 0 if bias is None else _F_ID[bias.dtype],
-        *_policy(m, n, k, a_t, b_t, user_kwargs, num_sms), status)
-
-
-def _layout(layout: str) -> str:
-    low = layout.lower()
-    if low not in _LAYOUTS:
+@functools.lru_cache(maxsize=4096)
+def _call_plan(a_shape, a_stride, a_dtype, b_shape, b_stride, b_dtype, sa_shape, sa_stride, sa_dtype, sb_shape, sb_stride, sb_dtype,
+               out_dtype, bias_dtype, layout, kwargs, num_sms) -> tuple:
+    """(m, n, k, sizes of the argument block) of a call with operands of these shapes, strides and types; raises what the call
+    raises. Everything here follows from the sizes, so a repeated call pays for it once."""
+    if layout not in _LAYOUTS:
         raise ValueError(f"unsupported GEMM layout: {layout!r}; expected 'nn', 'nt', 'tn', or 'tt'")
-    return low
+    a_t, b_t = _LAYOUTS[layout]
+    assert len(a_shape) == len(b_shape) == len(sa_shape) == len(sb_shape) == 2, "operands and scales are matrices"
+    (m, k), n = a_shape, b_shape[1]
+    assert b_shape[0] == k, f"A is {tuple(a_shape)}, B is {tuple(b_shape)}"
+    if a_dtype not in _F8_ID or b_dtype not in _F8_ID:
+        raise ValueError(f"gemm_a8w8 takes float8_e4m3fn or float8_e5m2 operands, got {a_dtype} and {b_dtype}")
+    if out_dtype not in _F_ID:
+        raise ValueError(f"unsupported output dtype {out_dtype}; expected float32, bfloat16 or float16")
+    if bias_dtype is not None and bias_dtype not in _F_ID:
+        raise ValueError(f"unsupported bias dtype {bias_dtype}; expected float32, bfloat16 or float16")
+    kb = _blocks(k)
+    a_block = _check_scale("a_scale", sa_dtype, sa_shape[0], sa_shape[1], m, kb)
+    b_block = _check_scale("b_scale", sb_dtype, sb_shape[1], sb_shape[0], n, kb)
+    policy = _policy(m, n, k, a_t, b_t, dict(kwargs), num_sms)
+    if not (m and n and k):
+        return m, n, k, None
+    sizes = _SIZES.pack(
+        m, n, k, _leading("A", a_shape, a_stride, a_t), _leading("B", b_shape, b_stride, b_t), n, *sa_stride, sb_stride[1], sb_stride[0],
+        a_t, b_t, _F8_ID[a_dtype], _F8_ID[b_dtype], a_block, b_block, _F_ID[out_dtype], 0 if bias_dtype is None else _F_ID[bias_dtype],
+        *policy)
+    return m, n, k, sizes
+
+
+def _plan_of(a, a_scale, b, b_scale, out_dtype, bias_dtype, layout, user_kwargs, num_sms) -> tuple:
+    return _call_plan(a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype, a_scale.shape, a_scale.stride(), a_scale.dtype,
+                      b_scale.shape, b_scale.stride(), b_scale.dtype, out_dtype, bias_dtype, layout.lower(),
+                      tuple(user_kwargs.items()) if user_kwargs else (), num_sms)
+
+
+def _launch_gemm(a, a_scale, b, b_scale, out, bias, out_dtype, m, n, k, sizes, index) -> torch.Tensor:
+    """On the current device and stream."""
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    elif out.shape != (m, n):
+        out = out.view(m, n)
+    if sizes is None:
+        return out if m == 0 or n == 0 else out.zero_() if bias is None else out.copy_(bias.expand(m, n))
+    bias_ptr = 0
+    if bias is not None:
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    stream_ptr = raw_stream(index)
+    args = (_POINTERS.pack(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), out.data_ptr(), bias_ptr) + sizes
+            + _workspace_for(a.device, stream_ptr).status_bytes)
+    rc = _lib.fast("b200_gemm_a8w8")(args, stream_ptr)
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_a8w8 failed ({rc}): {_lib.strerror(rc)}")
+    return out
 
 
 def gemm_a8w8(
@@ -177,54 +206,33 @@ def gemm_a8w8(
 
     user_kwargs: tile_n (16, 32, 64, 128; with cta_group 2: 128, 256), cta_group, split_k (K blocks of a tile over the CTAs of a
     cluster), swap_ab, group_m, max_ctas, pdl, wait_limit_us; without tile_n the tiling is chosen by `heuristic_a8w8`."""
-    layout = _layout(layout)
-    assert a.ndim == 2 and b.ndim == 2 and a_scale.ndim == 2 and b_scale.ndim == 2, "operands and scales are matrices"
-    m, k = a.shape
-    n = b.shape[1]
-    assert b.shape[0] == k, f"A is {tuple(a.shape)}, B is {tuple(b.shape)}"
-    device = a.device
-    if b.device != device or a_scale.device != device or b_scale.device != device:
-        raise ValueError(f"operands and scales are on different devices: {device}, {b.device}, {a_scale.device}, {b_scale.device}")
+    index = a.get_device()
     if out_dtype is None:
         out_dtype = torch.bfloat16 if out is None else out.dtype
-    if out_dtype not in _F_ID:
-        raise ValueError(f"unsupported output dtype {out_dtype}; expected float32, bfloat16 or float16")
+    m, n, k, sizes = _plan_of(a, a_scale, b, b_scale, out_dtype, None if bias is None else bias.dtype, layout, user_kwargs,
+                              device_sms(index) if index >= 0 else 148)
+    if b.get_device() != index or a_scale.get_device() != index or b_scale.get_device() != index:
+        raise ValueError(f"operands and scales are on different devices: {a.device}, {b.device}, {a_scale.device}, {b_scale.device}")
     if bias is not None:
-        if bias.dtype not in _F_ID:
-            raise ValueError(f"unsupported bias dtype {bias.dtype}; expected float32, bfloat16 or float16")
-        assert bias.ndim == 1 and bias.shape[0] == n and bias.device == device
+        assert bias.ndim == 1 and bias.shape[0] == n and bias.get_device() == index
     if out is not None:
         assert out.dtype == out_dtype
-        assert out.device == device
+        assert out.get_device() == index
         assert out.is_contiguous()
         assert out.numel() == m * n, f"out has {out.numel()} elements, the product {m * n}"
-    if not a.is_cuda:
-        _arguments(a, a_scale, b, b_scale, 0, out_dtype, bias, layout, user_kwargs, 148, 0)
-        raise AssertionError("gemm_a8w8 runs on CUDA tensors only (there is no CPU path)")
-    index = device.index
+    if sizes is not None and (a.data_ptr() | b.data_ptr()) & 15:
+        raise ValueError("A and B must start on a 16-byte-aligned address")
+    assert index >= 0, "gemm_a8w8 runs on CUDA tensors only (there is no CPU path)"
+    if stream is None and is_current(index):
+        return _launch_gemm(a, a_scale, b, b_scale, out, bias, out_dtype, m, n, k, sizes, index)
     with on_device(index, stream):
-        if out is None:
-            out = torch.empty(m, n, dtype=out_dtype, device=device)
-        elif out.shape != (m, n):
-            out = out.view(m, n)
-        if bias is not None and not bias.is_contiguous():
-            bias = bias.contiguous()
-        if m == 0 or n == 0:
-            return out
-        if k == 0:
-            return out.zero_() if bias is None else out.copy_(bias.expand(m, n))
-        stream_ptr = raw_stream(index)
-        args = _arguments(a, a_scale, b, b_scale, out.data_ptr(), out_dtype, bias, layout, user_kwargs, device_sms(index),
-                          _workspace_for(device, stream_ptr).status_ptr)
-        rc = _lib.fast("b200_gemm_a8w8")(args, stream_ptr)
-    if rc != 0:
-        raise RuntimeError(f"b200_gemm_a8w8 failed ({rc}): {_lib.strerror(rc)}")
-    return out
+        return _launch_gemm(a, a_scale, b, b_scale, out, bias, out_dtype, m, n, k, sizes, index)
 
 
 def plan(a, a_scale, b, b_scale, layout="nt", user_kwargs: dict = {}, out_dtype=torch.bfloat16) -> dict:
     """What a call with these arguments would launch (tile, cluster split, grid, shared memory)."""
-    raw = _arguments(a, a_scale, b, b_scale, 0, out_dtype, None, _layout(layout), user_kwargs, 148, 0)
+    sizes = _plan_of(a, a_scale, b, b_scale, out_dtype, None, layout, user_kwargs, 148)[3]
+    raw = _POINTERS.pack(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), 0, 0) + (sizes or bytes(_SIZES.size)) + bytes(8)
     pl = _lib.Plan()
     rc = _lib.load().b200_gemm_a8w8_plan_query(C.byref(_lib.Args8.from_buffer_copy(raw)), C.byref(pl))
     if rc != 0:
@@ -233,59 +241,62 @@ def plan(a, a_scale, b, b_scale, layout="nt", user_kwargs: dict = {}, out_dtype=
 
 
 # --------------------------------------------------------------------------------------------------------- quantizer
-def _pitched(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
-    """[rows, cols] with rows that start on 16-byte boundaries."""
-    if cols % 16 == 0:
-        return torch.empty(rows, cols, dtype=dtype, device=device)
-    return torch.empty(rows, -(-cols // 16) * 16, dtype=dtype, device=device)[:, :cols]
+def _up(n: int, to: int) -> int:
+    return -(-n // to) * to
 
 
-def _is_row_major(x: torch.Tensor) -> bool:
-    rows, cols = x.shape
-    return (cols <= 1 or x.stride(1) == 1) and (rows <= 1 or x.stride(0) >= cols)
+def _row_major_strides(rows: int, cols: int, stride) -> bool:
+    return (cols <= 1 or stride[1] == 1) and (rows <= 1 or stride[0] >= cols)
 
 
 def _row_major(x: torch.Tensor) -> torch.Tensor:
-    return x if _is_row_major(x) else x.contiguous()
+    return x if _row_major_strides(*x.shape, x.stride()) else x.contiguous()
 
 
 _QUANT_ARGS = struct.Struct("@P3q4i" + "PqP2q" * 2 + "Pq")  # b200_gemm_quantize_args
 _GROUPS = {"row": 1, "col": 2, "both": 3, "block": 4}
 
 
-def _quantize(x, group, dtype, stream):
+@functools.lru_cache(maxsize=4096)
+def _quantize_plan(shape, stride, x_dtype, group, dtype) -> tuple:
+    """(mode, shapes and strides of the outputs, parts of the argument block) for an input of this shape; raises what the call
+    raises."""
     if group not in _GROUPS:
         raise ValueError(f"unknown group {group!r}; expected one of {tuple(_GROUPS)}")
     if dtype not in _F8_ID:
         raise ValueError(f"quantize_a8 makes float8_e4m3fn or float8_e5m2, not {dtype}")
-    if x.dtype not in _F_ID:
-        raise ValueError(f"quantize_a8 takes float32, bfloat16 or float16, not {x.dtype}")
-    assert x.ndim == 2, f"quantize_a8 takes a matrix, got {x.ndim} dimensions"
-    rows, cols = x.shape
-    if not _is_row_major(x):
-        raise ValueError(f"x must be row-major: expected stride(1) == 1; got shape={tuple(x.shape)} and stride={x.stride()}")
-    assert x.is_cuda, "quantize_a8 runs on CUDA tensors only (there is no CPU path)"
+    if x_dtype not in _F_ID:
+        raise ValueError(f"quantize_a8 takes float32, bfloat16 or float16, not {x_dtype}")
+    assert len(shape) == 2, f"quantize_a8 takes a matrix, got {len(shape)} dimensions"
+    rows, cols = shape
+    if not _row_major_strides(rows, cols, stride):
+        raise ValueError(f"x must be row-major: expected stride(1) == 1; got shape={tuple(shape)} and stride={stride}")
+    mode, pitch = _GROUPS[group], _up(cols, 16)
+    head = (rows, cols, stride[0] if rows > 1 else cols, _F_ID[x_dtype], _F8_ID[dtype], mode, 0)
+    n_rows = _blocks(rows) if mode == 4 else rows
+    # the product reads the scales of 128 rows at a time: rows are the contiguous dimension
+    row = ((n_rows, _blocks(cols)), (1, n_rows)) if mode != 2 else None
+    col = (_blocks(rows), cols) if mode in (2, 3) else None
+    return rows, cols, pitch, head, row, col
+
+
+def _launch_quantize(x, dtype, plan, index) -> tuple:
+    """On the current device and stream."""
+    rows, cols, pitch, head, row, col = plan
     device = x.device
-    index = device.index
-    mode = _GROUPS[group]
     got = []
-    row = col = (0, 0, 0, 0, 0)
-    with on_device(index, stream):
-        if mode != 2:
-            q = _pitched(rows, cols, dtype, device)
-            # the product reads the scales of 128 rows at a time: rows are the contiguous dimension
-            n_rows = _blocks(rows) if mode == 4 else rows
-            s = torch.empty_strided((n_rows, _blocks(cols)), (1, n_rows), dtype=torch.float32, device=device)
-            row = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), 1, n_rows)
-            got += [q, s]
-        if mode == 2 or mode == 3:
-            q = _pitched(rows, cols, dtype, device)
-            s = torch.empty(_blocks(rows), cols, dtype=torch.float32, device=device)
-            col = (q.data_ptr(), -(-cols // 16) * 16, s.data_ptr(), cols, 1)
-            got += [q, s]
-        args = _QUANT_ARGS.pack(x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, _F_ID[x.dtype], _F8_ID[dtype], mode, 0,
-                                *row, *col, 0, 0)
-        rc = _lib.fast("b200_gemm_quantize_a8")(args, raw_stream(index))
+    row_args = col_args = (0, 0, 0, 0, 0)
+    if row is not None:
+        q = torch.empty(rows, pitch, dtype=dtype, device=device)
+        s = torch.empty_strided(*row, dtype=torch.float32, device=device)
+        row_args = (q.data_ptr(), pitch, s.data_ptr(), 1, row[0][0])
+        got += [q if pitch == cols else q[:, :cols], s]
+    if col is not None:
+        q = torch.empty(rows, pitch, dtype=dtype, device=device)
+        s = torch.empty(*col, dtype=torch.float32, device=device)
+        col_args = (q.data_ptr(), pitch, s.data_ptr(), cols, 1)
+        got += [q if pitch == cols else q[:, :cols], s]
+    rc = _lib.fast("b200_gemm_quantize_a8")(_QUANT_ARGS.pack(x.data_ptr(), *head, *row_args, *col_args, 0, 0), raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
     return tuple(got)
@@ -302,147 +313,175 @@ def quantize_a8(x: torch.Tensor, group: str = "row", dtype: torch.dtype = torch.
     A group's scale is the smallest power of two (at least 2^-126) that brings its largest finite magnitude to the format's
     largest value or below; 1 for a group of zeros. q is x / s rounded to nearest even, the only rounding. NaN stays NaN; an
     infinity becomes NaN in e4m3 and stays infinite in e5m2; neither changes its group's scale. Asynchronous on `stream`."""
-    return _quantize(x, group, dtype, stream)
+    plan = _quantize_plan(x.shape, x.stride(), x.dtype, group, dtype)
+    index = x.get_device()
+    assert index >= 0, "quantize_a8 runs on CUDA tensors only (there is no CPU path)"
+    if stream is None and is_current(index):
+        return _launch_quantize(x, dtype, plan, index)
+    with on_device(index, stream):
+        return _launch_quantize(x, dtype, plan, index)
 
 
 # ------------------------------------------------------------------------------------------------------ linear layer
 # A step of the layer is eight launches, and a launch through the public calls costs the host more than the GPU needs for it at
-# ordinary sizes. The layer checks its tensors once, keeps each pass's operands in one buffer and packs the argument blocks
-# itself.
-def _up(n: int, to: int) -> int:
-    return -(-n // to) * to
-
-
-class _Buffer:
+# ordinary sizes. The layer checks its tensors once, keeps each pass's operands in one buffer, and works out sizes,
+# offsets and argument blocks once per combination of sizes and types (`_forward_plan`, `_backward_plan`).
+class _Pieces:
     """Offsets of the pieces of one allocation, each on a 256-byte boundary."""
 
-    __slots__ = ("at", "size")
+    def __init__(self):
+        self.size = 0
 
-    def __init__(self, *sizes: int):
-        self.at, self.size = [], 0
-        for n in sizes:
-            self.at.append(self.size)
-            self.size += _up(n, 256)
+    def add(self, nbytes: int) -> int:
+        at = self.size
+        self.size += _up(nbytes, 256)
+        return at
 
-
-@functools.lru_cache(maxsize=1024)
-def _quantized(rows: int, cols: int, row: bool, col: bool, block: bool) -> _Buffer:
-    """Values (pitch a multiple of 16) and scales of each kind that is asked for, in this order."""
-    values, sizes = rows * _up(cols, 16), []
-    if row:
-        sizes += [values, 4 * rows * _blocks(cols)]
-    if col:
-        sizes += [values, 4 * _blocks(rows) * cols]
-    if block:
-        sizes += [values, 4 * _blocks(rows) * _blocks(cols)]
-    return _Buffer(*sizes)
+    def quantized(self, rows: int, cols: int, groups: str) -> tuple:
+        """(values, scales) of a matrix; the values' pitch is a multiple of 16."""
+        n = {"row": rows * _blocks(cols), "col": _blocks(rows) * cols, "block": _blocks(rows) * _blocks(cols)}[groups]
+        return self.add(rows * _up(cols, 16)), self.add(4 * n)
 
 
-def _check(rc: int, name: str) -> None:
-    if rc != 0:
-        raise RuntimeError(f"{name} failed ({rc}): {_lib.strerror(rc)}")
-
-
-def _quantize_at(x, f8_id, row_at, col_at, block_at, sums, stream) -> None:
-    """Quantizes a row-major matrix to device addresses (0: not wanted), laid out as `_quantized` has them."""
-    rows, cols = x.shape
-    if rows == 0 or cols == 0:
-        return
+def _quant_sizes(rows, cols, ld, in_id, out_id, mode) -> tuple:
+    """The constant members of a b200_gemm_quantize_args: the head, then pitch and scale strides of the rows' and the columns'
+    outputs (which mode needs them is the kernel's business)."""
     pitch = _up(cols, 16)
-    mode = 4 if block_at else (1 if row_at else 0) + (2 if col_at else 0)
-    q = rows * pitch
-    row = (block_at or row_at, pitch, (block_at or row_at) + _up(q, 256), 1, _blocks(rows) if block_at else rows) if mode != 2 else (0,) * 5
-    col = (col_at, pitch, col_at + _up(q, 256), cols, 1) if mode in (2, 3) else (0,) * 5
-    args = _QUANT_ARGS.pack(x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols, _F_ID[x.dtype], f8_id, mode, 0, *row, *col, *sums)
-    _check(_lib.fast("b200_gemm_quantize_a8")(args, stream), "b200_gemm_quantize_a8")
+    return (rows, cols, ld, in_id, out_id, mode, 0), pitch, (1, _blocks(rows) if mode == 4 else rows), (cols, 1)
 
 
-def _gemm_at(pointers, m, n, k, lda, ldb, scale_strides, a_t, b_t, a_id, b_id, b_block, out_id, bias_id, index, status, stream) -> None:
-    """b200_gemm_a8w8 on device addresses; pointers: a, b, a_scale, b_scale, out, bias."""
-    if m == 0 or n == 0:
-        return
-    args = _ARGS.pack(*pointers, m, n, k, lda, ldb, n, *scale_strides, a_t, b_t, a_id, b_id, 0, b_block, out_id, bias_id,
-                      *_policy(m, n, k, a_t, b_t, {}, device_sms(index)), status)
-    _check(_lib.fast("b200_gemm_a8w8")(args, stream), "b200_gemm_a8w8")
+def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
+    """row, col: device addresses of (values, scales)."""
+    head, pitch, row_strides, col_strides = sizes
+    args = _QUANT_ARGS.pack(x_ptr, *head, row[0], pitch, row[1], *row_strides, col[0], pitch, col[1], *col_strides, *sums)
+    rc = _lib.fast("b200_gemm_quantize_a8")(args, stream)
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
+
+
+def _gemm_sizes(m, n, k, lda, ldb, scale_strides, a_t, b_t, a_id, b_id, b_block, out_id, bias_id, num_sms) -> bytes:
+    return _SIZES.pack(m, n, k, lda, ldb, n, *scale_strides, a_t, b_t, a_id, b_id, 0, b_block, out_id, bias_id,
+                       *_policy(m, n, k, a_t, b_t, {}, num_sms))
+
+
+def _call_gemm(pointers, sizes, status, stream) -> None:
+    """pointers: a, b, a_scale, b_scale, out, bias."""
+    rc = _lib.fast("b200_gemm_a8w8")(_POINTERS.pack(*pointers) + sizes + status, stream)
+    if rc != 0:
+        raise RuntimeError(f"b200_gemm_a8w8 failed ({rc}): {_lib.strerror(rc)}")
+
+
+class _ForwardPlan:
+    def __init__(self, m, n, k, x_ld, x_dtype, w_ld, w_dtype, bias_dtype, need_x, need_w, num_sms):
+        e4 = _lib.DTYPE_E4M3
+        temp, keep = _Pieces(), _Pieces()
+        self.xr = temp.quantized(m, k, "row")
+        # what the backward pass reads: x by columns and the weight, as far as they are needed
+        self.xc = keep.quantized(m, k, "col") if need_w else None
+        self.wq = (keep if need_x else temp).quantized(n, k, "block")
+        self.temp_size, self.keep_size = temp.size, keep.size
+        self.quant_x = _quant_sizes(m, k, x_ld, _F_ID[x_dtype], e4, 3 if need_w else 1)
+        self.quant_w = _quant_sizes(n, k, w_ld, _F_ID[w_dtype], e4, 4)
+        kp = _up(k, 16)
+        self.gemm = _gemm_sizes(m, n, k, kp, kp, (1, m, 1, _blocks(n)), False, True, e4, e4, 1, _F_ID[x_dtype],
+                                0 if bias_dtype is None else _F_ID[bias_dtype], num_sms) if m and n and k else None
+
+
+class _BackwardPlan:
+    def __init__(self, m, n, k, g_ld, g_dtype, g_id, x_dtype, w_dtype, need_x, need_w, need_b, num_sms):
+        e4 = _lib.DTYPE_E4M3
+        temp = _Pieces()
+        by_col = need_w or need_b
+        self.gr = temp.quantized(m, n, "row") if need_x else None
+        self.gc = temp.quantized(m, n, "col") if by_col else None
+        self.pitch = _up(n, 4)
+        self.sums = temp.add(4 * _blocks(m) * self.pitch) if need_b else None
+        self.temp_size = temp.size
+        self.quant = _quant_sizes(m, n, g_ld, _F_ID[g_dtype], g_id, 3 if need_x and by_col else 2 if by_col else 1) if m and n else None
+        np_, kp, full = _up(n, 16), _up(k, 16), m and n and k
+        self.dx = _gemm_sizes(m, k, n, np_, kp, (1, m, _blocks(n), 1), False, False, g_id, e4, 1, _F_ID[x_dtype], 0, num_sms) if full else None
+        self.dw = _gemm_sizes(n, k, m, np_, kp, (1, n, 1, k), True, False, g_id, e4, 0, _F_ID[w_dtype], 0, num_sms) if full else None
+
+
+_forward_plan = functools.lru_cache(maxsize=1024)(_ForwardPlan)
+_backward_plan = functools.lru_cache(maxsize=1024)(_BackwardPlan)
+
+
+def _at(base: int, offsets) -> tuple:
+    return (0, 0) if offsets is None else (base + offsets[0], base + offsets[1])
 
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, grad_dtype):
-        k, n = x.shape[-1], weight.shape[0]
-        x2, w2 = _row_major(x.reshape(-1, k)), _row_major(weight)
+        shape, (n, k) = x.shape, weight.shape
+        x2, w2 = _row_major(x if x.ndim == 2 else x.reshape(-1, k)), _row_major(weight)
         m = x2.shape[0]
         need_x, need_w = ctx.needs_input_grad[:2]
-        index, device, e4 = x.get_device(), x.device, _lib.DTYPE_E4M3
-        kp, mb, nb, kb = _up(k, 16), _blocks(m), _blocks(n), _blocks(k)
+        index, device = x.get_device(), x.device
+        bias_dtype = None if bias is None else bias.dtype
+        plan = _forward_plan(m, n, k, x2.stride(0) if m > 1 else k, x.dtype, w2.stride(0) if n > 1 else k, weight.dtype, bias_dtype, need_x,
+                             need_w, device_sms(index))
         with on_device(index, None):
             stream = raw_stream(index)
-            y = torch.empty(m, n, dtype=x.dtype, device=device)
-            rows, cols, blocks = _quantized(m, k, True, False, False), _quantized(m, k, False, True, False), _quantized(n, k, False, False, True)
-            # what the backward pass reads: x by columns and the weight, as far as they are needed
-            keep = _Buffer(cols.size if need_w else 0, blocks.size if need_x else 0)
-            temp = torch.empty(rows.size + (0 if need_x else blocks.size), dtype=torch.uint8, device=device)
-            saved = torch.empty(keep.size, dtype=torch.uint8, device=device)
-            xr = temp.data_ptr()
-            xc = saved.data_ptr() if need_w else 0
-            wq = saved.data_ptr() + keep.at[1] if need_x else xr + rows.size
-            if k == 0:
-                y.copy_(0 if bias is None else bias.expand(m, n))
-            else:
-                _quantize_at(x2, e4, xr, xc, 0, (0, 0), stream)
-                _quantize_at(w2, e4, 0, 0, wq, (0, 0), stream)
-                _gemm_at((xr, wq, xr + rows.at[1], wq + blocks.at[1], y.data_ptr(), 0 if bias is None else bias.data_ptr()), m, n, k, kp, kp,
-                         (1, m, 1, nb), False, True, e4, e4, 1, _F_ID[x.dtype], 0 if bias is None else _F_ID[bias.dtype], index,
-                         _workspace_for(device, stream).status_ptr, stream)
-        ctx.save_for_backward(saved)
-        ctx.meta = (x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype, _F8_ID[grad_dtype], m, n, k, keep, cols, blocks)
-        return y.view(*x.shape[:-1], n)
+            y = torch.empty(*shape[:-1], n, dtype=x.dtype, device=device)
+            keep = torch.empty(plan.keep_size, dtype=torch.uint8, device=device)
+            if plan.gemm is not None:
+                temp = torch.empty(plan.temp_size, dtype=torch.uint8, device=device)
+                temp_ptr, keep_ptr = temp.data_ptr(), keep.data_ptr()
+                xr, wq = _at(temp_ptr, plan.xr), _at(keep_ptr if need_x else temp_ptr, plan.wq)
+                _call_quantize(x2.data_ptr(), plan.quant_x, xr, _at(keep_ptr, plan.xc), (0, 0), stream)
+                _call_quantize(w2.data_ptr(), plan.quant_w, wq, (0, 0), (0, 0), stream)
+                _call_gemm((xr[0], wq[0], xr[1], wq[1], y.data_ptr(), 0 if bias is None else bias.data_ptr()), plan.gemm,
+                           _workspace_for(device, stream).status_bytes, stream)
+            elif k == 0:
+                y.zero_() if bias is None else y.copy_(bias.expand_as(y))
+        ctx.save_for_backward(keep)
+        ctx.plan = plan
+        ctx.meta = (shape, m, n, k, x.dtype, weight.dtype, bias_dtype, _F8_ID[grad_dtype])
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        (saved,) = ctx.saved_tensors
-        shape, x_dtype, w_dtype, b_dtype, g_id, m, n, k, keep, cols, blocks = ctx.meta
+        (keep,) = ctx.saved_tensors
+        shape, m, n, k, x_dtype, w_dtype, b_dtype, g_id = ctx.meta
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        g = _row_major(dy.reshape(m, n))  # an expanded gradient (of a sum) is spread out here
-        index, device, e4 = dy.get_device(), dy.device, _lib.DTYPE_E4M3
-        np_, kp, mb, nb = _up(n, 16), _up(k, 16), _blocks(m), _blocks(n)
-        by_col = need_w or need_b
+        g = _row_major(dy if dy.ndim == 2 else dy.reshape(m, n))  # an expanded gradient (of a sum) is spread out here
+        index, device = dy.get_device(), dy.device
+        plan = _backward_plan(m, n, k, g.stride(0) if m > 1 else n, g.dtype, g_id, x_dtype, w_dtype, need_x, need_w, need_b, device_sms(index))
         dx = dw = db = None
         with on_device(index, None):
             stream = raw_stream(index)
-            status = _workspace_for(device, stream).status_ptr
-            grows, gcols = _quantized(m, n, True, False, False), _quantized(m, n, False, True, False)
-            pitch = _up(n, 4)
-            parts = _Buffer(grows.size if need_x else 0, gcols.size if by_col else 0, 4 * mb * pitch if need_b else 0)
-            temp = torch.empty(parts.size, dtype=torch.uint8, device=device)
-            gr, gc, sums = (temp.data_ptr() + at for at in parts.at)
-            if by_col or need_x:
-                _quantize_at(g, g_id, gr if need_x else 0, gc if by_col else 0, 0, (sums, pitch) if need_b else (0, 0), stream)
+            status = _workspace_for(device, stream).status_bytes
+            temp = torch.empty(plan.temp_size, dtype=torch.uint8, device=device)
+            base, keep_ptr = temp.data_ptr(), keep.data_ptr()
+            gr, gc = _at(base, plan.gr), _at(base, plan.gc)
+            if plan.quant is not None and (need_x or need_w or need_b):
+                _call_quantize(g.data_ptr(), plan.quant, gr, gc, (base + plan.sums, plan.pitch) if need_b else (0, 0), stream)
             if need_x:
-                dx = torch.empty(m, k, dtype=x_dtype, device=device)
-                if n == 0:
+                dx = torch.empty(shape, dtype=x_dtype, device=device)
+                if plan.dx is not None:
+                    wq = _at(keep_ptr, ctx.plan.wq)
+                    _call_gemm((gr[0], wq[0], gr[1], wq[1], dx.data_ptr(), 0), plan.dx, status, stream)
+                else:
                     dx.zero_()
-                elif k:
-                    wq = saved.data_ptr() + keep.at[1]
-                    _gemm_at((gr, wq, gr + grows.at[1], wq + blocks.at[1], dx.data_ptr(), 0), m, k, n, np_, kp, (1, m, nb, 1), False, False,
-                             g_id, e4, 1, _F_ID[x_dtype], 0, index, status, stream)
-                dx = dx.view(shape)
             if need_w:
                 dw = torch.empty(n, k, dtype=w_dtype, device=device)
-                if m == 0:
+                if plan.dw is not None:
+                    xc = _at(keep_ptr, ctx.plan.xc)
+                    _call_gemm((gc[0], xc[0], gc[1], xc[1], dw.data_ptr(), 0), plan.dw, status, stream)
+                else:
                     dw.zero_()
-                elif k:
-                    xc = saved.data_ptr()
-                    _gemm_at((gc, xc, gc + gcols.at[1], xc + cols.at[1], dw.data_ptr(), 0), n, k, m, np_, kp, (1, n, 1, k), True, False,
-                             g_id, e4, 0, _F_ID[w_dtype], 0, index, status, stream)
             if need_b:
-                db = torch.empty(pitch, dtype=b_dtype, device=device)
-                if m == 0:
+                db = torch.empty(plan.pitch, dtype=b_dtype, device=device)
+                if plan.quant is not None:  # the columns' sums over each 128 rows, added in order
+                    rc = _lib.load().b200_gemm_reduce_slots(base + plan.sums, plan.pitch, _blocks(m), db.data_ptr(), None, 1, plan.pitch,
+                                                            _F_ID[b_dtype], 0, stream)
+                    if rc != 0:
+                        raise RuntimeError(f"b200_gemm_reduce_slots failed ({rc}): {_lib.strerror(rc)}")
+                else:
                     db.zero_()
-                elif n:  # the columns' sums over each 128 rows, added in order
-                    _check(_lib.load().b200_gemm_reduce_slots(sums, pitch, mb, db.data_ptr(), None, 1, pitch, _F_ID[b_dtype], 0, stream),
-                           "b200_gemm_reduce_slots")
                 db = db[:n]
         return dx, dw, db, None
 

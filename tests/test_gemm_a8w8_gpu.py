@@ -378,3 +378,69 @@ def test_no_offset_over_32_bits_wraps():
     q, s = quantize_a8(got, "both")[:2]
     q2, s2 = quantize_a8(got[m - 256:].contiguous(), "row")
     assert same8(q[m - 256:], q2) and torch.equal(s[m - 256:], s2)
+
+
+def test_linear_captured_with_its_backward_and_changed_in_place():
+    g = torch.Generator(device=DEV).manual_seed(12)
+    x = torch.randn(130, 256, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randn(200, 256, generator=g, device=DEV).to(torch.bfloat16)
+    b = torch.randn(200, generator=g, device=DEV).to(torch.bfloat16)
+    dy = torch.randn(130, 200, generator=g, device=DEV).to(torch.bfloat16)
+
+    def step(x_, w_, b_):
+        leaves = [t.detach().requires_grad_() for t in (x_, w_, b_)]
+        y = linear_a8w8(*leaves)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+    want = step(x, w, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w, b)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, w, b)
+    for t in got:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    x.copy_(x.flip(0).contiguous())
+    dy.copy_(dy.flip(0).contiguous())
+    graph.replay()
+    again = step(x, w, b)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+    xl = x.clone().requires_grad_()
+    y = linear_a8w8(xl, w, b)
+    y.relu_()  # the output is no view, so it may be changed in place
+    y.sum().backward()
+    assert xl.grad.isfinite().all()
+    check_status()
+
+
+def test_threads_share_the_calls():
+    import threading
+
+    g = torch.Generator(device=DEV).manual_seed(13)
+    a, sa = operand(g, 50, 512, E4, False, False)
+    b, sb = operand(g, 300, 512, E4, True, False)
+    x = torch.randn(50, 512, generator=g, device=DEV)
+    want, want_q = gemm_a8w8(a, sa, b.t(), sb.t()), quantize_a8(x, "both")
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got, q = gemm_a8w8(a, sa, b.t(), sb.t()), quantize_a8(x, "both")
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want) or not all(torch.equal(p.float(), r.float()) for p, r in zip(q, want_q)):
+                    bad.append(1)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    check_status()

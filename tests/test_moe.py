@@ -86,7 +86,7 @@ def test_python_refusals():
         moe_a16w16(x, logits, w13, w2[:, :56], 2)
     with pytest.raises(ValueError, match="w13"):
         moe_a16w16(x, logits, w13.transpose(1, 2), w2, 2)
-    with pytest.raises(ValueError, match="x must"):
+    with pytest.raises(ValueError, match="16-byte"):
         moe_a16w16(torch.zeros(4, 72, dtype=bf)[:, 4:68], logits, w13, w2, 2)
     with pytest.raises(ValueError, match="key"):
         moe_a16w16(x, logits, w13, w2, 2, user_kwargs={"tile_n": 16})
