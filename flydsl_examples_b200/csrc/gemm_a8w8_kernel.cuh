@@ -344,10 +344,12 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
 #pragma unroll
               for (int j = 0; j < k8TK / 32; ++j)
                 umma_f8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), p.idesc, j != 0 ? 1u : 0u);
-              if constexpr (CG == 2)
-                umma_commit_both(done_bar(stage));
-              else
+              if constexpr (CG == 2) {
+                umma_commit_pair(mapa_cluster(done_bar(stage), 0));
+                umma_commit_pair(mapa_cluster(done_bar(stage), 1));
+              } else {
                 umma_commit(done_bar(stage));
+              }
             }
             __syncwarp();
             if (++stage == STAGES) stage = 0, phase ^= 1u;

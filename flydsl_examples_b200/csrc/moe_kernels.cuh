@@ -11,7 +11,8 @@
 //  * Every block of the first kernel routes for itself (the logits are a few kilobytes), so routing has no launch and no pass
 //    of its own; the list of chosen experts goes to the second kernel. (The second kernel routing again, in order to fill
 //    its ring with weights while the first one's last tiles run, took 26.2 instead of 24.4 us for one token of 8 / 128
-//    experts, 169 instead of 171 us for 8 tokens of 2 / 16: its blocks mostly start when the first kernel's end.)
+//    experts, 169 instead of 171 us for 8 tokens of 2 / 16: its blocks mostly start when the first kernel's end. The first
+//    kernel asking for the down weights into L2 behind its own last loads: 28.0 instead of 24.4 us for one token.)
 //  * First kernel: a tile is 64 gate rows over 64 up rows of one expert; its epilogue computes h[slot][t][i] = p * silu(gate) *
 //    up, zero for pairs that were not chosen, with the weight of the pair folded in. h is the second product's 16-bit
 //    operand; it is stored as two of them, the rounded value and the rounded remainder, which cost that product columns

@@ -87,29 +87,6 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
   return ok != 0;
 }
 
-// Whether the phase has completed, without waiting (try_wait may suspend the thread for a while).
-template <bool kCluster = false>
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  if constexpr (kCluster)
-    asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, P;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, P;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-  return ok != 0;
-}
-
 // Bounded wait. `abort_flag` is a CTA-shared int: non-zero means some role gave up.
 // Returns false when the wait was abandoned (limit hit, or another role aborted).
 // With kPollAbort == false only the time limit ends the wait, so that all threads waiting on one barrier
@@ -292,12 +269,6 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
 // cta_group::2 form; `bar` is a shared::cluster address (may belong to the peer CTA).
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// The same for the barriers at one shared-memory offset in both CTAs of a pair (cluster ranks 0 and 1), in one instruction.
-__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-               "h"((uint16_t)3)
-               : "memory");
 }
 __device__ __forceinline__ uint32_t mapa_cluster(uint32_t addr, uint32_t cta_rank) {
   uint32_t r;
