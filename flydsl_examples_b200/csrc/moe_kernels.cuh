@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
     }
   }
   grid_dependency_wait();
-  grid_launch_dependents();
+  if (!UP) grid_launch_dependents();
   if constexpr (UP) {
     route_all(p, reinterpret_cast<uint32_t*>(sm), ids, weights, mask);  // the ring is free until the first load
     fence_proxy_async_smem();
@@ -356,6 +356,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
         if (++stage == STAGES) stage = 0, phase ^= 1u;
       }
     }
+    // The second kernel may take the SMs that this one leaves; not before all of this block's loads are on their way (1 %).
+    if (UP) grid_launch_dependents();
     if (!ok && lane == 0) {  // loads in flight still write shared memory: a bounded time to land
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 1000000ull) {
