@@ -10,8 +10,10 @@
 // two in general, so the tensor core cannot apply them. Eight epilogue warps read that accumulator, multiply by
 // us[p] * vs[q] and add to the running sums, which stay in their registers for the whole tile (128 fp32 values per
 // thread of a 256-column tile). TMEM holds two (256 columns) or four accumulators, so the tensor core works on the next
-// blocks meanwhile. Per 128 x 256 half-tile and block the tensor core needs 512 cycles, the eight warps about 300 issue
-// cycles per scheduler: the product stays tensor-bound.
+// blocks meanwhile. Per 128 x 256 half-tile and block the tensor core needs 512 cycles and the eight warps about 400 issue
+// slots per scheduler; a block takes 750 to 830 cycles, the rest being the chain accumulator done -> read -> handed back ->
+// next instructions, twice deep. 8192^3: 454 us in a burst (2420 TFLOP/s), 534 us under the power cap; 2048 x 4096 x 4096:
+// 33 us; with a scale per row on both sides (two multiplications and a shared-memory read per element) 647 us.
 //
 // Roles (384 threads): warp 0 = TMA producer, warp 1 = TMEM owner and MMA issuer, warps 2-3 = scale loaders, warps 4-11 =
 // epilogue (warp w reads TMEM lanes 32 * (w % 4).. and column half (w - 4) / 4). The scale loaders copy the scales of a
@@ -193,6 +195,10 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
   // 128 running sums, 32 loaded values and addresses do not fit the 168 registers a thread of 384 gets at launch: the
   // wide tile moves registers to the epilogue, 128 * 40 + 256 * 232 = 384 * 168.
   constexpr bool kMoveRegs = HC > 64;
+  // Look for the next block's barriers before this block's last additions. It pays where those are long (256 columns with a
+  // scale each: 58.8 -> 54.2 us at 4096 x 4096 x 2048) and costs elsewhere (one scale per half: 454 -> 479 us at 8192^3; 128
+  // columns: 61 -> 64 us).
+  constexpr bool kLookAhead = VVEC && HC > 64;
   constexpr uint32_t kTxBytes = CG * L::kStageBytes;  // both CTAs of a pair count on the leader's barrier
 
   extern __shared__ uint8_t smem_raw[];
@@ -427,12 +433,13 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
 #pragma unroll
       for (int i = 0; i < HC / 2; ++i) acc2[i] = 0;
       auto acc = [&](int i) { return __uint_as_float((uint32_t)(i & 1 ? acc2[i >> 1] >> 32 : acc2[i >> 1])); };
-      bool ok = true;
+      bool ok = true, seen = false;
 #pragma unroll 1
       for (int kb = kb0; kb < p.kb_total; kb += kbstep, ++g) {
         const int buf = g % kBufs, ss = g % k8ScaleStages;
         // The verdict is the warp's: tcgen05.ld needs all its lanes.
-        if (!wait_two(sfull_bar(ss), (g / k8ScaleStages) & 1, done_bar(stage), phase, abort_s, wait_limit)) {
+        if (!(kLookAhead && __all_sync(0xffffffffu, seen)) &&
+            !wait_two(sfull_bar(ss), (g / k8ScaleStages) & 1, done_bar(stage), phase, abort_s, wait_limit)) {
           ok = false;
           break;
         }
@@ -481,7 +488,14 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
 #pragma unroll
         for (int c = 0; c < NCH; c += 2) {
           tmem_ld_wait();
-          if (c + 2 >= NCH) release();
+          if (c + 2 >= NCH) {
+            release();
+            if constexpr (kLookAhead) {
+              const int nstage = stage + 1 == STAGES ? 0 : stage + 1;
+              seen = mbar_test(sfull_bar((g + 1) % k8ScaleStages), ((g + 1) / k8ScaleStages) & 1) &&
+                     mbar_test(done_bar(nstage), nstage == 0 ? phase ^ 1u : phase);
+            }
+          }
           add_chunk(ra, c);
           if (c + 2 < NCH) load_chunk(ra, c + 2);
           if (c + 1 < NCH) add_chunk(rb, c + 1);

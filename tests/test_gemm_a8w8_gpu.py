@@ -444,3 +444,14 @@ def test_threads_share_the_calls():
         t.join()
     assert not bad
     check_status()
+
+
+@pytest.mark.parametrize("kw", [{"tile_n": 256, "cta_group": 2}, {"tile_n": 64}, {"tile_n": 16, "swap_ab": True, "split_k": 2}], ids=str)
+@pytest.mark.parametrize("bias_dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_bias_types_and_offsets(kw, bias_dtype):
+    g = torch.Generator(device=DEV).manual_seed(14)
+    a, sa = operand(g, 150, 300, E4, False, False)
+    b, sb = operand(g, 277, 300, E4, False, False)
+    wide = torch.randn(600, generator=g, device=DEV).to(bias_dtype)
+    for bias in (wide[:277], wide[3:280], wide[:554:2]):  # aligned, off 16 bytes, strided
+        check(gemm_a8w8(a, sa, b.t(), sb.t(), bias=bias, user_kwargs=kw, out_dtype=torch.float32), a, sa, b, sb, bias)
