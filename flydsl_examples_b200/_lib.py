@@ -112,28 +112,11 @@ class Args8(C.Structure):
 
 class QuantizeArgs(C.Structure):
     """b200_gemm_quantize_args"""
-    _fields_ = [
-        ("x", C.c_void_p),
-        ("rows", C.c_int64),
-        ("cols", C.c_int64),
-        ("ldx", C.c_int64),
-        ("in_dtype", C.c_int32),
-        ("out_dtype", C.c_int32),
-        ("mode", C.c_int32),
-        ("reserved", C.c_int32),
-        ("q_row", C.c_void_p),
-        ("ldq_row", C.c_int64),
-        ("s_row", C.c_void_p),
-        ("sr_row", C.c_int64),
-        ("sr_group", C.c_int64),
-        ("q_col", C.c_void_p),
-        ("ldq_col", C.c_int64),
-        ("s_col", C.c_void_p),
-        ("sc_group", C.c_int64),
-        ("sc_col", C.c_int64),
-        ("colsum", C.c_void_p),
-        ("colsum_ld", C.c_int64),
-    ]
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("x", "q_row", "s_row", "q_col", "s_col", "colsum")]
+        + [(n, C.c_int64) for n in ("rows", "cols", "ldx", "ldq_row", "sr_row", "sr_group", "ldq_col", "sc_group", "sc_col", "colsum_ld")]
+        + [(n, C.c_int32) for n in ("in_dtype", "out_dtype", "mode", "reserved")]
+    )
 
 
 class MoeArgs(C.Structure):

@@ -93,8 +93,8 @@ def _policy(m, n, k, a_t, b_t, user_kwargs, num_sms) -> tuple:
 
 # -------------------------------------------------------------------------------------------------------------- GEMM
 _LAYOUTS = {"nn": (False, False), "nt": (False, True), "tn": (True, False), "tt": (True, True)}
-_ARGS = struct.Struct("@6P10q8i16iP")  # b200_gemm_a8w8_args
-_POINTERS, _SIZES = struct.Struct("@6P"), struct.Struct("@10q8i16i")  # the same in parts; the last member is the status address
+# b200_gemm_a8w8_args in parts; the last member is the status address
+_POINTERS, _SIZES = struct.Struct("@6P"), struct.Struct("@10q8i16i")
 
 
 def _leading(name: str, shape, stride, transposed: bool) -> int:
@@ -253,8 +253,13 @@ def _row_major(x: torch.Tensor) -> torch.Tensor:
     return x if _row_major_strides(*x.shape, x.stride()) else x.contiguous()
 
 
-_QUANT_ARGS = struct.Struct("@P3q4i" + "PqP2q" * 2 + "Pq")  # b200_gemm_quantize_args
+_QUANT_SIZES = struct.Struct("@10q4i")  # b200_gemm_quantize_args behind its six pointers
 _GROUPS = {"row": 1, "col": 2, "both": 3, "block": 4}
+
+
+def _quant_sizes(rows, cols, ld, in_id, out_id, mode, sums_pitch) -> bytes:
+    pitch = _up(cols, 16)
+    return _QUANT_SIZES.pack(rows, cols, ld, pitch, 1, _blocks(rows) if mode == 4 else rows, pitch, cols, 1, sums_pitch, in_id, out_id, mode, 0)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -272,31 +277,31 @@ def _quantize_plan(shape, stride, x_dtype, group, dtype) -> tuple:
     if not _row_major_strides(rows, cols, stride):
         raise ValueError(f"x must be row-major: expected stride(1) == 1; got shape={tuple(shape)} and stride={stride}")
     mode, pitch = _GROUPS[group], _up(cols, 16)
-    head = (rows, cols, stride[0] if rows > 1 else cols, _F_ID[x_dtype], _F8_ID[dtype], mode, 0)
     n_rows = _blocks(rows) if mode == 4 else rows
+    sizes = _quant_sizes(rows, cols, stride[0] if rows > 1 else cols, _F_ID[x_dtype], _F8_ID[dtype], mode, 0)
     # the product reads the scales of 128 rows at a time: rows are the contiguous dimension
     row = ((n_rows, _blocks(cols)), (1, n_rows)) if mode != 2 else None
     col = (_blocks(rows), cols) if mode in (2, 3) else None
-    return rows, cols, pitch, head, row, col
+    return rows, cols, pitch, sizes, row, col
 
 
 def _launch_quantize(x, dtype, plan, index) -> tuple:
     """On the current device and stream."""
-    rows, cols, pitch, head, row, col = plan
+    rows, cols, pitch, sizes, row, col = plan
     device = x.device
     got = []
-    row_args = col_args = (0, 0, 0, 0, 0)
+    q_row = s_row = q_col = s_col = 0
     if row is not None:
         q = torch.empty(rows, pitch, dtype=dtype, device=device)
         s = torch.empty_strided(*row, dtype=torch.float32, device=device)
-        row_args = (q.data_ptr(), pitch, s.data_ptr(), 1, row[0][0])
+        q_row, s_row = q.data_ptr(), s.data_ptr()
         got += [q if pitch == cols else q[:, :cols], s]
     if col is not None:
         q = torch.empty(rows, pitch, dtype=dtype, device=device)
         s = torch.empty(*col, dtype=torch.float32, device=device)
-        col_args = (q.data_ptr(), pitch, s.data_ptr(), cols, 1)
+        q_col, s_col = q.data_ptr(), s.data_ptr()
         got += [q if pitch == cols else q[:, :cols], s]
-    rc = _lib.fast("b200_gemm_quantize_a8")(_QUANT_ARGS.pack(x.data_ptr(), *head, *row_args, *col_args, 0, 0), raw_stream(index))
+    rc = _lib.fast("b200_gemm_quantize_a8")(_POINTERS.pack(x.data_ptr(), q_row, s_row, q_col, s_col, 0) + sizes, raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
     return tuple(got)
@@ -343,18 +348,9 @@ class _Pieces:
         return self.add(rows * _up(cols, 16)), self.add(4 * n)
 
 
-def _quant_sizes(rows, cols, ld, in_id, out_id, mode) -> tuple:
-    """The constant members of a b200_gemm_quantize_args: the head, then pitch and scale strides of the rows' and the columns'
-    outputs (which mode needs them is the kernel's business)."""
-    pitch = _up(cols, 16)
-    return (rows, cols, ld, in_id, out_id, mode, 0), pitch, (1, _blocks(rows) if mode == 4 else rows), (cols, 1)
-
-
 def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
-    """row, col: device addresses of (values, scales)."""
-    head, pitch, row_strides, col_strides = sizes
-    args = _QUANT_ARGS.pack(x_ptr, *head, row[0], pitch, row[1], *row_strides, col[0], pitch, col[1], *col_strides, *sums)
-    rc = _lib.fast("b200_gemm_quantize_a8")(args, stream)
+    """row, col: device addresses of (values, scales); sums: of the columns' sums."""
+    rc = _lib.fast("b200_gemm_quantize_a8")(_POINTERS.pack(x_ptr, *row, *col, sums) + sizes, stream)
     if rc != 0:
         raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
 
@@ -380,8 +376,8 @@ class _ForwardPlan:
         self.xc = keep.quantized(m, k, "col") if need_w else None
         self.wq = (keep if need_x else temp).quantized(n, k, "block")
         self.temp_size, self.keep_size = temp.size, keep.size
-        self.quant_x = _quant_sizes(m, k, x_ld, _F_ID[x_dtype], e4, 3 if need_w else 1)
-        self.quant_w = _quant_sizes(n, k, w_ld, _F_ID[w_dtype], e4, 4)
+        self.quant_x = _quant_sizes(m, k, x_ld, _F_ID[x_dtype], e4, 3 if need_w else 1, 0)
+        self.quant_w = _quant_sizes(n, k, w_ld, _F_ID[w_dtype], e4, 4, 0)
         kp = _up(k, 16)
         self.gemm = _gemm_sizes(m, n, k, kp, kp, (1, m, 1, _blocks(n)), False, True, e4, e4, 1, _F_ID[x_dtype],
                                 0 if bias_dtype is None else _F_ID[bias_dtype], num_sms) if m and n and k else None
@@ -397,7 +393,8 @@ class _BackwardPlan:
         self.pitch = _up(n, 4)
         self.sums = temp.add(4 * _blocks(m) * self.pitch) if need_b else None
         self.temp_size = temp.size
-        self.quant = _quant_sizes(m, n, g_ld, _F_ID[g_dtype], g_id, 3 if need_x and by_col else 2 if by_col else 1) if m and n else None
+        self.quant = (_quant_sizes(m, n, g_ld, _F_ID[g_dtype], g_id, 3 if need_x and by_col else 2 if by_col else 1, self.pitch)
+                      if m and n else None)
         np_, kp, full = _up(n, 16), _up(k, 16), m and n and k
         self.dx = _gemm_sizes(m, k, n, np_, kp, (1, m, _blocks(n), 1), False, False, g_id, e4, 1, _F_ID[x_dtype], 0, num_sms) if full else None
         self.dw = _gemm_sizes(n, k, m, np_, kp, (1, n, 1, k), True, False, g_id, e4, 0, _F_ID[w_dtype], 0, num_sms) if full else None
@@ -430,8 +427,8 @@ class _Linear8(torch.autograd.Function):
                 temp = torch.empty(plan.temp_size, dtype=torch.uint8, device=device)
                 temp_ptr, keep_ptr = temp.data_ptr(), keep.data_ptr()
                 xr, wq = _at(temp_ptr, plan.xr), _at(keep_ptr if need_x else temp_ptr, plan.wq)
-                _call_quantize(x2.data_ptr(), plan.quant_x, xr, _at(keep_ptr, plan.xc), (0, 0), stream)
-                _call_quantize(w2.data_ptr(), plan.quant_w, wq, (0, 0), (0, 0), stream)
+                _call_quantize(x2.data_ptr(), plan.quant_x, xr, _at(keep_ptr, plan.xc), 0, stream)
+                _call_quantize(w2.data_ptr(), plan.quant_w, wq, (0, 0), 0, stream)
                 _call_gemm((xr[0], wq[0], xr[1], wq[1], y.data_ptr(), 0 if bias is None else bias.data_ptr()), plan.gemm,
                            _workspace_for(device, stream).status_bytes, stream)
             elif k == 0:
@@ -458,7 +455,7 @@ class _Linear8(torch.autograd.Function):
             base, keep_ptr = temp.data_ptr(), keep.data_ptr()
             gr, gc = _at(base, plan.gr), _at(base, plan.gc)
             if plan.quant is not None and (need_x or need_w or need_b):
-                _call_quantize(g.data_ptr(), plan.quant, gr, gc, (base + plan.sums, plan.pitch) if need_b else (0, 0), stream)
+                _call_quantize(g.data_ptr(), plan.quant, gr, gc, base + plan.sums if need_b else 0, stream)
             if need_x:
                 dx = torch.empty(shape, dtype=x_dtype, device=device)
                 if plan.dx is not None:

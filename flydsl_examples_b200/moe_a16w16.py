@@ -21,8 +21,8 @@ MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 512, 16
 _IDS = {torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _KWARGS = ("wait_limit_us", "pdl")
 
-_ARGS = struct.Struct("@5P12q6iPQP")  # b200_gemm_moe_args
-_POINTERS, _SIZES, _SCRATCH = struct.Struct("@5P"), struct.Struct("@12q6i"), struct.Struct("@PQ")  # the same in parts
+# b200_gemm_moe_args in parts; the last member is the status address
+_POINTERS, _SIZES, _SCRATCH = struct.Struct("@5P"), struct.Struct("@12q6i"), struct.Struct("@PQ")
 
 
 def _check_matrix(name: str, have, strides, shape: tuple) -> None:

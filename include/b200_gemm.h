@@ -284,21 +284,19 @@ int b200_gemm_a8w8_plan_query(const b200_gemm_a8w8_args* args, b200_gemm_plan* p
  * rounding. NaN stays NaN; an infinity becomes NaN in e4m3 and stays infinite in e5m2; neither changes its group's scale. */
 typedef struct b200_gemm_quantize_args {
   const void* x;
+  void* q_row;
+  float* s_row; /* scale of (row r, or r / 128 in mode 4; group c / 128): s_row[r * sr_row + g * sr_group]                */
+  void* q_col;
+  float* s_col;  /* scale of (group r / 128, column c): s_col[g * sc_group + c * sc_col]                               */
+  float* colsum; /* optional, modes 2 and 3: fp32 sums of x over each group of 128 rows, [group][colsum_ld]            */
   int64_t rows, cols, ldx;
+  int64_t ldq_row, sr_row, sr_group;
+  int64_t ldq_col, sc_group, sc_col;
+  int64_t colsum_ld;
   int32_t in_dtype, out_dtype; /* FP32 / BF16 / FP16; E4M3 / E5M2                                                     */
   int32_t mode;                /* 1: groups of 128 columns in a row; 2: of 128 rows in a column; 3: both, two outputs from one
                                   read; 4: 128 x 128 blocks (written through q_row, s_row)                            */
   int32_t reserved;
-  void* q_row;
-  int64_t ldq_row;
-  float* s_row; /* scale of (row r, or r / 128 in mode 4; group c / 128): s_row[r * sr_row + g * sr_group]                */
-  int64_t sr_row, sr_group;
-  void* q_col;
-  int64_t ldq_col;
-  float* s_col; /* scale of (group r / 128, column c): s_col[g * sc_group + c * sc_col]                                 */
-  int64_t sc_group, sc_col;
-  float* colsum; /* optional, modes 2 and 3: fp32 sums of x over each group of 128 rows, [group][colsum_ld]            */
-  int64_t colsum_ld;
 } b200_gemm_quantize_args;
 int b200_gemm_quantize_a8(const b200_gemm_quantize_args* args, void* cuda_stream);
 

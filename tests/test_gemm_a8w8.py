@@ -80,8 +80,8 @@ def test_structures_match_the_header(tmp_path):
     for name, st in pairs:
         lines.append(f'printf("%zu\\n", sizeof({name}));')
         want.append(C.sizeof(st))
-        packed = module._ARGS if st is _lib.Args8 else module._QUANT_ARGS
-        assert packed.size == C.sizeof(st)  # the byte string that the Python calls pass
+        tail = module._SIZES.size + 8 if st is _lib.Args8 else module._QUANT_SIZES.size
+        assert module._POINTERS.size + tail == C.sizeof(st)  # the byte string that the Python calls pass
         for field, _ in st._fields_:
             lines.append(f'printf("%zu\\n", offsetof({name}, {field}));')
             want.append(getattr(st, field).offset)

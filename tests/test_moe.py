@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from flydsl_examples_b200 import _lib
-from flydsl_examples_b200.moe_a16w16 import _ARGS, _scratch_bytes, moe_a16w16
+from flydsl_examples_b200.moe_a16w16 import _POINTERS, _SCRATCH, _SIZES, _scratch_bytes, moe_a16w16
 
 
 def args(**kw):
@@ -42,7 +42,7 @@ def test_entry_points_refuse_before_any_device_work():
     for t, i, e, k in ((4, 32, 8, 2), (1, 32, 8, 2), (64, 2048, 512, 16)):  # the Python call's own sum
         assert _scratch_bytes(t, i, e, k) == lib.b200_gemm_moe_workspace_bytes(C.byref(args(
             tokens=t, inner=i, w2_row=i, w2_expert=64 * i, w13_expert=128 * i, experts=e, top_k=k)))
-    assert _ARGS.size == C.sizeof(_lib.MoeArgs)
+    assert _POINTERS.size + _SIZES.size + _SCRATCH.size + 8 == C.sizeof(_lib.MoeArgs)  # the byte string that the Python call passes
 
 
 def test_structure_matches_the_header(tmp_path):
