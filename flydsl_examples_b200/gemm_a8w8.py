@@ -32,6 +32,15 @@ def _blocks(n: int) -> int:
 
 
 # ------------------------------------------------------------------------------------------------------------ policy
+# Clusters of one CTA per SM that a B200 with its 148 SMs holds at a time, as its occupancy query answers: a cluster lies
+# within one of its groups of SMs, so large ones leave some SMs over.
+_HELD = {1: 148, 2: 74, 4: 33, 8: 15, 16: 7}
+
+
+def _clusters(size: int, num_sms: int) -> int:
+    return _HELD[size] * num_sms // 148
+
+
 @functools.lru_cache(maxsize=4096)
 def _heuristic_items(m, n, k, a_t, b_t, num_sms) -> tuple:
     pol = heuristic_a8w8(m, n, k, a_t, b_t, num_sms)
@@ -42,14 +51,15 @@ def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: boo
     """Tile, split and operand order for a call without a tiling of its own.
 
     Up to 64 rows of A the product streams the weights: B takes the 128-row side (swap_ab), the tokens fill a tile of 16 to
-    64 columns, and a cluster splits K until the CTAs fill the SMs. Above that the time of a call is taken as whole waves
+    64 columns, and a cluster splits K, down to a block of 128 per CTA, as far as all clusters run at once (8 x 1024 x 2048:
+    split 4 4.5 us, 8 4.0; 16, whose eighth cluster waits for one of the others, 7.5). Above that the time of a call is taken as whole waves
     times the measured cycles of a K block, and the cheapest of the tiles is used."""
     kb = _blocks(k)
     if m <= 64 and not a_transposed:
         tile = 16 if m <= 16 else 32 if m <= 32 else 64
         tiles = _blocks(n)
         split = 1
-        while split < 16 and tiles * split * 2 <= num_sms and kb >= split * 4:
+        while split < 16 and tiles <= _clusters(split * 2, num_sms) and kb >= split * 2:
             split *= 2
         return {"tile_n": tile, "cta_group": 1, "swap_ab": True, "split_k": split}
     best = None
@@ -60,7 +70,7 @@ def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: boo
         tiles = -(-m // (128 * cg)) * -(-n // tile)
         slots = num_sms // cg
         for split in (1, 2, 4, 8) if cg == 1 else (1,):
-            if split > 1 and (tiles * split > slots or kb < 4 * split):
+            if split > 1 and (tiles > _clusters(split, num_sms) or kb < 4 * split):
                 continue
             waves = -(-tiles * split // slots)
             cost = waves * (-(-kb // split) * cycles + 1500) + (reduction if split > 1 else 0)

@@ -159,3 +159,15 @@ def test_plan_through_python():
     a, b = zeros8(8, 4096), zeros8(4096, 4096).t()
     got = plan(a, torch.ones(8, 32), b, torch.ones(32, 32))
     assert got["swap_ab"] == 1 and got["tile_n"] == 16 and got["cluster_split"] > 1
+
+
+@pytest.mark.parametrize("sms", [148, 132, 74])
+def test_a_split_keeps_all_its_clusters_running_at_once(sms):
+    for m in (1, 8, 33, 64, 65, 128, 256, 700):
+        for n in (1, 129, 512, 1024, 2048, 4096, 5000):
+            for k in (1, 128, 1000, 1024, 2048, 4096, 14336):
+                pol = module.heuristic_a8w8(m, n, k, False, True, sms)
+                tiles = -(-n // 128) if pol["swap_ab"] else -(-m // 128) * -(-n // pol["tile_n"])
+                if pol["split_k"] > 1:
+                    assert tiles <= module._clusters(pol["split_k"], sms)
+                    assert pol["split_k"] <= -(-k // 128)  # no CTA without a block
