@@ -38,7 +38,7 @@ _HELD = {1: 148, 2: 74, 4: 33, 8: 15, 16: 7}
 
 
 def _clusters(size: int, num_sms: int) -> int:
-    return _HELD[size] * num_sms // 148
+    return max(1, _HELD[size] * num_sms // 148)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -47,36 +47,46 @@ def _heuristic_items(m, n, k, a_t, b_t, num_sms) -> tuple:
     return pol["tile_n"], pol["cta_group"], pol["split_k"], pol.get("group_m", 0), int(pol["swap_ab"])
 
 
-def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: bool, num_sms: int = 148) -> dict:
-    """Tile, split and operand order for a call without a tiling of its own.
+# Microseconds of a call by (tile_n, cta_group, swap_ab): of a wave of tiles, of a K block in it, of a cluster's reduction times
+# its size (each CTA joins 1 / split of the tile), and of the SMs that all start together, times the part of them in use. Least
+# squares over 5,800 times of 870 random problems (1 to 12288 rows and columns, 100 to 12288 deep, all layouts and scales).
+_COST = {
+    (16, 1, False): (2.3, 0.27, 3.4, 1.7),
+    (16, 1, True): (2.1, 0.26, 3.9, 0.9),
+    (32, 1, False): (2.9, 0.30, 3.3, 2.1),
+    (32, 1, True): (2.8, 0.29, 5.1, 0.6),
+    (64, 1, False): (3.2, 0.32, 6.6, 2.9),
+    (64, 1, True): (4.3, 0.33, 6.2, 0.9),
+    (128, 1, False): (3.7, 0.38, 13.8, 3.5),
+    (128, 2, False): (4.2, 0.36, 0.0, 3.0),
+    (256, 2, False): (5.5, 0.49, 0.0, 3.8),
+}
 
-    Up to 64 rows of A the product streams the weights: B takes the 128-row side (swap_ab), the tokens fill a tile of 16 to
-    64 columns, and a cluster splits K, down to a block of 128 per CTA, as far as all clusters run at once (8 x 1024 x 2048:
-    split 4 4.5 us, 8 4.0; 16, whose eighth cluster waits for one of the others, 7.5). Above that the time of a call is taken as whole waves
-    times the measured cycles of a K block, and the cheapest of the tiles is used."""
+
+def heuristic_a8w8(m: int, n: int, k: int, a_transposed: bool, b_transposed: bool, num_sms: int = 148) -> dict:
+    """Tile, split and operand order for a call without a tiling of its own: the cheapest by a model of the call's time.
+
+    A call takes whole waves of tiles; a cluster splits the K of a tile, down to a block of 128 per CTA, only as far as all
+    clusters run at once (8 x 1024 x 2048: split 4 4.5 us, 8 4.0; 16, whose eighth cluster waits for one of the others, 7.5).
+    Up to 64 rows of A the weights take the 128-row side (swap_ab) and the tokens fill a tile of 16 to 64 columns; small
+    problems of any shape want small tiles as well (396 x 161 x 206: 128 wide 6.2 us, 16 wide 3.6), large ones CTA pairs."""
     kb = _blocks(k)
-    if m <= 64 and not a_transposed:
-        tile = 16 if m <= 16 else 32 if m <= 32 else 64
-        tiles = _blocks(n)
-        split = 1
-        while split < 16 and tiles <= _clusters(split * 2, num_sms) and kb >= split * 2:
-            split *= 2
-        return {"tile_n": tile, "cta_group": 1, "swap_ab": True, "split_k": split}
-    best = None
-    # cycles of a K block and of a cluster's reduction, measured at 256 ... 8192 rows
-    for tile, cg, cycles, reduction in ((256, 2, 830, 0), (128, 2, 640, 0), (128, 1, 560, 8500), (64, 1, 400, 3000)):
-        if not b_transposed and tile // cg != 128:
-            continue  # a row-contiguous B arrives in boxes of 128 columns per CTA
-        tiles = -(-m // (128 * cg)) * -(-n // tile)
-        slots = num_sms // cg
-        for split in (1, 2, 4, 8) if cg == 1 else (1,):
-            if split > 1 and (tiles > _clusters(split, num_sms) or kb < 4 * split):
-                continue
-            waves = -(-tiles * split // slots)
-            cost = waves * (-(-kb // split) * cycles + 1500) + (reduction if split > 1 else 0)
-            if best is None or cost < best[0]:
-                best = (cost, {"tile_n": tile, "cta_group": cg, "swap_ab": False, "split_k": split})
-    pol = best[1]
+    best = pol = None
+    for (tile, cg, swap), (wave, block, reduction, start) in _COST.items():
+        if swap and m > 1024:
+            continue  # a tile's columns are rows of the output here: stores of more rows than that cost more than they save
+        if tile // cg != 128 and (a_transposed if swap else not b_transposed):
+            continue  # an operand whose rows are contiguous along its own dimension arrives in boxes of 128 per CTA
+        rows, cols = (n, m) if swap else (m, n)
+        tiles = -(-rows // (128 * cg)) * -(-cols // tile)
+        for split in (1, 2, 4, 8, 16) if cg == 1 else (1,):
+            held = _clusters(split * cg, num_sms)
+            if split > 1 and (tiles > held or split > kb):
+                break
+            cost = (-(-tiles // held) * (wave + -(-kb // split) * block) + (reduction / split if split > 1 else 0.0)
+                    + start * min(1.0, tiles * split * cg / num_sms))
+            if best is None or cost < best:
+                best, pol = cost, {"tile_n": tile, "cta_group": cg, "swap_ab": swap, "split_k": split}
     pol["group_m"] = 8 if m > 1024 else 0  # eight tile rows share the columns of B that L2 holds
     return pol
 
