@@ -115,7 +115,7 @@ class QuantizeArgs(C.Structure):
     _fields_ = (
         [(n, C.c_void_p) for n in ("x", "q_row", "s_row", "q_col", "s_col", "colsum")]
         + [(n, C.c_int64) for n in ("rows", "cols", "ldx", "ldq_row", "sr_row", "sr_group", "ldq_col", "sc_group", "sc_col", "colsum_ld")]
-        + [(n, C.c_int32) for n in ("in_dtype", "out_dtype", "mode", "reserved")]
+        + [(n, C.c_int32) for n in ("in_dtype", "out_dtype", "mode", "packed")]
     )
 
 

@@ -24,6 +24,9 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   if (!is_fp8(a->a_dtype) || !is_fp8(a->b_dtype)) return B200_GEMM_ERR_BAD_ARG;
   if (a->out_dtype < 1 || a->out_dtype > 3) return B200_GEMM_ERR_BAD_ARG;
   if (a->lda < (a->a_trans ? a->m : a->k) || a->ldb < (a->b_trans ? a->k : a->n) || a->ldo < a->n) return B200_GEMM_ERR_BAD_ARG;
+  // exponent tiles: for both operands or for neither
+  if (a->a_block < 0 || a->a_block > 2 || a->b_block < 0 || a->b_block > 2 || (a->a_block == 2) != (a->b_block == 2)) return B200_GEMM_ERR_BAD_ARG;
+  const int packed = a->a_block == 2;
   const b200_gemm_policy& pol = a->policy;
   // this kernel has one ring depth and one K depth per tile, and no stream-K, ticket, atomic or loader-warp mode
   if (pol.stages != 0 || pol.stream_k != 0 || pol.tile_k != 0 || pol.loader != 0) return B200_GEMM_ERR_BAD_POLICY;
@@ -35,7 +38,8 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   pl.tile_k = k8TK;
   pl.group_m = pol.group_m < 0 ? 0 : pol.group_m;
   const int v_vector = (pl.swap_ab ? a->a_block : a->b_block) ? 0 : 1;
-  if (!variant8(pl.tile_n, pl.cta_group, v_vector, var)) return B200_GEMM_ERR_BAD_POLICY;
+  if (packed && (pl.swap_ab || pol.split_k > 1)) return B200_GEMM_ERR_BAD_POLICY;
+  if (!variant8(pl.tile_n, pl.cta_group, v_vector, packed, var)) return B200_GEMM_ERR_BAD_POLICY;
   pl.tile_m = k8TileP * pl.cta_group;
   pl.stages = var->stages;
   pl.smem_bytes = var->smem_bytes;
@@ -60,8 +64,7 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   int cap = (pol.max_ctas > 0 ? pol.max_ctas : sms) / pl.cta_group;
   if (cap < 1) cap = 1;
   pl.grid = s > 1 ? pl.num_units : (int)(tiles < cap ? tiles : cap) * pl.cta_group;
-  const int bufs = pl.tile_n > 128 ? 2 : 4;
-  pl.tmem_cols = pl.tile_n * bufs;
+  pl.tmem_cols = packed || pl.tile_n > 128 ? 512 : pl.tile_n * 4;
   *out = pl;
   return 0;
 }
@@ -76,6 +79,22 @@ static int encode8(CUtensorMap* map, const void* ptr, int mn_major, int64_t rows
   cuuint32_t estr[2] = {1, 1};
   const CUresult res = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return res == CUDA_SUCCESS ? 0 : B200_GEMM_ERR_TENSOR_MAP;
+}
+
+// The exponent tiles of an operand, 512 bytes each, as rows of 128 bytes.
+static int encode_tiles(CUtensorMap* map, const void* ptr, int64_t row_tiles, int64_t k_blocks, int64_t s_row, int64_t s_kb) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return B200_GEMM_ERR_DRIVER;
+  const int64_t tiles = (row_tiles - 1) * s_row + (k_blocks - 1) * s_kb + 1;
+  if (tiles > 0x1fffffff) return B200_GEMM_ERR_TOO_LARGE;
+  cuuint64_t dims[2] = {128, (cuuint64_t)(4 * tiles)};
+  cuuint64_t strides[1] = {128};
+  cuuint32_t box[2] = {128, 4};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult res = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return res == CUDA_SUCCESS ? 0 : B200_GEMM_ERR_TENSOR_MAP;
 }
@@ -100,7 +119,9 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   const int es = a->out_dtype == B200_GEMM_DTYPE_FP32 ? 4 : 2;
   auto aligned = [](const void* ptr, int64_t to) { return (reinterpret_cast<uintptr_t>(ptr) % (uintptr_t)to) == 0; };
   if (!aligned(a->a, 16) || !aligned(a->b, 16) || a->lda % 16 != 0 || a->ldb % 16 != 0) return B200_GEMM_ERR_BAD_ARG;
-  if (!aligned(a->a_scale, 4) || !aligned(a->b_scale, 4) || !aligned(a->out, es)) return B200_GEMM_ERR_BAD_ARG;
+  const int packed = a->a_block == 2;
+  if (packed && (a->sa_row < 0 || a->sa_kb < 0 || a->sb_col < 0 || a->sb_kb < 0)) return B200_GEMM_ERR_BAD_ARG;
+  if (!aligned(a->a_scale, packed ? 16 : 4) || !aligned(a->b_scale, packed ? 16 : 4) || !aligned(a->out, es)) return B200_GEMM_ERR_BAD_ARG;
   if (a->bias != nullptr && (a->bias_dtype < 1 || a->bias_dtype > 3 || !aligned(a->bias, a->bias_dtype == 1 ? 4 : 2)))
     return B200_GEMM_ERR_BAD_ARG;
   rc = current_sms(&dev, &sms);
@@ -118,6 +139,12 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   if (rc) return rc;
   rc = encode8(&p.tmap_v, sw ? a->a : a->b, p.v_mn_major, p.Q, a->k, sw ? a->lda : a->ldb, pl.tile_n / pl.cta_group);
   if (rc) return rc;
+  if (packed) {
+    const int64_t kb = (a->k + k8TK - 1) / k8TK;
+    rc = encode_tiles(&p.tmap_us, a->a_scale, (a->m + 127) / 128, kb, a->sa_row, a->sa_kb);
+    if (!rc) rc = encode_tiles(&p.tmap_vs, a->b_scale, (a->n + 127) / 128, kb, a->sb_col, a->sb_kb);
+    if (rc) return rc;
+  }
   p.u_scale = sw ? a->b_scale : a->a_scale, p.v_scale = sw ? a->a_scale : a->b_scale;
   p.us_row = sw ? a->sb_col : a->sa_row, p.us_kb = sw ? a->sb_kb : a->sa_kb;
   p.vs_row = sw ? a->sa_row : a->sb_col, p.vs_kb = sw ? a->sa_kb : a->sb_kb;
@@ -149,6 +176,8 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   // instruction descriptor: fp32 accumulator, the operands' 8-bit formats, their major-ness, N / 8, M / 16
   p.idesc = (1u << 4) | (u_fmt << 7) | (v_fmt << 10) | (uint32_t(p.u_mn_major) << 15) | (uint32_t(p.v_mn_major) << 16) |
             (uint32_t(pl.tile_n >> 3) << 17) | (uint32_t(pl.tile_m >> 4) << 24);
+  // with scales the accumulator is always fp32, its field (bits 4 and 5) names B's exponent byte (0, as for A), bit 23 the type
+  if (packed) p.idesc = (p.idesc & ~(3u << 4)) | (1u << 23);
   make_desc8(p.u_mn_major, &p.u_desc_hi, &p.u_desc_lo, &p.u_kstep);
   make_desc8(p.v_mn_major, &p.v_desc_hi, &p.v_desc_lo, &p.v_kstep);
   p.wait_limit_ns = a->policy.wait_limit_us > 0 ? (unsigned long long)a->policy.wait_limit_us * 1000ull : kWaitLimitNs;
@@ -220,7 +249,7 @@ int b200_gemm_a8w8(const b200_gemm_a8w8_args* args, void* cuda_stream) {
 int b200_gemm_quantize_a8(const b200_gemm_quantize_args* a, void* cuda_stream) {
   if (a == nullptr || a->rows < 0 || a->cols < 0) return B200_GEMM_ERR_BAD_ARG;
   if (a->in_dtype < 1 || a->in_dtype > 3 || !b200::is_fp8(a->out_dtype)) return B200_GEMM_ERR_BAD_ARG;
-  if (a->mode < 1 || a->mode > 4) return B200_GEMM_ERR_BAD_ARG;
+  if (a->mode < 1 || a->mode > 4 || a->packed < 0 || a->packed > 1) return B200_GEMM_ERR_BAD_ARG;
   if (a->rows == 0 || a->cols == 0) return 0;
   if (a->rows > 0x7fffff00LL || a->cols > 0x7fffff00LL) return B200_GEMM_ERR_TOO_LARGE;
   const bool row = a->mode != 2, col = a->mode == 2 || a->mode == 3;
@@ -237,6 +266,7 @@ int b200_gemm_quantize_a8(const b200_gemm_quantize_args* a, void* cuda_stream) {
   p.q_row = static_cast<uint8_t*>(a->q_row), p.ldq_row = a->ldq_row, p.s_row = a->s_row, p.sr_row = a->sr_row, p.sr_group = a->sr_group;
   p.q_col = static_cast<uint8_t*>(a->q_col), p.ldq_col = a->ldq_col, p.s_col = a->s_col, p.sc_group = a->sc_group, p.sc_col = a->sc_col;
   p.colsum = a->colsum, p.colsum_ld = a->colsum_ld;
+  p.packed = a->packed;
   const bool e5m2 = a->out_dtype == B200_GEMM_DTYPE_E5M2;
   void* fn = a->in_dtype == B200_GEMM_DTYPE_FP32   ? b200::quant_fn<float>(a->mode, e5m2)
              : a->in_dtype == B200_GEMM_DTYPE_BF16 ? b200::quant_fn<__nv_bfloat16>(a->mode, e5m2)

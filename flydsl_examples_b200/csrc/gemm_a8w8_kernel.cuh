@@ -37,6 +37,7 @@ constexpr int k8UBytes = k8TileP * k8TK;
 struct alignas(64) Gemm8Params {
   CUtensorMap tmap_u;
   CUtensorMap tmap_v;
+  CUtensorMap tmap_us, tmap_vs;  // PACKED: the exponent tiles as rows of 128 bytes, box 4 rows
   CUtensorMap tmap_out;  // box = 32 rows x 128 bytes (valid when tma_store != 0)
   const float* u_scale;
   const float* v_scale;
@@ -61,7 +62,8 @@ struct alignas(64) Gemm8Params {
 };
 
 // VVEC: V has a scale per row; otherwise one per 128 rows, so one value serves each half of a tile's columns.
-template <int TILE_Q, int STAGES, int CG, bool VVEC>
+// PACKED: scales are powers of two, in exponent tiles, and the tensor core applies them.
+template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED>
 struct Smem8 {
   static constexpr int kVRows = TILE_Q / CG;
   static constexpr int kVBytes = kVRows * k8TK;
@@ -71,12 +73,14 @@ struct Smem8 {
   // send (2 % on 256 columns; the fifth ring stage that they displace gained nothing), else one
   static constexpr int kImages = TILE_Q >= 256 ? 2 : 1;
   static constexpr int kStagingBytes = TILE_Q >= 64 ? 8 * kImages * 4096 : 0;
-  static constexpr int kRecvBytes = CG == 1 ? k8TileP * TILE_Q * 4 : 0;   // cluster split: [source][own column][128] fp32
+  static constexpr int kRecvBytes = CG == 1 && !PACKED ? k8TileP * TILE_Q * 4 : 0;   // cluster split: [source][own column][128] fp32
   static constexpr int kOutBytes = kRecvBytes > kStagingBytes ? kRecvBytes : kStagingBytes;
   static constexpr int kScaleOff = kOutOff + kOutBytes;
   static constexpr int kScaleVals = k8TileP + (VVEC ? TILE_Q : 4);
-  static constexpr int kScaleBytes = k8ScaleStages * kScaleVals * 4;
-  static constexpr int kBufs = TILE_Q > 128 ? 2 : 4;  // accumulators in TMEM
+  static constexpr int kTileBytes = 512 * (1 + TILE_Q / 128);  // PACKED: exponents of a stage, U's then V's
+  static constexpr int kScaleBytes = PACKED ? STAGES * kTileBytes : k8ScaleStages * kScaleVals * 4;
+  // accumulators in TMEM; PACKED needs the other columns for the exponents of its stages
+  static constexpr int kBufs = PACKED ? 256 / TILE_Q : TILE_Q > 128 ? 2 : 4;
   static constexpr int kBarOff = kScaleOff + kScaleBytes;
   static constexpr int kNumBars = 2 * STAGES + 2 * k8ScaleStages + kBufs;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
@@ -184,14 +188,16 @@ __device__ __forceinline__ bool wait_two(uint32_t bar0, uint32_t parity0, uint32
   return __all_sync(0xffffffffu, good);
 }
 
-template <int TILE_Q, int STAGES, int CG, bool VVEC>
+template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED>
 __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __grid_constant__ Gemm8Params p) {
-  using L = Smem8<TILE_Q, STAGES, CG, VVEC>;
+  using L = Smem8<TILE_Q, STAGES, CG, VVEC, PACKED>;
   constexpr int HC = TILE_Q / 2;               // columns per epilogue warp (the two warps of a lane quarter split the tile)
   constexpr int CW = HC < 32 ? HC : 32;        // columns per tcgen05.ld
   constexpr int NCH = HC / CW;
   constexpr int kBufs = L::kBufs;
-  constexpr uint32_t kTmemCols = TILE_Q * kBufs < 32 ? 32 : TILE_Q * kBufs;
+  constexpr uint32_t kTmemCols = PACKED ? 512 : TILE_Q * kBufs < 32 ? 32 : TILE_Q * kBufs;
+  constexpr uint32_t kExpCols = 4 * (1 + TILE_Q / 128);  // TMEM columns of a stage's exponents, behind the accumulators
+  static_assert(!PACKED || (TILE_Q % 128 == 0 && 256 + STAGES * kExpCols <= 512), "exponents in TMEM");
   // 128 running sums, 32 loaded values and addresses do not fit the 168 registers a thread of 384 gets at launch: the
   // wide tile moves registers to the epilogue, 128 * 40 + 256 * 232 = 384 * 168.
   constexpr bool kMoveRegs = HC > 64;
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
   // scale each: 58.8 -> 54.2 us at 4096 x 4096 x 2048) and costs elsewhere (one scale per half: 454 -> 479 us at 8192^3; 128
   // columns: 61 -> 64 us).
   constexpr bool kLookAhead = VVEC && HC > 64;
-  constexpr uint32_t kTxBytes = CG * L::kStageBytes;  // both CTAs of a pair count on the leader's barrier
+  constexpr uint32_t kTxBytes = CG * (L::kStageBytes + (PACKED ? L::kTileBytes : 0));  // both CTAs of a pair count on the leader's barrier
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
       mbar_init(done_bar(s), 1);
     }
     for (int s = 0; s < k8ScaleStages; ++s) {
-      mbar_init(sfull_bar(s), 64);
+      mbar_init(sfull_bar(s), PACKED ? 1 : 64);  // PACKED: the first of them are the accumulators' "complete"
       mbar_init(sempty_bar(s), 8);
     }
     for (int b = 0; b < kBufs; ++b) mbar_init(acce_bar(b), 8 * CG);
@@ -246,6 +252,10 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
     prefetch_tmap(&p.tmap_u);
     prefetch_tmap(&p.tmap_v);
     if (p.tma_store) prefetch_tmap(&p.tmap_out);
+    if (PACKED) {
+      prefetch_tmap(&p.tmap_us);
+      prefetch_tmap(&p.tmap_vs);
+    }
   }
   if (warp == 1) {
     tmem_alloc<CG>(smem_u32(const_cast<uint32_t*>(tmem_ptr_s)), kTmemCols);
@@ -312,6 +322,13 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
               load(sv, &p.tmap_v, k0, q0, fb);
             else
               load(sv, &p.tmap_v, q0, k0, fb);
+            if constexpr (PACKED) {
+              const uint32_t se = base + L::kScaleOff + stage * L::kTileBytes;
+              load(se, &p.tmap_us, 0, 4 * (int)(kb * p.us_kb + (tp * CG + prank) * p.us_row), fb);
+#pragma unroll
+              for (int j = 0; j < TILE_Q / 128; ++j)  // both CTAs of a pair need V's
+                load(se + 512u * (1 + j), &p.tmap_vs, 0, 4 * (int)(kb * p.vs_kb + (tq * (TILE_Q / 128) + j) * p.vs_row), fb);
+            }
           }
           __syncwarp();
           ++issued;
@@ -329,12 +346,12 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
       if (prank == 0) {
         int stage = 0;
         uint32_t phase = 0;
-        int g = 0;  // K blocks so far; each has an accumulator of its own
+        int g = 0;  // K blocks so far; each has an accumulator of its own (PACKED: tiles)
         bool ok = true;
 #pragma unroll 1
-        for (int tile = tile0; ok && tile < p.num_tiles; tile += tile_step) {
+        for (int tile = tile0; ok && tile < p.num_tiles; tile += tile_step, g += PACKED) {
 #pragma unroll 1
-          for (int kb = kb0; kb < p.kb_total; kb += kbstep, ++g) {
+          for (int kb = kb0; kb < p.kb_total; kb += kbstep, g += !PACKED) {
             const int buf = g % kBufs;
             if (!wait_two(acce_bar(buf), ((g / kBufs) & 1) ^ 1u, full_bar(stage), phase, abort_s, wait_limit)) {
               if (lane == 0) report_abort8(p.status, 1, tile);
@@ -347,8 +364,19 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
               const uint64_t du = (uint64_t(p.u_desc_hi) << 32) | uint64_t(p.u_desc_lo | ((su >> 4) & 0x3fffu));
               const uint64_t dv = (uint64_t(p.v_desc_hi) << 32) | uint64_t(p.v_desc_lo | ((sv >> 4) & 0x3fffu));
               const uint32_t d_tmem = tmem_base + buf * TILE_Q;
+              if constexpr (PACKED) {
+                const uint32_t se = base + L::kScaleOff + stage * L::kTileBytes, exps = tmem_base + 256 + stage * kExpCols;
+                // rows of 16 bytes without swizzle, eight of them 128 bytes apart from the next eight
+                const uint64_t de = (uint64_t((128u >> 4) | (1u << 14)) << 32) | uint64_t((1u << 16) | ((se >> 4) & 0x3fffu));
 #pragma unroll
-              for (int j = 0; j < k8TK / 32; ++j)
+                for (int j = 0; j <= TILE_Q / 128; ++j) tmem_copy_scales<CG>(exps + 4 * j, de + uint64_t(j * (512 >> 4)));
+#pragma unroll
+                for (int j = 0; j < k8TK / 32; ++j)
+                  umma_mxf8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), p.idesc, exps, exps + 4,
+                                kb != kb0 || j != 0 ? 1u : 0u);
+              }
+#pragma unroll
+              for (int j = 0; j < (PACKED ? 0 : k8TK / 32); ++j)
                 umma_f8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), p.idesc, j != 0 ? 1u : 0u);
               if constexpr (CG == 2) {
                 umma_commit_pair(mapa_cluster(done_bar(stage), 0));
@@ -356,13 +384,21 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
               } else {
                 umma_commit(done_bar(stage));
               }
+              if (PACKED && kb + kbstep >= p.kb_total) {
+                if constexpr (CG == 2) {
+                  umma_commit_pair(mapa_cluster(sfull_bar(buf), 0));
+                  umma_commit_pair(mapa_cluster(sfull_bar(buf), 1));
+                } else {
+                  umma_commit(sfull_bar(buf));
+                }
+              }
             }
             __syncwarp();
             if (++stage == STAGES) stage = 0, phase ^= 1u;
           }
         }
       }
-    } else {
+    } else if constexpr (!PACKED) {
       // ------------------------------------------------------------------ scale loaders (warps 2 and 3)
       const int lt = threadIdx.x - 64;
       int g = 0;
@@ -434,8 +470,34 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
       for (int i = 0; i < HC / 2; ++i) acc2[i] = 0;
       auto acc = [&](int i) { return __uint_as_float((uint32_t)(i & 1 ? acc2[i >> 1] >> 32 : acc2[i >> 1])); };
       bool ok = true, seen = false;
+      if constexpr (PACKED) {  // all K blocks are in one accumulator
+        const int buf = g % kBufs;
+        const uint32_t done = (g / kBufs) & 1;
+        ++g;
+        ok = wait_two(sfull_bar(buf), done, sfull_bar(buf), done, abort_s, wait_limit);
+        if (ok) {
+          tc_fence_after();
+          const uint32_t t_acc = tmem_base + buf * TILE_Q + half * HC + (uint32_t(quarter * 32) << 16);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            uint32_t r[32];
+            tmem_ld_32x32(t_acc + c * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) acc2[(c * 32 + i) / 2] = pack_u32x2(r[i], r[i + 1]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2 && prank != 0)
+              mbar_arrive_remote(acce_bar(buf), 0);
+            else
+              mbar_arrive(acce_bar(buf));
+          }
+        }
+      }
 #pragma unroll 1
-      for (int kb = kb0; kb < p.kb_total; kb += kbstep, ++g) {
+      for (int kb = kb0; !PACKED && kb < p.kb_total; kb += kbstep, ++g) {
         const int buf = g % kBufs, ss = g % k8ScaleStages;
         // The verdict is the warp's: tcgen05.ld needs all its lanes.
         if (!(kLookAhead && __all_sync(0xffffffffu, seen)) &&

@@ -36,6 +36,7 @@ struct QuantParams {
   long long ldq_col;
   float* s_col;
   long long sc_group, sc_col;
+  int packed;     // scales as exponent bytes in tiles for the tensor core, see store_packed
   float* colsum;  // optional: sums of the tile's columns, [tile row][cols_pitch]
   long long colsum_ld;
 };
@@ -156,6 +157,12 @@ static __device__ __noinline__ void store_row8_slow(uint8_t* dst, uint32_t lo, u
   for (int j = 0; j < min(n, 8); ++j) dst[j] = (uint8_t)(v >> (8 * j));
 }
 
+// Packed scales: 512 bytes for each 128 rows of an operand and K block; row r of them is the 32-bit word r % 32 * 4 + r / 32, its
+// scale's exponent in all four bytes (one for each 32 of the block's 128 elements, as the tensor core takes them).
+__device__ __forceinline__ void store_packed(float* tiles, long long tile, int r, uint32_t bits) {
+  reinterpret_cast<uint32_t*>(tiles)[tile * 128 + (r & 31) * 4 + (r >> 5)] = (bits >> 23) * 0x01010101u;
+}
+
 // MODE: 1 = groups along rows, 2 = along columns, 4 = 128 x 128 blocks (written through the row members).
 template <typename T, int MODE, bool E5M2>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantize_a8_kernel(const QuantParams p) {
@@ -266,7 +273,12 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     }
     const uint32_t sb = scale_bits(fmaxf(rmax[0], __shfl_xor_sync(0xffffffffu, rmax[0], 1)), n);
     const int own = ty + 16 * (tx >> 1);
-    if ((tx & 1) == 0 && own < nrow) p.s_row[(long long)(r0 + own) * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+    if ((tx & 1) == 0 && own < nrow) {
+      if (p.packed)
+        store_packed(p.s_row, (long long)tc * p.sr_group + tr, own, sb);
+      else
+        p.s_row[(long long)(r0 + own) * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+    }
     const float own_inv = inverse_of_scale(sb);
     uint8_t* dst = p.q_row + (long long)(r0 + ty) * p.ldq_row + col;
 #pragma unroll
@@ -307,7 +319,10 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
       const uint32_t sb = scale_bits(m, n);
       const int c = tc * 128 + threadIdx.x;
       if (c < p.cols) {
-        p.s_col[(long long)tr * p.sc_group + (long long)c * p.sc_col] = __uint_as_float(sb);
+        if (p.packed)
+          store_packed(p.s_col, (long long)tr * p.sc_group + tc, threadIdx.x, sb);
+        else
+          p.s_col[(long long)tr * p.sc_group + (long long)c * p.sc_col] = __uint_as_float(sb);
         if (p.colsum != nullptr) {
 #pragma unroll
           for (int w = 0; w < 8; ++w) t += red2[w][threadIdx.x];
@@ -340,7 +355,11 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w]);
     const uint32_t sb = scale_bits(m, n);
-    if (threadIdx.x == 0) p.s_row[(long long)tr * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+    if (p.packed) {
+      if (threadIdx.x < 128) store_packed(p.s_row, (long long)tc * p.sr_group + tr, threadIdx.x, sb);
+    } else if (threadIdx.x == 0) {
+      p.s_row[(long long)tr * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
+    }
     const float s = inverse_of_scale(sb);
     const float inv[8] = {s, s, s, s, s, s, s, s};
     if (ncol > 0) {

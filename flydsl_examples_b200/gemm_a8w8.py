@@ -277,9 +277,10 @@ _QUANT_SIZES = struct.Struct("@10q4i")  # b200_gemm_quantize_args behind its six
 _GROUPS = {"row": 1, "col": 2, "both": 3, "block": 4}
 
 
-def _quant_sizes(rows, cols, ld, in_id, out_id, mode, sums_pitch) -> bytes:
+def _quant_sizes(rows, cols, ld, in_id, out_id, mode, sums_pitch, packed=False) -> bytes:
     pitch = _up(cols, 16)
-    return _QUANT_SIZES.pack(rows, cols, ld, pitch, 1, _blocks(rows) if mode == 4 else rows, pitch, cols, 1, sums_pitch, in_id, out_id, mode, 0)
+    row_groups, col_groups = (_blocks(rows), _blocks(cols)) if packed else (_blocks(rows) if mode == 4 else rows, cols)
+    return _QUANT_SIZES.pack(rows, cols, ld, pitch, 1, row_groups, pitch, col_groups, 1, sums_pitch, in_id, out_id, mode, int(packed))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -362,10 +363,9 @@ class _Pieces:
         self.size += _up(nbytes, 256)
         return at
 
-    def quantized(self, rows: int, cols: int, groups: str) -> tuple:
-        """(values, scales) of a matrix; the values' pitch is a multiple of 16."""
-        n = {"row": rows * _blocks(cols), "col": _blocks(rows) * cols, "block": _blocks(rows) * _blocks(cols)}[groups]
-        return self.add(rows * _up(cols, 16)), self.add(4 * n)
+    def quantized(self, rows: int, cols: int) -> tuple:
+        """(values, exponent tiles) of a matrix; the values' pitch is a multiple of 16."""
+        return self.add(rows * _up(cols, 16)), self.add(512 * _blocks(rows) * _blocks(cols))
 
 
 def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
@@ -375,9 +375,16 @@ def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
         raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
 
 
-def _gemm_sizes(m, n, k, lda, ldb, scale_strides, a_t, b_t, a_id, b_id, b_block, out_id, bias_id, num_sms) -> bytes:
-    return _SIZES.pack(m, n, k, lda, ldb, n, *scale_strides, a_t, b_t, a_id, b_id, 0, b_block, out_id, bias_id,
-                       *_policy(m, n, k, a_t, b_t, {}, num_sms))
+def _packed_policy(m, n, k, num_sms) -> tuple:
+    """Tiling of a product whose scales are exponent tiles, as the fields of b200_gemm_policy: CTA pairs with 256 x 256 tiles or
+    CTAs with 128 x 128, by whole waves times the measured times of a tile and of a K block in it."""
+    pairs = -(-(-(-m // 256) * -(-n // 256)) // max(1, num_sms // 2)) * (5.0 + _blocks(k) * 0.45)
+    single = -(-(-(-m // 128) * -(-n // 128)) // num_sms) * (3.5 + _blocks(k) * 0.30)
+    return (256 if pairs < single else 128, 0, 1, 8 if m > 1024 else 0, 0, 2 if pairs < single else 1) + (0,) * 10
+
+
+def _gemm_sizes(m, n, k, lda, ldb, scale_strides, a_t, b_t, a_id, b_id, out_id, bias_id, num_sms) -> bytes:
+    return _SIZES.pack(m, n, k, lda, ldb, n, *scale_strides, a_t, b_t, a_id, b_id, 2, 2, out_id, bias_id, *_packed_policy(m, n, k, num_sms))
 
 
 def _call_gemm(pointers, sizes, status, stream) -> None:
@@ -391,15 +398,15 @@ class _ForwardPlan:
     def __init__(self, m, n, k, x_ld, x_dtype, w_ld, w_dtype, bias_dtype, need_x, need_w, num_sms):
         e4 = _lib.DTYPE_E4M3
         temp, keep = _Pieces(), _Pieces()
-        self.xr = temp.quantized(m, k, "row")
+        self.xr = temp.quantized(m, k)
         # what the backward pass reads: x by columns and the weight, as far as they are needed
-        self.xc = keep.quantized(m, k, "col") if need_w else None
-        self.wq = (keep if need_x else temp).quantized(n, k, "block")
+        self.xc = keep.quantized(m, k) if need_w else None
+        self.wq = (keep if need_x else temp).quantized(n, k)
         self.temp_size, self.keep_size = temp.size, keep.size
-        self.quant_x = _quant_sizes(m, k, x_ld, _F_ID[x_dtype], e4, 3 if need_w else 1, 0)
-        self.quant_w = _quant_sizes(n, k, w_ld, _F_ID[w_dtype], e4, 4, 0)
+        self.quant_x = _quant_sizes(m, k, x_ld, _F_ID[x_dtype], e4, 3 if need_w else 1, 0, True)
+        self.quant_w = _quant_sizes(n, k, w_ld, _F_ID[w_dtype], e4, 4, 0, True)
         kp = _up(k, 16)
-        self.gemm = _gemm_sizes(m, n, k, kp, kp, (1, m, 1, _blocks(n)), False, True, e4, e4, 1, _F_ID[x_dtype],
+        self.gemm = _gemm_sizes(m, n, k, kp, kp, (1, _blocks(m), 1, _blocks(n)), False, True, e4, e4, _F_ID[x_dtype],
                                 0 if bias_dtype is None else _F_ID[bias_dtype], num_sms) if m and n and k else None
 
 
@@ -408,16 +415,16 @@ class _BackwardPlan:
         e4 = _lib.DTYPE_E4M3
         temp = _Pieces()
         by_col = need_w or need_b
-        self.gr = temp.quantized(m, n, "row") if need_x else None
-        self.gc = temp.quantized(m, n, "col") if by_col else None
+        self.gr = temp.quantized(m, n) if need_x else None
+        self.gc = temp.quantized(m, n) if by_col else None
         self.pitch = _up(n, 4)
         self.sums = temp.add(4 * _blocks(m) * self.pitch) if need_b else None
         self.temp_size = temp.size
-        self.quant = (_quant_sizes(m, n, g_ld, _F_ID[g_dtype], g_id, 3 if need_x and by_col else 2 if by_col else 1, self.pitch)
+        self.quant = (_quant_sizes(m, n, g_ld, _F_ID[g_dtype], g_id, 3 if need_x and by_col else 2 if by_col else 1, self.pitch, True)
                       if m and n else None)
         np_, kp, full = _up(n, 16), _up(k, 16), m and n and k
-        self.dx = _gemm_sizes(m, k, n, np_, kp, (1, m, _blocks(n), 1), False, False, g_id, e4, 1, _F_ID[x_dtype], 0, num_sms) if full else None
-        self.dw = _gemm_sizes(n, k, m, np_, kp, (1, n, 1, k), True, False, g_id, e4, 0, _F_ID[w_dtype], 0, num_sms) if full else None
+        self.dx = _gemm_sizes(m, k, n, np_, kp, (1, _blocks(m), _blocks(n), 1), False, False, g_id, e4, _F_ID[x_dtype], 0, num_sms) if full else None
+        self.dw = _gemm_sizes(n, k, m, np_, kp, (1, _blocks(n), 1, _blocks(k)), True, False, g_id, e4, _F_ID[w_dtype], 0, num_sms) if full else None
 
 
 _forward_plan = functools.lru_cache(maxsize=1024)(_ForwardPlan)
