@@ -84,10 +84,10 @@ static int encode8(CUtensorMap* map, const void* ptr, int mn_major, int64_t rows
 }
 
 // The exponent tiles of an operand, 512 bytes each, as rows of 128 bytes.
-static int encode_tiles(CUtensorMap* map, const void* ptr, int64_t row_tiles, int64_t k_blocks, int64_t s_row, int64_t s_kb) {
+static int encode_tiles(CUtensorMap* map, const void* ptr, int64_t row_tiles, int64_t k_groups, int64_t s_row, int64_t s_kb) {
   EncodeTiledFn enc = get_encode_fn();
   if (enc == nullptr) return B200_GEMM_ERR_DRIVER;
-  const int64_t tiles = (row_tiles - 1) * s_row + (k_blocks - 1) * s_kb + 1;
+  const int64_t tiles = (row_tiles - 1) * s_row + (k_groups - 1) * s_kb + 1;
   if (tiles > 0x1fffffff) return B200_GEMM_ERR_TOO_LARGE;
   cuuint64_t dims[2] = {128, (cuuint64_t)(4 * tiles)};
   cuuint64_t strides[1] = {128};
@@ -140,7 +140,7 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   rc = encode8(&p.tmap_v, sw ? a->a : a->b, p.v_mn_major, p.Q, a->k, sw ? a->lda : a->ldb, pl.tile_n / pl.cta_group);
   if (rc) return rc;
   if (packed) {
-    const int64_t kb = (a->k + k8TK - 1) / k8TK;
+    const int64_t kb = (a->k + 4 * k8TK - 1) / (4 * k8TK);
     rc = encode_tiles(&p.tmap_us, a->a_scale, (a->m + 127) / 128, kb, a->sa_row, a->sa_kb);
     if (!rc) rc = encode_tiles(&p.tmap_vs, a->b_scale, (a->n + 127) / 128, kb, a->sb_col, a->sb_kb);
     if (rc) return rc;
@@ -176,7 +176,7 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   // instruction descriptor: fp32 accumulator, the operands' 8-bit formats, their major-ness, N / 8, M / 16
   p.idesc = (1u << 4) | (u_fmt << 7) | (v_fmt << 10) | (uint32_t(p.u_mn_major) << 15) | (uint32_t(p.v_mn_major) << 16) |
             (uint32_t(pl.tile_n >> 3) << 17) | (uint32_t(pl.tile_m >> 4) << 24);
-  // with scales the accumulator is always fp32, its field (bits 4 and 5) names B's exponent byte (0, as for A), bit 23 the type
+  // with scales the accumulator is always fp32; bits 4-5 and 29-30 name B's and A's exponent byte, bit 23 the scales' type
   if (packed) p.idesc = (p.idesc & ~(3u << 4)) | (1u << 23);
   make_desc8(p.u_mn_major, &p.u_desc_hi, &p.u_desc_lo, &p.u_kstep);
   make_desc8(p.v_mn_major, &p.v_desc_hi, &p.v_desc_lo, &p.v_kstep);

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
   // scale each: 58.8 -> 54.2 us at 4096 x 4096 x 2048) and costs elsewhere (one scale per half: 454 -> 479 us at 8192^3; 128
   // columns: 61 -> 64 us).
   constexpr bool kLookAhead = VVEC && HC > 64;
-  constexpr uint32_t kTxBytes = CG * (L::kStageBytes + (PACKED ? L::kTileBytes : 0));  // both CTAs of a pair count on the leader's barrier
+  constexpr uint32_t kTxBytes = CG * L::kStageBytes;  // both CTAs of a pair count on the leader's barrier
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -313,7 +313,8 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
           if (elect_one()) {
             const uint32_t su = base + stage * L::kStageBytes, sv = su + k8UBytes;
             const int k0 = kb * k8TK;
-            if (prank == 0) mbar_arrive_expect_tx(full_bar(stage), kTxBytes);
+            const bool exps = PACKED && (kb & 3) == 0;  // with the first of four blocks
+            if (prank == 0) mbar_arrive_expect_tx(full_bar(stage), exps ? kTxBytes + CG * L::kTileBytes : kTxBytes);
             if (!p.u_mn_major)
               load(su, &p.tmap_u, k0, p0, fb);
             else
@@ -322,12 +323,13 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
               load(sv, &p.tmap_v, k0, q0, fb);
             else
               load(sv, &p.tmap_v, q0, k0, fb);
-            if constexpr (PACKED) {
+            if (exps) {
               const uint32_t se = base + L::kScaleOff + stage * L::kTileBytes;
-              load(se, &p.tmap_us, 0, 4 * (int)(kb * p.us_kb + (tp * CG + prank) * p.us_row), fb);
+              const int q = kb >> 2;
+              load(se, &p.tmap_us, 0, 4 * (int)(q * p.us_kb + (tp * CG + prank) * p.us_row), fb);
 #pragma unroll
               for (int j = 0; j < TILE_Q / 128; ++j)  // both CTAs of a pair need V's
-                load(se + 512u * (1 + j), &p.tmap_vs, 0, 4 * (int)(kb * p.vs_kb + (tq * (TILE_Q / 128) + j) * p.vs_row), fb);
+                load(se + 512u * (1 + j), &p.tmap_vs, 0, 4 * (int)(q * p.vs_kb + (tq * (TILE_Q / 128) + j) * p.vs_row), fb);
             }
           }
           __syncwarp();
@@ -347,12 +349,14 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
         int stage = 0;
         uint32_t phase = 0;
         int g = 0;  // K blocks so far; each has an accumulator of its own (PACKED: tiles)
+        int group = -1;  // PACKED: fours of K blocks so far
         bool ok = true;
 #pragma unroll 1
         for (int tile = tile0; ok && tile < p.num_tiles; tile += tile_step, g += PACKED) {
 #pragma unroll 1
           for (int kb = kb0; kb < p.kb_total; kb += kbstep, g += !PACKED) {
             const int buf = g % kBufs;
+            if (PACKED && (kb & 3) == 0) ++group;
             if (!wait_two(acce_bar(buf), ((g / kBufs) & 1) ^ 1u, full_bar(stage), phase, abort_s, wait_limit)) {
               if (lane == 0) report_abort8(p.status, 1, tile);
               ok = false;
@@ -365,14 +369,19 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
               const uint64_t dv = (uint64_t(p.v_desc_hi) << 32) | uint64_t(p.v_desc_lo | ((sv >> 4) & 0x3fffu));
               const uint32_t d_tmem = tmem_base + buf * TILE_Q;
               if constexpr (PACKED) {
-                const uint32_t se = base + L::kScaleOff + stage * L::kTileBytes, exps = tmem_base + 256 + stage * kExpCols;
+                // Four blocks share a place in TMEM, one byte each. There are STAGES places: before one is written again its four
+                // blocks have left the ring.
+                const uint32_t se = base + L::kScaleOff + stage * L::kTileBytes, exps = tmem_base + 256 + (group % STAGES) * kExpCols;
                 // rows of 16 bytes without swizzle, eight of them 128 bytes apart from the next eight
                 const uint64_t de = (uint64_t((128u >> 4) | (1u << 14)) << 32) | uint64_t((1u << 16) | ((se >> 4) & 0x3fffu));
+                if ((kb & 3) == 0) {
 #pragma unroll
-                for (int j = 0; j <= TILE_Q / 128; ++j) tmem_copy_scales<CG>(exps + 4 * j, de + uint64_t(j * (512 >> 4)));
+                  for (int j = 0; j <= TILE_Q / 128; ++j) tmem_copy_scales<CG>(exps + 4 * j, de + uint64_t(j * (512 >> 4)));
+                }
+                const uint32_t idesc = p.idesc | (uint32_t)(kb & 3) << 4 | (uint32_t)(kb & 3) << 29;  // the byte of V's and of U's
 #pragma unroll
                 for (int j = 0; j < k8TK / 32; ++j)
-                  umma_mxf8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), p.idesc, exps, exps + 4,
+                  umma_mxf8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), idesc, exps, exps + 4,
                                 kb != kb0 || j != 0 ? 1u : 0u);
               }
 #pragma unroll

@@ -157,10 +157,10 @@ static __device__ __noinline__ void store_row8_slow(uint8_t* dst, uint32_t lo, u
   for (int j = 0; j < min(n, 8); ++j) dst[j] = (uint8_t)(v >> (8 * j));
 }
 
-// Packed scales: 512 bytes for each 128 rows of an operand and K block; row r of them is the 32-bit word r % 32 * 4 + r / 32, its
-// scale's exponent in all four bytes (one for each 32 of the block's 128 elements, as the tensor core takes them).
-__device__ __forceinline__ void store_packed(float* tiles, long long tile, int r, uint32_t bits) {
-  reinterpret_cast<uint32_t*>(tiles)[tile * 128 + (r & 31) * 4 + (r >> 5)] = (bits >> 23) * 0x01010101u;
+// Packed scales: 512 bytes for 128 rows of an operand and four K blocks, as the tensor core takes them; row r and block b are byte
+// r % 32 * 16 + r / 32 * 4 + b % 4, the scale's exponent. `step`: tiles from four blocks to the next four.
+__device__ __forceinline__ void store_packed(float* tiles, long long step, int row_tile, int block, int r, uint32_t bits) {
+  reinterpret_cast<uint8_t*>(tiles)[((block >> 2) * step + row_tile) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (block & 3)] = (uint8_t)(bits >> 23);
 }
 
 // MODE: 1 = groups along rows, 2 = along columns, 4 = 128 x 128 blocks (written through the row members).
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     const int own = ty + 16 * (tx >> 1);
     if ((tx & 1) == 0 && own < nrow) {
       if (p.packed)
-        store_packed(p.s_row, (long long)tc * p.sr_group + tr, own, sb);
+        store_packed(p.s_row, p.sr_group, tr, tc, own, sb);
       else
         p.s_row[(long long)(r0 + own) * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
     }
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
       const int c = tc * 128 + threadIdx.x;
       if (c < p.cols) {
         if (p.packed)
-          store_packed(p.s_col, (long long)tr * p.sc_group + tc, threadIdx.x, sb);
+          store_packed(p.s_col, p.sc_group, tc, tr, threadIdx.x, sb);
         else
           p.s_col[(long long)tr * p.sc_group + (long long)c * p.sc_col] = __uint_as_float(sb);
         if (p.colsum != nullptr) {
@@ -356,7 +356,10 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w]);
     const uint32_t sb = scale_bits(m, n);
     if (p.packed) {
-      if (threadIdx.x < 128) store_packed(p.s_row, (long long)tc * p.sr_group + tr, threadIdx.x, sb);
+      if (threadIdx.x < 128)
+        store_packed(p.s_row, p.sr_group, tr, tc, threadIdx.x, sb);
+      else if (p.s_col != nullptr)
+        store_packed(p.s_col, p.sc_group, tc, tr, threadIdx.x - 128, sb);
     } else if (threadIdx.x == 0) {
       p.s_row[(long long)tr * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
     }

@@ -363,9 +363,13 @@ class _Pieces:
         self.size += _up(nbytes, 256)
         return at
 
-    def quantized(self, rows: int, cols: int) -> tuple:
-        """(values, exponent tiles) of a matrix; the values' pitch is a multiple of 16."""
-        return self.add(rows * _up(cols, 16)), self.add(512 * _blocks(rows) * _blocks(cols))
+    def quantized(self, rows: int, cols: int, by_col: bool = False) -> tuple:
+        """(values, exponent tiles for 128 rows and four groups of columns, or the other way round) of a matrix; the values'
+        pitch is a multiple of 16."""
+        return self.add(rows * _up(cols, 16)), self.tiles(cols, rows) if by_col else self.tiles(rows, cols)
+
+    def tiles(self, rows: int, k: int) -> int:
+        return self.add(512 * _blocks(rows) * -(-_blocks(k) // 4))
 
 
 def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
@@ -400,8 +404,9 @@ class _ForwardPlan:
         temp, keep = _Pieces(), _Pieces()
         self.xr = temp.quantized(m, k)
         # what the backward pass reads: x by columns and the weight, as far as they are needed
-        self.xc = keep.quantized(m, k) if need_w else None
+        self.xc = keep.quantized(m, k, True) if need_w else None
         self.wq = (keep if need_x else temp).quantized(n, k)
+        self.wt = keep.tiles(k, n) if need_x else None  # the weight's scales as dx needs them, with K = n
         self.temp_size, self.keep_size = temp.size, keep.size
         self.quant_x = _quant_sizes(m, k, x_ld, _F_ID[x_dtype], e4, 3 if need_w else 1, 0, True)
         self.quant_w = _quant_sizes(n, k, w_ld, _F_ID[w_dtype], e4, 4, 0, True)
@@ -416,14 +421,14 @@ class _BackwardPlan:
         temp = _Pieces()
         by_col = need_w or need_b
         self.gr = temp.quantized(m, n) if need_x else None
-        self.gc = temp.quantized(m, n) if by_col else None
+        self.gc = temp.quantized(m, n, True) if by_col else None
         self.pitch = _up(n, 4)
         self.sums = temp.add(4 * _blocks(m) * self.pitch) if need_b else None
         self.temp_size = temp.size
         self.quant = (_quant_sizes(m, n, g_ld, _F_ID[g_dtype], g_id, 3 if need_x and by_col else 2 if by_col else 1, self.pitch, True)
                       if m and n else None)
         np_, kp, full = _up(n, 16), _up(k, 16), m and n and k
-        self.dx = _gemm_sizes(m, k, n, np_, kp, (1, _blocks(m), _blocks(n), 1), False, False, g_id, e4, _F_ID[x_dtype], 0, num_sms) if full else None
+        self.dx = _gemm_sizes(m, k, n, np_, kp, (1, _blocks(m), 1, _blocks(k)), False, False, g_id, e4, _F_ID[x_dtype], 0, num_sms) if full else None
         self.dw = _gemm_sizes(n, k, m, np_, kp, (1, _blocks(n), 1, _blocks(k)), True, False, g_id, e4, _F_ID[w_dtype], 0, num_sms) if full else None
 
 
@@ -455,7 +460,7 @@ class _Linear8(torch.autograd.Function):
                 temp_ptr, keep_ptr = temp.data_ptr(), keep.data_ptr()
                 xr, wq = _at(temp_ptr, plan.xr), _at(keep_ptr if need_x else temp_ptr, plan.wq)
                 _call_quantize(x2.data_ptr(), plan.quant_x, xr, _at(keep_ptr, plan.xc), 0, stream)
-                _call_quantize(w2.data_ptr(), plan.quant_w, wq, (0, 0), 0, stream)
+                _call_quantize(w2.data_ptr(), plan.quant_w, wq, (0, keep_ptr + plan.wt if need_x else 0), 0, stream)
                 _call_gemm((xr[0], wq[0], xr[1], wq[1], y.data_ptr(), 0 if bias is None else bias.data_ptr()), plan.gemm,
                            _workspace_for(device, stream).status_bytes, stream)
             elif k == 0:
@@ -486,8 +491,8 @@ class _Linear8(torch.autograd.Function):
             if need_x:
                 dx = torch.empty(shape, dtype=x_dtype, device=device)
                 if plan.dx is not None:
-                    wq = _at(keep_ptr, ctx.plan.wq)
-                    _call_gemm((gr[0], wq[0], gr[1], wq[1], dx.data_ptr(), 0), plan.dx, status, stream)
+                    fwd = ctx.plan
+                    _call_gemm((gr[0], keep_ptr + fwd.wq[0], gr[1], keep_ptr + fwd.wt, dx.data_ptr(), 0), plan.dx, status, stream)
                 else:
                     dx.zero_()
             if need_w:

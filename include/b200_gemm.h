@@ -266,9 +266,9 @@ typedef struct b200_gemm_a8w8_args {
   int32_t a_dtype, b_dtype;     /* B200_GEMM_DTYPE_E4M3 or _E5M2, each operand its own                               */
   int32_t a_block, b_block;     /* 1: a scale per 128 rows of A / columns of B, 0: one per row / column; 2, for both operands: powers
                                    of two as exponent tiles, which the tensor core applies. A tile holds the scales of 128 rows
-                                   of A (columns of B) for one K block in 512 bytes: row r is the 32-bit word r % 32 * 4 + r / 32, the
-                                   scale's biased fp32 exponent in each of its bytes. The tile of rows 128 i.. and K block b is at
-                                   a_scale + 512 bytes * (i * sa_row + b * sa_kb); a_scale starts on 16 bytes. Tilings: tile_n 128, or
+                                   of A (columns of B) for four K blocks in 512 bytes: byte r % 32 * 16 + r / 32 * 4 + b % 4 is the biased
+                                   fp32 exponent of the scale of row r and block b. The tile of rows 128 i.. and K blocks 4 j.. is at
+                                   a_scale + 512 bytes * (i * sa_row + j * sa_kb); a_scale starts on 16 bytes. Tilings: tile_n 128, or
                                    256 with cta_group 2; no swap_ab or split_k                                             */
   int32_t out_dtype, bias_dtype; /* B200_GEMM_DTYPE_FP32, _BF16 or _FP16, in any combination                           */
   b200_gemm_policy policy; /* tile_n 16, 32, 64, 128 (one CTA per 128 rows) or 128, 256 (cta_group 2); split_k > 1: the K blocks
@@ -301,9 +301,10 @@ typedef struct b200_gemm_quantize_args {
   int32_t in_dtype, out_dtype; /* FP32 / BF16 / FP16; E4M3 / E5M2                                                     */
   int32_t mode;                /* 1: groups of 128 columns in a row; 2: of 128 rows in a column; 3: both, two outputs from one
                                   read; 4: 128 x 128 blocks (written through q_row, s_row)                            */
-  int32_t packed;              /* 1: scales as exponent tiles (below) instead: the one of rows 128 r.., group g at s_row + 512 bytes
-                                  * (g * sr_group + r), of columns 128 c.. at s_col + 512 bytes * (g * sc_group + c); modes 1 and 4
-                                  fill one tile per 128 rows and group; entries of rows outside the matrix are not written */
+  int32_t packed;              /* 1: scales as the exponent tiles of b200_gemm_a8w8 instead: rows 128 r.., groups 4 g.. at s_row + 512
+                                  bytes * (g * sr_group + r); columns 128 c.., groups 4 g.. at s_col + 512 bytes * (g * sc_group + c),
+                                  which mode 4 writes too unless s_col is NULL. Bytes of rows, columns and groups outside the
+                                  matrix are left as they were                                                        */
 } b200_gemm_quantize_args;
 int b200_gemm_quantize_a8(const b200_gemm_quantize_args* args, void* cuda_stream);
 
