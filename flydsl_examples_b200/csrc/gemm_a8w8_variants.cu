@@ -24,7 +24,7 @@ Variant8 make(int v_vector) {
 bool variant8(int tile_q, int cta_group, int v_vector, int packed, Variant8* out) {
   if (packed) {
     if (cta_group == 1 && tile_q == 128) return *out = make_one<128, 5, 1, false, true>(), true;
-    if (cta_group == 2 && tile_q == 256) return *out = make_one<256, 4, 2, false, true>(), true;
+    if (cta_group == 2 && tile_q == 256) return *out = make_one<256, 5, 2, false, true>(), true;
     return false;
   }
   if (cta_group == 1 && tile_q == 16) return *out = make<16, 10, 1>(v_vector), true;

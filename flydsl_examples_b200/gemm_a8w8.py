@@ -381,9 +381,10 @@ def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
 
 def _packed_policy(m, n, k, num_sms) -> tuple:
     """Tiling of a product whose scales are exponent tiles, as the fields of b200_gemm_policy: CTA pairs with 256 x 256 tiles or
-    CTAs with 128 x 128, by whole waves times the measured times of a tile and of a K block in it."""
-    pairs = -(-(-(-m // 256) * -(-n // 256)) // max(1, num_sms // 2)) * (5.0 + _blocks(k) * 0.45)
-    single = -(-(-(-m // 128) * -(-n // 128)) // num_sms) * (3.5 + _blocks(k) * 0.30)
+    CTAs with 128 x 128, by whole waves times the microseconds of a tile and of a K block in it (1024 x 2048 x 4096: pairs 16.5
+    us, single CTAs 14.2; 2048 x 4096 x 4096: 30.1 and 46.2; 4096 x 4096 x 128: 13.1 and 10.3)."""
+    pairs = -(-(-(-m // 256) * -(-n // 256)) // max(1, num_sms // 2)) * (2.2 + _blocks(k) * 0.36)
+    single = -(-(-(-m // 128) * -(-n // 128)) // num_sms) * (0.9 + _blocks(k) * 0.31)
     return (256 if pairs < single else 128, 0, 1, 8 if m > 1024 else 0, 0, 2 if pairs < single else 1) + (0,) * 10
 
 
