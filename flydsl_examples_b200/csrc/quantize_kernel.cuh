@@ -36,7 +36,7 @@ struct QuantParams {
   long long ldq_col;
   float* s_col;
   long long sc_group, sc_col;
-  int packed;     // scales as exponent bytes in tiles for the tensor core, see store_packed
+  int packed;  // scales as exponent bytes in tiles for the tensor core, see store_packed; s_col of mode 4: with K along the rows
   float* colsum;  // optional: sums of the tile's columns, [tile row][cols_pitch]
   long long colsum_ld;
 };
@@ -356,10 +356,9 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     for (int w = 0; w < 8; ++w) m = fmaxf(m, red[0][w]);
     const uint32_t sb = scale_bits(m, n);
     if (p.packed) {
-      if (threadIdx.x < 128)
-        store_packed(p.s_row, p.sr_group, tr, tc, threadIdx.x, sb);
-      else if (p.s_col != nullptr)
-        store_packed(p.s_col, p.sc_group, tc, tr, threadIdx.x - 128, sb);
+      const int i = threadIdx.x & 127;
+      if (threadIdx.x < 128 && i < nrow) store_packed(p.s_row, p.sr_group, tr, tc, i, sb);
+      if (threadIdx.x >= 128 && p.s_col != nullptr && tc * 128 + i < p.cols) store_packed(p.s_col, p.sc_group, tc, tr, i, sb);
     } else if (threadIdx.x == 0) {
       p.s_row[(long long)tr * p.sr_row + (long long)tc * p.sr_group] = __uint_as_float(sb);
     }

@@ -48,6 +48,30 @@ def test_plan_and_bad_policies():
     assert query(tile_n=16, split_k=16)[1].cluster_split == 2
 
 
+def test_exponent_tiles_plan_and_refusals():
+    both = dict(a_block=2, b_block=2, sa_kb=2, sb_kb=2)
+    rc, pl = query(**both)
+    assert rc == 0 and (pl.tile_n, pl.tmem_cols, pl.tiles_p, pl.tiles_q) == (128, 512, 2, 2) and pl.smem_bytes <= 227 * 1024
+    for layout in (dict(b_trans=0), dict(a_trans=1, b_trans=0), dict(a_trans=1)):
+        rc, pl = query(**both, tile_n=256, cta_group=2, **layout)
+        assert rc == 0 and pl.tile_m == 256 and pl.tmem_cols == 512 and pl.smem_bytes <= 227 * 1024
+    for bad in (dict(tile_n=64), dict(tile_n=16), dict(tile_n=128, cta_group=2), dict(split_k=2), dict(swap_ab=1)):
+        assert query(**both, **bad)[0] == -2, bad
+    for bad in (dict(a_block=2), dict(b_block=2), dict(a_block=3), dict(b_block=-1), dict(a_block=2, b_block=0)):
+        assert query(**bad)[0] == -1, bad
+    lib = _lib.load()
+    for bad in (dict(a_scale=4104), dict(b_scale=4100), dict(sa_row=-1), dict(sb_kb=-1)):
+        assert lib.b200_gemm_a8w8(C.byref(args8(**{**both, **bad})), None) == -1, bad
+
+
+def test_tiling_of_products_with_exponent_tiles():
+    for sms in (148, 74, 1):
+        for m, n, k in ((1, 1, 1), (300, 5000, 256), (1024, 2048, 4096), (2048, 4096, 4096), (8192, 8192, 8192)):
+            tile, stages, split, group, swap, cg, *rest = module._packed_policy(m, n, k, sms)
+            assert (tile, cg) in ((128, 1), (256, 2)) and (stages, split, swap) == (0, 1, 0) and not any(rest) and len(rest) == 10
+    assert module._packed_policy(8192, 8192, 8192, 148)[0] == 256 and module._packed_policy(16, 4096, 4096, 148)[0] == 128
+
+
 def test_entry_points_refuse_before_any_device_work():
     lib = _lib.load()
     for bad in (dict(a=None), dict(b_scale=None), dict(out=None), dict(a=4100), dict(b=8200), dict(lda=264), dict(a_scale=4098), dict(out=4097),
@@ -62,7 +86,7 @@ def test_entry_points_refuse_before_any_device_work():
             setattr(q, key, v)
         return lib.b200_gemm_quantize_a8(C.byref(q), None)
     for bad in (dict(rows=-1), dict(in_dtype=4), dict(out_dtype=2), dict(mode=0), dict(mode=5), dict(x=None), dict(ldx=63), dict(x=4097),
-                dict(q_row=None), dict(s_row=None), dict(ldq_row=63), dict(mode=2), dict(mode=3), dict(colsum=4096, colsum_ld=64)):
+                dict(q_row=None), dict(s_row=None), dict(ldq_row=63), dict(mode=2), dict(mode=3), dict(colsum=4096, colsum_ld=64), dict(packed=2), dict(packed=-1)):
         assert quant(**bad) == -1, bad
     assert quant(rows=0) == 0 and quant(cols=0) == 0 and lib.b200_gemm_quantize_a8(None, None) == -1
 

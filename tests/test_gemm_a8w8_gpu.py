@@ -4,12 +4,14 @@ Bounds. An 8-bit product is exact in fp32. With S = sum |a| |b| times the scales
 by a few units of 2^-23 of its S (four accumulating instructions; 8 units are allowed), each fp32 addition of the running
 sum and each product of scales adds at most 2^-24 of S: |error| <= (8 + blocks) * 2^-23 * S, plus half a step of the output type.
 """
+import ctypes as C
 import functools
 
 import pytest
 import torch
 
-from flydsl_examples_b200.gemm_a16w16 import check_status
+from flydsl_examples_b200 import _lib
+from flydsl_examples_b200.gemm_a16w16 import _workspace_for, check_status
 from flydsl_examples_b200.gemm_a8w8 import gemm_a8w8, linear_a8w8, plan, quantize_a8
 
 pytestmark = pytest.mark.gpu
@@ -455,3 +457,115 @@ def test_bias_types_and_offsets(kw, bias_dtype):
     wide = torch.randn(600, generator=g, device=DEV).to(bias_dtype)
     for bias in (wide[:277], wide[3:280], wide[:554:2]):  # aligned, off 16 bytes, strided
         check(gemm_a8w8(a, sa, b.t(), sb.t(), bias=bias, user_kwargs=kw, out_dtype=torch.float32), a, sa, b, sb, bias)
+
+
+# ------------------------------------------------------------------------------------------------------ exponent tiles
+# Every element of a block carries its scales into the tensor core, whose accumulator then holds the sum over all blocks: four
+# accumulating instructions per block instead of four in all, so |error| <= (8 * blocks) * 2^-23 * S.
+def tiles_of(s, fill):
+    """[K groups of four, row tiles, 512] bytes of power-of-two scales s [rows, K blocks]; bytes of no scale are `fill`."""
+    rows, nb = s.shape
+    out = torch.full((-(-nb // 4), blocks(rows), 512), fill, dtype=torch.uint8, device=s.device)
+    r = torch.arange(rows, device=s.device)
+    at = r % 32 * 16 + r % 128 // 32 * 4
+    for b in range(nb):
+        out[b // 4, r // 128, at + b % 4] = (s[:, b].contiguous().view(torch.int32) >> 23).to(torch.uint8)
+    return out
+
+
+def quantize_packed(x, mode, dtype, fill):
+    rows, cols = x.shape
+    pitch = -(-cols // 16) * 16
+    q = [torch.zeros(rows, pitch, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    by_row = torch.full((-(-blocks(cols) // 4), blocks(rows), 512), fill, dtype=torch.uint8, device=DEV)
+    by_col = torch.full((-(-blocks(rows) // 4), blocks(cols), 512), fill, dtype=torch.uint8, device=DEV)
+    a = _lib.QuantizeArgs()
+    for key, v in dict(x=x.data_ptr(), q_row=q[0].data_ptr(), s_row=by_row.data_ptr(), q_col=q[1].data_ptr(), s_col=by_col.data_ptr(), rows=rows,
+                       cols=cols, ldx=x.stride(0), ldq_row=pitch, sr_group=blocks(rows), ldq_col=pitch, sc_group=blocks(cols),
+                       in_dtype={torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}[x.dtype], out_dtype=4 if dtype == E4 else 5, mode=mode,
+                       packed=1).items():
+        setattr(a, key, v)
+    assert _lib.load().b200_gemm_quantize_a8(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    return [t[:, :cols].view(dtype) for t in q], by_row, by_col
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (128, 128), (130, 700), (517, 140), (640, 1100)])
+@pytest.mark.parametrize("mode", [1, 2, 3, 4])
+def test_quantizer_writes_the_same_scales_as_tiles(rows, cols, mode):
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    for x_dtype, dtype in ((torch.bfloat16, E4), (torch.float32, E5), (torch.float16, E4)):
+        x = (torch.randn(rows, cols, generator=g, device=DEV) * torch.exp2(torch.randint(-9, 5, (rows, cols), generator=g, device=DEV))).to(x_dtype)
+        x[rows // 2] = 0
+        (q_row, q_col), by_row, by_col = quantize_packed(x, mode, dtype, 0xAB)
+        if mode == 4:
+            q, s = quantize_a8(x, dtype=dtype, group="block")
+            assert torch.equal(by_row, tiles_of(s.repeat_interleave(128, 0)[:rows], 0xAB))
+            assert torch.equal(by_col, tiles_of(s.t().repeat_interleave(128, 0)[:cols], 0xAB))
+            assert torch.equal(q.view(torch.uint8), q_row.view(torch.uint8))
+            continue
+        if mode & 1:
+            q, s = quantize_a8(x, dtype=dtype, group="row")
+            assert torch.equal(by_row, tiles_of(s, 0xAB)) and torch.equal(q.view(torch.uint8), q_row.view(torch.uint8))
+        else:
+            assert (by_row == 0xAB).all()
+        if mode & 2:
+            q, s = quantize_a8(x, dtype=dtype, group="col")
+            assert torch.equal(by_col, tiles_of(s.t(), 0xAB)) and torch.equal(q.view(torch.uint8), q_col.view(torch.uint8))
+        else:
+            assert (by_col == 0xAB).all()
+
+
+def run_packed(m, n, k, layout, tile_n, ad=E4, bd=E4, out_dtype=torch.bfloat16, bias=False, spread=12, shift=0):
+    g = torch.Generator(device=DEV).manual_seed(m + 3 * n + 5 * k)
+    a, _ = operand(g, m, k, ad, False, layout[0] == "t")
+    b, _ = operand(g, n, k, bd, False, layout[1] == "n")
+    sa, sb = (torch.exp2(torch.randint(-spread, spread + 1, (r, blocks(k)), generator=g, device=DEV).float() + d) for r, d in ((m, shift), (n, -shift)))
+    ta, tb = tiles_of(sa, 0xFF), tiles_of(sb, 0xFF)  # 0xFF is NaN: what belongs to no row must not matter
+    bv = torch.randn(n, generator=g, device=DEV) if bias else None
+    guard = torch.full((m * n + 64,), 7.0, dtype=out_dtype, device=DEV)
+    args = _lib.Args8()
+    for key, v in dict(a=a.data_ptr(), b=b.data_ptr(), a_scale=ta.data_ptr(), b_scale=tb.data_ptr(), out=guard.data_ptr(), bias=bv.data_ptr() if bias else None,
+                       m=m, n=n, k=k, lda=a.stride(0) if layout[0] == "n" else a.stride(1), ldb=b.stride(0) if layout[1] == "t" else b.stride(1),
+                       ldo=n, sa_row=1, sa_kb=ta.shape[1], sb_col=1, sb_kb=tb.shape[1], a_trans=int(layout[0] == "t"), b_trans=int(layout[1] == "t"),
+                       a_dtype=4 if ad == E4 else 5, b_dtype=4 if bd == E4 else 5, a_block=2, b_block=2, bias_dtype=1 if bias else 0,
+                       out_dtype={torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}[out_dtype],
+                       status=_workspace_for(torch.device(DEV, torch.cuda.current_device()), torch.cuda.current_stream().cuda_stream).status_ptr).items():
+        setattr(args, key, v)
+    args.policy.tile_n, args.policy.cta_group, args.policy.group_m = tile_n, 2 if tile_n == 256 else 1, 8 if m > 1024 else 0
+    assert _lib.load().b200_gemm_a8w8(C.byref(args), torch.cuda.current_stream().cuda_stream) == 0
+    check_status()
+    assert (guard[m * n:] == 7).all()
+    got = guard[: m * n].view(m, n)
+    va, vb = values(a, sa), values(b, sb)
+    ref, mag = va @ vb.t(), va.abs() @ vb.abs().t()
+    if bias:
+        ref, mag = ref + bv.double(), mag + bv.double().abs()
+    bound = (8 * blocks(k) + 1) * 2.0 ** -23 * mag + torch.finfo(out_dtype).eps / 2 * 1.000001 * ref.abs()
+    bad = ~((got.double() - ref).abs() <= bound)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), got[bad][:4].tolist(), ref[bad][:4].tolist())
+
+
+@pytest.mark.parametrize("tile_n", [128, 256])
+@pytest.mark.parametrize("layout", ["nt", "nn", "tn", "tt"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (128, 128, 128), (256, 256, 512), (129, 257, 513), (300, 140, 1700), (1100, 530, 640), (2600, 2700, 150)])
+def test_product_with_exponent_tiles(m, n, k, layout, tile_n):
+    run_packed(m, n, k, layout, tile_n)
+    run_packed(m, n, k, layout, tile_n, E5, E4, torch.float32, bias=True)
+
+
+def test_product_with_exponent_tiles_of_extreme_scales():
+    run_packed(200, 300, 700, "nt", 256, out_dtype=torch.float32, spread=20, shift=100)
+    run_packed(200, 300, 700, "tn", 128, E4, E5, torch.float32, spread=20, shift=-100)
+
+
+def test_linear_of_tiny_by_huge_values():
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = (torch.randn(150, 600, generator=g, device=DEV) * torch.exp2(torch.randint(-110, -89, (150, 1), generator=g, device=DEV).float())).requires_grad_()
+    w = (torch.randn(200, 600, generator=g, device=DEV) * 2.0 ** 100).requires_grad_()
+    dy = torch.randn(150, 200, generator=g, device=DEV) * 2.0 ** -20
+    y = linear_a8w8(x, w)
+    y.backward(dy)
+    for got, (want, mag, nb) in zip((y.detach(), x.grad, w.grad), reference_linear(x.detach(), w.detach(), None, dy, E4)):
+        bound = (8 * nb + 1) * 2.0 ** -23 * mag + 2.0 ** -24 * 1.000001 * want.abs() + 2.0 ** -149
+        assert ((got.double() - want).abs() <= bound).all()
+    check_status()
