@@ -1,6 +1,7 @@
 // Host side of the 8-bit block-scaled GEMM and its quantizer: validation, plan, tensor maps, launch. Exports the
 // b200_gemm_a8w8_* and b200_gemm_quantize_a8 entry points of include/b200_gemm.h. No device allocation, no synchronisation.
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/b200_gemm.h"
 #include "gemm_a8w8_variants.h"
@@ -83,12 +84,14 @@ static int encode8(CUtensorMap* map, const void* ptr, int mn_major, int64_t rows
   return res == CUDA_SUCCESS ? 0 : B200_GEMM_ERR_TENSOR_MAP;
 }
 
+constexpr int64_t kMaxTiles = 0x0fffffff;  // 32-bit coordinates, with room for the tiles that a CTA asks for past the last row
+
 // The exponent tiles of an operand, 512 bytes each, as rows of 128 bytes.
 static int encode_tiles(CUtensorMap* map, const void* ptr, int64_t row_tiles, int64_t k_groups, int64_t s_row, int64_t s_kb) {
   EncodeTiledFn enc = get_encode_fn();
   if (enc == nullptr) return B200_GEMM_ERR_DRIVER;
   const int64_t tiles = (row_tiles - 1) * s_row + (k_groups - 1) * s_kb + 1;
-  if (tiles > 0x1fffffff) return B200_GEMM_ERR_TOO_LARGE;
+  if (tiles > kMaxTiles) return B200_GEMM_ERR_TOO_LARGE;
   cuuint64_t dims[2] = {128, (cuuint64_t)(4 * tiles)};
   cuuint64_t strides[1] = {128};
   cuuint32_t box[2] = {128, 4};
@@ -120,7 +123,11 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
   auto aligned = [](const void* ptr, int64_t to) { return (reinterpret_cast<uintptr_t>(ptr) % (uintptr_t)to) == 0; };
   if (!aligned(a->a, 16) || !aligned(a->b, 16) || a->lda % 16 != 0 || a->ldb % 16 != 0) return B200_GEMM_ERR_BAD_ARG;
   const int packed = a->a_block == 2;
-  if (packed && (a->sa_row < 0 || a->sa_kb < 0 || a->sb_col < 0 || a->sb_kb < 0)) return B200_GEMM_ERR_BAD_ARG;
+  if (packed)
+    for (const int64_t s : {a->sa_row, a->sa_kb, a->sb_col, a->sb_kb}) {
+      if (s < 0) return B200_GEMM_ERR_BAD_ARG;
+      if (s > kMaxTiles) return B200_GEMM_ERR_TOO_LARGE;
+    }
   if (!aligned(a->a_scale, packed ? 16 : 4) || !aligned(a->b_scale, packed ? 16 : 4) || !aligned(a->out, es)) return B200_GEMM_ERR_BAD_ARG;
   if (a->bias != nullptr && (a->bias_dtype < 1 || a->bias_dtype > 3 || !aligned(a->bias, a->bias_dtype == 1 ? 4 : 2)))
     return B200_GEMM_ERR_BAD_ARG;

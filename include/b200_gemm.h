@@ -261,7 +261,7 @@ typedef struct b200_gemm_a8w8_args {
   const void* bias;     /* bias[N], contiguous, of bias_dtype; NULL = none                                          */
   int64_t m, n, k;
   int64_t lda, ldb, ldo;              /* leading strides in elements, as for b200_gemm_args                              */
-  int64_t sa_row, sa_kb, sb_col, sb_kb; /* strides of the scales in elements                                               */
+  int64_t sa_row, sa_kb, sb_col, sb_kb; /* strides of the scales in elements (of exponent tiles: in tiles)              */
   int32_t a_trans, b_trans;
   int32_t a_dtype, b_dtype;     /* B200_GEMM_DTYPE_E4M3 or _E5M2, each operand its own                               */
   int32_t a_block, b_block;     /* 1: a scale per 128 rows of A / columns of B, 0: one per row / column; 2, for both operands: powers

@@ -62,6 +62,7 @@ def test_exponent_tiles_plan_and_refusals():
     lib = _lib.load()
     for bad in (dict(a_scale=4104), dict(b_scale=4100), dict(sa_row=-1), dict(sb_kb=-1)):
         assert lib.b200_gemm_a8w8(C.byref(args8(**{**both, **bad})), None) == -1, bad
+    assert lib.b200_gemm_a8w8(C.byref(args8(**{**both, "sa_row": 1 << 28})), None) == -7
 
 
 def test_tiling_of_products_with_exponent_tiles():
