@@ -119,6 +119,15 @@ class QuantizeArgs(C.Structure):
     )
 
 
+class ReduceArgs(C.Structure):
+    """b200_gemm_reduce_args"""
+    _fields_ = (
+        [(n, C.c_void_p) for n in ("slots", "out", "bias")]
+        + [(n, C.c_int64) for n in ("slot_stride", "rows", "cols")]
+        + [(n, C.c_int32) for n in ("n_slots", "out_dtype", "bias_dtype", "reserved")]
+    )
+
+
 class MoeArgs(C.Structure):
     """b200_gemm_moe_args"""
     _fields_ = (
@@ -154,6 +163,7 @@ EXPORTS = (
     "b200_gemm_a8w8",
     "b200_gemm_a8w8_plan_query",
     "b200_gemm_quantize_a8",
+    "b200_gemm_sequence",
     "b200_gemm_moe_a16w16",
     "b200_gemm_moe_workspace_bytes",
     "b200_gemm_cast_bias",
@@ -217,6 +227,8 @@ def load() -> C.CDLL:
     lib.b200_gemm_a8w8_plan_query.restype = C.c_int
     lib.b200_gemm_quantize_a8.argtypes = [C.POINTER(QuantizeArgs), C.c_void_p]
     lib.b200_gemm_quantize_a8.restype = C.c_int
+    lib.b200_gemm_sequence.argtypes = [C.c_char_p, C.c_void_p]
+    lib.b200_gemm_sequence.restype = C.c_int
     lib.b200_gemm_moe_a16w16.argtypes = [C.POINTER(MoeArgs), C.c_void_p]
     lib.b200_gemm_moe_a16w16.restype = C.c_int
     lib.b200_gemm_moe_workspace_bytes.argtypes = [C.POINTER(MoeArgs)]

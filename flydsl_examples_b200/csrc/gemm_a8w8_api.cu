@@ -293,4 +293,27 @@ int b200_gemm_quantize_a8(const b200_gemm_quantize_args* a, void* cuda_stream) {
   return e == cudaSuccess ? 0 : b200::set_cuda_error(e);
 }
 
+int b200_gemm_sequence(const void* records, void* cuda_stream) {
+  const char* r = static_cast<const char*>(records);
+  if (r == nullptr || reinterpret_cast<uintptr_t>(r) % 8 != 0) return B200_GEMM_ERR_BAD_ARG;
+  for (;;) {
+    const int64_t kind = *reinterpret_cast<const int64_t*>(r);
+    r += 8;
+    int rc = B200_GEMM_ERR_BAD_ARG;
+    if (kind == 0) return 0;
+    if (kind == 1) {
+      rc = b200_gemm_a8w8(reinterpret_cast<const b200_gemm_a8w8_args*>(r), cuda_stream);
+      r += sizeof(b200_gemm_a8w8_args);
+    } else if (kind == 2) {
+      rc = b200_gemm_quantize_a8(reinterpret_cast<const b200_gemm_quantize_args*>(r), cuda_stream);
+      r += sizeof(b200_gemm_quantize_args);
+    } else if (kind == 3) {
+      const b200_gemm_reduce_args* a = reinterpret_cast<const b200_gemm_reduce_args*>(r);
+      rc = b200_gemm_reduce_slots(a->slots, a->slot_stride, a->n_slots, a->out, a->bias, a->rows, a->cols, a->out_dtype, a->bias_dtype, cuda_stream);
+      r += sizeof(b200_gemm_reduce_args);
+    }
+    if (rc) return rc;
+  }
+}
+
 }  // extern "C"

@@ -372,11 +372,15 @@ class _Pieces:
         return self.add(512 * _blocks(rows) * -(-_blocks(k) // 4))
 
 
-def _call_quantize(x_ptr, sizes, row, col, sums, stream) -> None:
-    """row, col: device addresses of (values, scales); sums: of the columns' sums."""
-    rc = _lib.fast("b200_gemm_quantize_a8")(_POINTERS.pack(x_ptr, *row, *col, sums) + sizes, stream)
+# The layer's launches leave in one call: records of b200_gemm_sequence, whose constant parts are worked out once.
+_QUANT_RECORD, _GEMM_RECORD, _REDUCE_RECORD = "q6P96s", "q6P176s8s", "q3P40s"
+_REDUCE_SIZES = struct.Struct("@3q4i")
+
+
+def _run(records: bytes, stream) -> None:
+    rc = _lib.fast("b200_gemm_sequence")(records, stream)
     if rc != 0:
-        raise RuntimeError(f"b200_gemm_quantize_a8 failed ({rc}): {_lib.strerror(rc)}")
+        raise RuntimeError(f"b200_gemm_sequence failed ({rc}): {_lib.strerror(rc)}")
 
 
 def _packed_policy(m, n, k, num_sms) -> tuple:
@@ -390,13 +394,6 @@ def _packed_policy(m, n, k, num_sms) -> tuple:
 
 def _gemm_sizes(m, n, k, lda, ldb, scale_strides, a_t, b_t, a_id, b_id, out_id, bias_id, num_sms) -> bytes:
     return _SIZES.pack(m, n, k, lda, ldb, n, *scale_strides, a_t, b_t, a_id, b_id, 2, 2, out_id, bias_id, *_packed_policy(m, n, k, num_sms))
-
-
-def _call_gemm(pointers, sizes, status, stream) -> None:
-    """pointers: a, b, a_scale, b_scale, out, bias."""
-    rc = _lib.fast("b200_gemm_a8w8")(_POINTERS.pack(*pointers) + sizes + status, stream)
-    if rc != 0:
-        raise RuntimeError(f"b200_gemm_a8w8 failed ({rc}): {_lib.strerror(rc)}")
 
 
 class _ForwardPlan:
@@ -414,10 +411,11 @@ class _ForwardPlan:
         kp = _up(k, 16)
         self.gemm = _gemm_sizes(m, n, k, kp, kp, (1, _blocks(m), 1, _blocks(n)), False, True, e4, e4, _F_ID[x_dtype],
                                 0 if bias_dtype is None else _F_ID[bias_dtype], num_sms) if m and n and k else None
+        self.records = struct.Struct("@" + 2 * _QUANT_RECORD + _GEMM_RECORD + "q")
 
 
 class _BackwardPlan:
-    def __init__(self, m, n, k, g_ld, g_dtype, g_id, x_dtype, w_dtype, need_x, need_w, need_b, num_sms):
+    def __init__(self, m, n, k, g_ld, g_dtype, g_id, x_dtype, w_dtype, b_dtype, need_x, need_w, need_b, num_sms):
         e4 = _lib.DTYPE_E4M3
         temp = _Pieces()
         by_col = need_w or need_b
@@ -431,6 +429,9 @@ class _BackwardPlan:
         np_, kp, full = _up(n, 16), _up(k, 16), m and n and k
         self.dx = _gemm_sizes(m, k, n, np_, kp, (1, _blocks(m), 1, _blocks(k)), False, False, g_id, e4, _F_ID[x_dtype], 0, num_sms) if full else None
         self.dw = _gemm_sizes(n, k, m, np_, kp, (1, _blocks(n), 1, _blocks(k)), True, False, g_id, e4, _F_ID[w_dtype], 0, num_sms) if full else None
+        self.reduce = _REDUCE_SIZES.pack(self.pitch, 1, self.pitch, _blocks(m), _F_ID[b_dtype], 0, 0) if need_b else None
+        self.records = struct.Struct("@" + _QUANT_RECORD + (_GEMM_RECORD if need_x and full else "") + (_GEMM_RECORD if need_w and full else "")
+                                     + (_REDUCE_RECORD if need_b else "") + "q") if m and n else None
 
 
 _forward_plan = functools.lru_cache(maxsize=1024)(_ForwardPlan)
@@ -460,10 +461,11 @@ class _Linear8(torch.autograd.Function):
                 temp = torch.empty(plan.temp_size, dtype=torch.uint8, device=device)
                 temp_ptr, keep_ptr = temp.data_ptr(), keep.data_ptr()
                 xr, wq = _at(temp_ptr, plan.xr), _at(keep_ptr if need_x else temp_ptr, plan.wq)
-                _call_quantize(x2.data_ptr(), plan.quant_x, xr, _at(keep_ptr, plan.xc), 0, stream)
-                _call_quantize(w2.data_ptr(), plan.quant_w, wq, (0, keep_ptr + plan.wt if need_x else 0), 0, stream)
-                _call_gemm((xr[0], wq[0], xr[1], wq[1], y.data_ptr(), 0 if bias is None else bias.data_ptr()), plan.gemm,
-                           _workspace_for(device, stream).status_bytes, stream)
+                _run(plan.records.pack(
+                    2, x2.data_ptr(), *xr, *_at(keep_ptr, plan.xc), 0, plan.quant_x,
+                    2, w2.data_ptr(), *wq, 0, keep_ptr + plan.wt if need_x else 0, 0, plan.quant_w,
+                    1, xr[0], wq[0], xr[1], wq[1], y.data_ptr(), 0 if bias is None else bias.data_ptr(), plan.gemm,
+                    _workspace_for(device, stream).status_bytes, 0), stream)
             elif k == 0:
                 y.zero_() if bias is None else y.copy_(bias.expand_as(y))
         ctx.save_for_backward(keep)
@@ -479,7 +481,8 @@ class _Linear8(torch.autograd.Function):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         g = _row_major(dy if dy.ndim == 2 else dy.reshape(m, n))  # an expanded gradient (of a sum) is spread out here
         index, device = dy.get_device(), dy.device
-        plan = _backward_plan(m, n, k, g.stride(0) if m > 1 else n, g.dtype, g_id, x_dtype, w_dtype, need_x, need_w, need_b, device_sms(index))
+        plan = _backward_plan(m, n, k, g.stride(0) if m > 1 else n, g.dtype, g_id, x_dtype, w_dtype, b_dtype, need_x, need_w, need_b,
+                              device_sms(index))
         dx = dw = db = None
         with on_device(index, None):
             stream = raw_stream(index)
@@ -487,32 +490,30 @@ class _Linear8(torch.autograd.Function):
             temp = torch.empty(plan.temp_size, dtype=torch.uint8, device=device)
             base, keep_ptr = temp.data_ptr(), keep.data_ptr()
             gr, gc = _at(base, plan.gr), _at(base, plan.gc)
-            if plan.quant is not None and (need_x or need_w or need_b):
-                _call_quantize(g.data_ptr(), plan.quant, gr, gc, base + plan.sums if need_b else 0, stream)
+            records = [2, g.data_ptr(), *gr, *gc, base + plan.sums if need_b else 0, plan.quant]
             if need_x:
                 dx = torch.empty(shape, dtype=x_dtype, device=device)
                 if plan.dx is not None:
-                    fwd = ctx.plan
-                    _call_gemm((gr[0], keep_ptr + fwd.wq[0], gr[1], keep_ptr + fwd.wt, dx.data_ptr(), 0), plan.dx, status, stream)
+                    records += (1, gr[0], keep_ptr + ctx.plan.wq[0], gr[1], keep_ptr + ctx.plan.wt, dx.data_ptr(), 0, plan.dx, status)
                 else:
                     dx.zero_()
             if need_w:
                 dw = torch.empty(n, k, dtype=w_dtype, device=device)
                 if plan.dw is not None:
                     xc = _at(keep_ptr, ctx.plan.xc)
-                    _call_gemm((gc[0], xc[0], gc[1], xc[1], dw.data_ptr(), 0), plan.dw, status, stream)
+                    records += (1, gc[0], xc[0], gc[1], xc[1], dw.data_ptr(), 0, plan.dw, status)
                 else:
                     dw.zero_()
             if need_b:
                 db = torch.empty(plan.pitch, dtype=b_dtype, device=device)
-                if plan.quant is not None:  # the columns' sums over each 128 rows, added in order
-                    rc = _lib.load().b200_gemm_reduce_slots(base + plan.sums, plan.pitch, _blocks(m), db.data_ptr(), None, 1, plan.pitch,
-                                                            _F_ID[b_dtype], 0, stream)
-                    if rc != 0:
-                        raise RuntimeError(f"b200_gemm_reduce_slots failed ({rc}): {_lib.strerror(rc)}")
+                if plan.records is not None:  # the columns' sums over each 128 rows, added in order
+                    records += (3, base + plan.sums, db.data_ptr(), 0, plan.reduce)
                 else:
                     db.zero_()
-                db = db[:n]
+                if plan.pitch != n:
+                    db = db[:n]
+            if plan.records is not None and (need_x or need_w or need_b):
+                _run(plan.records.pack(*records, 0), stream)
         return dx, dw, db, None
 
 

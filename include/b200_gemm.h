@@ -308,6 +308,19 @@ typedef struct b200_gemm_quantize_args {
 } b200_gemm_quantize_args;
 int b200_gemm_quantize_a8(const b200_gemm_quantize_args* args, void* cuda_stream);
 
+/* Several calls on one stream in one, for hosts whose calls cost more than the launches: `records` (8-byte aligned) is a run of
+ * records, each an int64 kind and the argument block of that call, ended by a kind of 0. Kinds: 1 b200_gemm_a8w8_args,
+ * 2 b200_gemm_quantize_args, 3 b200_gemm_reduce_args (b200_gemm_reduce_slots). The first call that fails ends the run and its
+ * code is returned; the ones before it are launched. */
+typedef struct b200_gemm_reduce_args {
+  const float* slots;
+  void* out;
+  const void* bias;
+  int64_t slot_stride, rows, cols;
+  int32_t n_slots, out_dtype, bias_dtype, reserved;
+} b200_gemm_reduce_args;
+int b200_gemm_sequence(const void* records, void* cuda_stream);
+
 /* ---------------------------------------------------------------------------------------------------------------------
  * A mixture-of-experts layer for a few tokens, in two kernels.
  *   p = softmax(logits[t, :]); the top_k experts of each token, ties to the lowest index; weights divided by their sum when

@@ -1,5 +1,6 @@
 """Refusals, policy and structures of the 8-bit product, without a GPU."""
 import ctypes as C
+import struct
 
 import pytest
 import torch
@@ -65,6 +66,20 @@ def test_exponent_tiles_plan_and_refusals():
     assert lib.b200_gemm_a8w8(C.byref(args8(**{**both, "sa_row": 1 << 28})), None) == -7
 
 
+def test_sequences_of_calls():
+    lib = _lib.load()
+    run = lambda *words: lib.b200_gemm_sequence(struct.pack(f"@{len(words)}q", *words), None)  # noqa: E731
+    assert run(0) == 0 and run(4, 0) == -1 and run(-1, 0) == -1 and lib.b200_gemm_sequence(None, None) == -1
+    quant = bytes(_lib.QuantizeArgs(rows=0, cols=8, in_dtype=1, out_dtype=4, mode=1))
+    assert lib.b200_gemm_sequence(struct.pack("@q", 2) + quant + struct.pack("@q", 0), None) == 0
+    bad = bytes(args8(m=0))
+    assert lib.b200_gemm_sequence(struct.pack("@q", 2) + quant + struct.pack("@q", 1) + bad + struct.pack("@q", 0), None) == -1
+    assert lib.b200_gemm_sequence(struct.pack("@q", 3) + bytes(_lib.ReduceArgs(rows=1, cols=4)) + struct.pack("@q", 0), None) == -1
+    # the records that the linear layer packs
+    for record, st in ((module._QUANT_RECORD, _lib.QuantizeArgs), (module._GEMM_RECORD, _lib.Args8), (module._REDUCE_RECORD, _lib.ReduceArgs)):
+        assert struct.calcsize("@" + record) == 8 + C.sizeof(st)
+
+
 def test_tiling_of_products_with_exponent_tiles():
     for sms in (148, 74, 1):
         for m, n, k in ((1, 1, 1), (300, 5000, 256), (1024, 2048, 4096), (2048, 4096, 4096), (8192, 8192, 8192)):
@@ -100,13 +115,15 @@ def test_structures_match_the_header(tmp_path):
     cc = shutil.which("gcc") or shutil.which("cc")
     if cc is None:
         pytest.skip("no host C compiler")
-    pairs = (("b200_gemm_a8w8_args", _lib.Args8), ("b200_gemm_quantize_args", _lib.QuantizeArgs))
+    pairs = (("b200_gemm_a8w8_args", _lib.Args8), ("b200_gemm_quantize_args", _lib.QuantizeArgs),
+             ("b200_gemm_reduce_args", _lib.ReduceArgs))
     lines, want = [], []
     for name, st in pairs:
         lines.append(f'printf("%zu\\n", sizeof({name}));')
         want.append(C.sizeof(st))
-        tail = module._SIZES.size + 8 if st is _lib.Args8 else module._QUANT_SIZES.size
-        assert module._POINTERS.size + tail == C.sizeof(st)  # the byte string that the Python calls pass
+        tail = {_lib.Args8: module._SIZES.size + 8, _lib.QuantizeArgs: module._QUANT_SIZES.size}.get(st)
+        if tail is not None:
+            assert module._POINTERS.size + tail == C.sizeof(st)  # the byte string that the Python calls pass
         for field, _ in st._fields_:
             lines.append(f'printf("%zu\\n", offsetof({name}, {field}));')
             want.append(getattr(st, field).offset)
