@@ -23,10 +23,9 @@
 // are as good as those above: relative errors of 1e-8 to 6e-7 at K = 128 to 4096.
 //
 // Roles (384 threads): warp 0 = TMA producer, warp 1 = TMEM owner and MMA issuer, warps 2-3 = scale loaders (PACKED: idle, the
-// producer loads the exponents), warps 4-11 =
-// epilogue (warp w reads TMEM lanes 32 * (w % 4).. and column half (w - 4) / 4). The scale loaders copy the scales of a
-// K block into an eight-deep ring with 4-byte cp.async, whose completion arrives on the ring's barrier by itself: any
-// strides are served, nobody waits for a load, and rows outside the operand get zero.
+// producer loads the exponents), warps 4-11 = epilogue (warp w reads TMEM lanes 32 * (w % 4).. and column half (w - 4) / 4). The
+// scale loaders copy the scales of a K block into an eight-deep ring with 4-byte cp.async, whose completion arrives on the
+// ring's barrier by itself: any strides are served, nobody waits for a load, and rows outside the operand get zero.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
