@@ -18,16 +18,28 @@ namespace b200 {
 constexpr uint64_t kCounterBytes = 1u << 20;  // fixed ticket region at the start of the workspace (262144 tiles)
 
 // ------------------------------------------------------------------ driver entry point (no -lcuda link needed)
+// The driver's function of that name; null when it has none.
+static void* driver_entry(const char* name) {
+  void* ptr = nullptr;
+  cudaDriverEntryPointQueryResult qres;
+  if (cudaGetDriverEntryPoint(name, &ptr, cudaEnableDefault, &qres) == cudaSuccess && qres == cudaDriverEntryPointSuccess) return ptr;
+  return nullptr;
+}
+
 EncodeTiledFn get_encode_fn() {
+  typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
   static EncodeTiledFn fn = nullptr;
+  static CtxGetCurrentFn current = nullptr;
   static std::once_flag once;
   std::call_once(once, []() {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+    fn = reinterpret_cast<EncodeTiledFn>(driver_entry("cuTensorMapEncodeTiled"));
+    current = reinterpret_cast<CtxGetCurrentFn>(driver_entry("cuCtxGetCurrent"));
   });
+  // The driver encodes only with a context, which a thread gets with its first runtime call that needs one; where this is the
+  // thread's first, its device's is made current.
+  CUcontext ctx = nullptr;
+  int dev = 0;
+  if (current != nullptr && current(&ctx) == CUDA_SUCCESS && ctx == nullptr && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
   return fn;
 }
 
@@ -36,13 +48,7 @@ typedef CUresult (*GetAddressRangeFn)(CUdeviceptr*, size_t*, CUdeviceptr);
 static GetAddressRangeFn get_address_range_fn() {
   static GetAddressRangeFn fn = nullptr;
   static std::once_flag once;
-  std::call_once(once, []() {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuMemGetAddressRange", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<GetAddressRangeFn>(ptr);
-  });
+  std::call_once(once, []() { fn = reinterpret_cast<GetAddressRangeFn>(driver_entry("cuMemGetAddressRange")); });
   return fn;
 }
 

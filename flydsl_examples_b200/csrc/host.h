@@ -12,7 +12,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// cuTensorMapEncodeTiled, looked up once; null when the driver does not have it.
+// cuTensorMapEncodeTiled, looked up once; null when the driver does not have it. Gives the calling thread a context if it has none.
 EncodeTiledFn get_encode_fn();
 
 // Keeps the error's text for b200_gemm_strerror and returns B200_GEMM_ERR_LAUNCH.
