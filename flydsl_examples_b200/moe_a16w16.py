@@ -79,19 +79,12 @@ def _launch_moe(x, logits, w13, w2, out, need, sizes, index) -> torch.Tensor:
     """On the current device and stream."""
     device = x.device
     stream_ptr = raw_stream(index)
-    ws = _workspace_for(device, stream_ptr)
-    if torch.cuda.is_current_stream_capturing():
-        # a graph keeps scratch of its own (its memory pool's), so that two graphs may run at once
-        scratch = torch.empty(need, dtype=torch.uint8, device=device)
-        at = scratch.data_ptr()
-    else:
-        # behind the split-K tickets that the 16-bit GEMM keeps at the start of the stream's workspace
-        scratch = ws.buf  # held until the launch: another thread may put a larger one in its place
-        if scratch is None or scratch.numel() < _lib.COUNTER_BYTES + need:
-            ws.ensure(_lib.COUNTER_BYTES + need, device, torch.cuda.current_stream(index))
-            scratch = ws.buf
-        at = scratch.data_ptr() + _lib.COUNTER_BYTES
-    args = _POINTERS.pack(x.data_ptr(), logits.data_ptr(), w13.data_ptr(), w2.data_ptr(), out.data_ptr()) + sizes + _SCRATCH.pack(at, need) + ws.status_bytes
+    # Scratch of this call's own, from the stream's (or a graph's) pool. Its two launches are not one step: another thread's call on
+    # this stream, or a GEMM that uses the stream's workspace, may come between them. (With a buffer that the stream's calls
+    # shared one token took 10.3 us of host time, it takes 12.0 so; a replayed graph pays nothing.)
+    scratch = torch.empty(need, dtype=torch.uint8, device=device)
+    args = (_POINTERS.pack(x.data_ptr(), logits.data_ptr(), w13.data_ptr(), w2.data_ptr(), out.data_ptr()) + sizes
+            + _SCRATCH.pack(scratch.data_ptr(), need) + _workspace_for(device, stream_ptr).status_bytes)
     rc = _lib.fast("b200_gemm_moe_a16w16")(args, stream_ptr)
     if rc != 0:
         raise RuntimeError(f"b200_gemm_moe_a16w16 failed ({rc}): {_lib.strerror(rc)}")

@@ -94,3 +94,40 @@ def test_python_refusals():
         moe_a16w16(x, logits, w13, w2, 2, out=torch.zeros(4, 72, dtype=bf))
     with pytest.raises(AssertionError, match="CUDA"):
         moe_a16w16(x, logits, w13, w2, 2)
+
+
+def test_calls_at_once_on_one_stream_have_scratch_of_their_own(monkeypatch):
+    # A call is two launches, and the entry point runs without Python's lock: while it runs, another thread's call on the same
+    # stream may come between the two. Here the second call is made from within the first one's.
+    import threading
+
+    from flydsl_examples_b200 import gemm_a16w16 as gemm, moe_a16w16 as module
+
+    shared = gemm._Workspace(torch.device("cpu"))
+    shared.ensure(_lib.COUNTER_BYTES + (1 << 20), torch.device("cpu"), None)
+    monkeypatch.setattr(module, "_workspace_for", lambda *a: shared)
+    monkeypatch.setattr(module, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: None)
+    bf, running = torch.bfloat16, []
+
+    def call(t):
+        x, logits, w13, w2 = torch.zeros(t, 64, dtype=bf), torch.zeros(t, 8), torch.zeros(8, 64, 64, dtype=bf), torch.zeros(8, 64, 32, dtype=bf)
+        need, sizes = module._call_plan(x.shape, x.stride(), x.dtype, logits.shape, logits.stride(), logits.dtype, w13.shape, w13.stride(), bf,
+                                        w2.shape, w2.stride(), bf, x.shape, bf, 2, True, ())
+        module._launch_moe(x, logits, w13, w2, torch.empty_like(x), need, sizes, 0)
+
+    def entry(args, stream):
+        a = _lib.MoeArgs.from_buffer_copy(args)
+        running.append((a.workspace, a.workspace + a.workspace_bytes))
+        if len(running) == 1:
+            other = threading.Thread(target=call, args=(5,))
+            other.start()
+            other.join()
+        return 0
+    monkeypatch.setattr(module._lib, "fast", lambda name: entry)
+    call(4)
+    spans = running + [(shared.buf.data_ptr(), shared.buf.data_ptr() + shared.buf.numel())]  # what split-K GEMMs of the stream use
+    assert len(spans) == 3
+    for i, (lo, hi) in enumerate(spans):
+        assert all(hi <= lo2 or hi2 <= lo for lo2, hi2 in spans[i + 1:])

@@ -238,3 +238,44 @@ def test_weights_past_32_bit_offsets():
     logits = torch.full((2, e), -5.0, device=DEV)
     logits[0, e - 1], logits[1, 0], logits[1, e - 1] = 4.0, 2.0, 3.0
     check(moe_a16w16(x, logits, w13, w2, 2), x, logits, w13, w2, 2)
+
+
+def test_threads_on_one_stream():
+    # torch's default stream is one for all threads: layers of different sizes and inputs from several threads, with ticket split-K
+    # GEMMs between, each thread's results as when it is alone
+    import threading
+
+    layers = [(inputs(t, e, 256, i, torch.bfloat16, seed=t), k) for t, e, i, k in ((3, 40, 264, 4), (17, 8, 512, 2), (64, 24, 64, 6), (9, 12, 1032, 3))]
+    want = [moe_a16w16(*a, k) for a, k in layers]
+    g = torch.Generator(device=DEV).manual_seed(5)
+    a = torch.randn(96, 4096, generator=g, device=DEV).to(torch.bfloat16)
+    b = torch.randn(256, 4096, generator=g, device=DEV).to(torch.bfloat16)
+    product = torch.empty(96, 256, device=DEV)
+    kw = {"tile_n": 128, "split_k": 8}
+    gemm_a16w16(a, b.t(), product, user_kwargs=kw, out_dtype=torch.float32)
+    want_product = product.clone()
+    torch.cuda.synchronize()
+    bad, go = [], threading.Barrier(len(layers) + 1)
+
+    def thread(body):
+        def work():
+            try:
+                go.wait()
+                for _ in range(200):
+                    body()
+            except Exception as e:
+                bad.append(e)
+        return threading.Thread(target=work)
+
+    got = [[] for _ in layers]
+    threads = [thread(lambda i=i: got[i].append(moe_a16w16(*layers[i][0], layers[i][1]))) for i in range(len(layers))]
+    threads.append(thread(lambda: gemm_a16w16(a, b.t(), product, user_kwargs=kw, out_dtype=torch.float32)))
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad and torch.equal(product, want_product)
+    for y, of_thread in zip(want, got):
+        assert len(of_thread) == 200 and all(torch.equal(y, v) for v in of_thread)
+    check_status()
