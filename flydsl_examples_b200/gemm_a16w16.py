@@ -389,33 +389,41 @@ def gemm_a16w16(
     assert why is None, f"unsupported gemm_a16w16 shape/config: {why}"
 
     args = _fill_args(a, b, out, bias, pol, a_t, b_t)
+    if _trace_buffer is not None:
+        args.trace = _trace_buffer.data_ptr()
+        args.trace_words = _trace_buffer.numel()
+    ent = _first_launch(args, n, device, stream)
+    # Remember the launch only when it describes the caller's own tensors (a made-contiguous bias is a temporary).
+    if key is not None and bias is bias_in and out_in is not None:
+        _remember(key, ent)
+    else:
+        _lib.load().b200_gemm_release(ent.handle)
+    return out
+
+
+def _first_launch(args: _lib.Args, n: int, device: torch.device, stream: torch.cuda.Stream) -> _Prepared:
+    """Resolve and launch a call that is not in the table. The stream's workspace is one for all threads, and a call that repacks an
+    operand is two launches: from the growing of the workspace to the last launch the lock keeps other calls out."""
     lib = _lib.load()
     ws = _workspace_for(device, stream)
     dev_index = device.index if device.index is not None else torch.cuda.current_device()
-    with torch.cuda.device(dev_index):
+    handle = C.c_void_p()
+    with _prepared_lock, torch.cuda.device(dev_index):
         need = lib.b200_gemm_workspace_bytes(C.byref(args))
         if need:
             ws.ensure(need, device, stream)
             args.workspace = ws.buf.data_ptr()
             args.workspace_bytes = ws.buf.numel()
         args.status = ws.status.data_ptr()
-        if _trace_buffer is not None:
-            args.trace = _trace_buffer.data_ptr()
-            args.trace_words = _trace_buffer.numel()
-        handle = C.c_void_p()
         rc = lib.b200_gemm_prepare(C.byref(args), C.byref(handle))
         if rc != 0:
             raise RuntimeError(f"b200_gemm_prepare failed ({rc}): {_lib.strerror(rc)}")
+        ent = _Prepared(handle, ws, dev_index, n)
         rc = lib.b200_gemm_launch(handle, C.c_void_p(stream.cuda_stream))
     if rc != 0:
         lib.b200_gemm_release(handle)
         raise RuntimeError(f"b200_gemm_launch failed ({rc}): {_lib.strerror(rc)}")
-    # Remember the launch only when it describes the caller's own tensors (a made-contiguous bias is a temporary).
-    if key is not None and bias is bias_in and out_in is not None:
-        _remember(key, _Prepared(handle, ws, dev_index, n))
-    else:
-        lib.b200_gemm_release(handle)
-    return out
+    return ent
 
 
 def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_dtype: torch.dtype, user_kwargs: dict = {},
@@ -434,7 +442,6 @@ def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_d
     key = ("ptr", a.data_ptr(), a.shape, a.stride(), a.dtype, b.data_ptr(), b.shape, b.stride(), out_ptr, out_dtype,
            kw_key, stream.cuda_stream, layout, device.index)
     lib = _lib.load()
-    dev_index = device.index if device.index is not None else torch.cuda.current_device()
     with _prepared_lock:  # held across lookup and launch, see gemm_a16w16
         ent = _prepared.get(key)
         if ent is not None and ent.ws_gen == ent.ws.generation:
@@ -454,24 +461,7 @@ def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_d
     assert why is None, f"unsupported gemm_a16w16 shape/config: {why}"
     args = _fill_args(a, b, torch.empty(0, dtype=out_dtype), None, pol, a_t, b_t)
     args.out = out_ptr
-    ws = _workspace_for(device, stream)
-    with torch.cuda.device(dev_index):
-        need = lib.b200_gemm_workspace_bytes(C.byref(args))
-        if need:
-            ws.ensure(need, device, stream)
-            args.workspace = ws.buf.data_ptr()
-            args.workspace_bytes = ws.buf.numel()
-        args.status = ws.status.data_ptr()
-        handle = C.c_void_p()
-        rc = lib.b200_gemm_prepare(C.byref(args), C.byref(handle))
-    if rc != 0:
-        raise RuntimeError(f"b200_gemm_prepare failed ({rc}): {_lib.strerror(rc)}")
-    ent = _Prepared(handle, ws, dev_index, n)
-    with torch.cuda.device(ent.dev):
-        rc = lib.b200_gemm_launch(ent.handle, C.c_void_p(stream.cuda_stream))
-    _remember(key, ent)  # only now can another thread find (and, by eviction, release) the handle
-    if rc != 0:
-        raise RuntimeError(f"b200_gemm_launch failed ({rc}): {_lib.strerror(rc)}")
+    _remember(key, _first_launch(args, n, device, stream))  # only now can another thread find (and, by eviction, release) the handle
 
 
 def plan(a: torch.Tensor, b: torch.Tensor, layout: str = "nt", user_kwargs: dict = {},
