@@ -163,6 +163,21 @@ __device__ __forceinline__ void store_packed(float* tiles, long long step, int r
   reinterpret_cast<uint8_t*>(tiles)[((block >> 2) * step + row_tile) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (block & 3)] = (uint8_t)(bits >> 23);
 }
 
+// Which of a thread's eight columns have infinities of one sign and no NaN: those sums stay infinite although v gets NaN in their place.
+template <typename T>
+__device__ __forceinline__ uint32_t infinite_columns(const RawRow<T> (&v)[8]) {
+  uint32_t up = 0, down = 0, nan = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = v[i].get(j);
+      up |= (f == INFINITY ? 1u : 0u) << j, down |= (f == -INFINITY ? 1u : 0u) << j, nan |= (f != f ? 1u : 0u) << j;
+    }
+  nan |= up & down;
+  return (up & ~nan) | (down & ~nan) << 8;
+}
+
 // MODE: 1 = groups along rows, 2 = along columns, 4 = 128 x 128 blocks (written through the row members).
 template <typename T, int MODE, bool E5M2>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantize_a8_kernel(const QuantParams p) {
@@ -218,9 +233,11 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     for (int i = 0; i < kPasses; ++i) all = M::max2(all, rmag[i]);
   }
   const bool odd = M::any_odd(all);  // an infinity or a NaN among them: it counts as zero
+  uint32_t infinite = 0;             // columns whose sum is an infinity: bit j +inf, bit 8 + j -inf
   if (odd) {
     maxima([](uint32_t m) { return M::only_finite(m); });
     if constexpr (!E5M2) {  // the conversion clamps infinities, e4m3 has none
+      if (MODE & 2) infinite = infinite_columns<T>(v);
 #pragma unroll
       for (int i = 0; i < kPasses; ++i)
 #pragma unroll
@@ -301,6 +318,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
       for (int j = 0; j < 8; ++j) {
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) csum[j] += v[i].get(j);
+        if (!E5M2 && (infinite >> j & 0x101u)) csum[j] = __uint_as_float(infinite >> j & 1u ? 0x7f800000u : 0xff800000u);
         csum[j] += __shfl_xor_sync(0xffffffffu, csum[j], 16);
       }
     }

@@ -569,3 +569,26 @@ def test_linear_of_tiny_by_huge_values():
         bound = (8 * nb + 1) * 2.0 ** -23 * mag + 2.0 ** -24 * 1.000001 * want.abs() + 2.0 ** -149
         assert ((got.double() - want).abs() <= bound).all()
     check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("grad_dtype", [E4, E5])
+def test_bias_gradient_of_infinities_and_nan(dtype, grad_dtype):
+    # the sum of the gradient as it is, whatever the 8-bit copy makes of an infinity
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator(device=DEV).manual_seed(15)
+    x = torch.randn(300, 64, generator=g, device=DEV).to(dtype)
+    w = torch.randn(140, 64, generator=g, device=DEV).to(dtype)
+    dy = torch.randint(-4, 5, (300, 140), generator=g, device=DEV).to(dtype)  # finite sums are exact
+    for i, j, v in ((3, 1, inf), (299, 2, -inf), (5, 3, inf), (250, 3, -inf), (6, 4, nan), (7, 5, inf), (7, 6, inf), (8, 6, nan), (130, 139, -inf)):
+        dy[i, j] = v
+    want = dy.double().sum(0).to(dtype)
+    for need in ((0, 0, 1), (1, 0, 1), (1, 1, 1)):  # columns alone, and with rows
+        x_, w_, b = x.clone().requires_grad_(bool(need[0])), w.clone().requires_grad_(bool(need[1])), torch.zeros(140, dtype=dtype, device=DEV, requires_grad=True)
+        linear_a8w8(x_, w_, b, grad_dtype).backward(dy)
+        assert torch.equal(b.grad.isnan(), want.isnan()) and torch.equal(b.grad[~want.isnan()], want[~want.isnan()])
+        if need[0]:  # the quantized copy has them as before
+            q, s = groups64(dy.float(), 1, 128, grad_dtype)
+            odd = ~q.float().isfinite().all(1)
+            assert odd.any() and not x_.grad[odd].isfinite().all(1).any() and x_.grad[~odd].isfinite().all()
+    check_status()
