@@ -37,7 +37,6 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   pl.swap_ab = pol.swap_ab ? 1 : 0;
   pl.tile_n = pol.tile_n;
   pl.tile_k = k8TK;
-  pl.group_m = pol.group_m < 0 ? 0 : pol.group_m;
   const int v_vector = (pl.swap_ab ? a->a_block : a->b_block) ? 0 : 1;
   if (packed && (pl.swap_ab || pol.split_k > 1)) return B200_GEMM_ERR_BAD_POLICY;
   if (!variant8(pl.tile_n, pl.cta_group, v_vector, packed, var)) return B200_GEMM_ERR_BAD_POLICY;
@@ -50,6 +49,8 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   const int64_t P = pl.swap_ab ? a->n : a->m, Q = pl.swap_ab ? a->m : a->n;
   pl.tiles_p = (int)((P + pl.tile_m - 1) / pl.tile_m);
   pl.tiles_q = (int)((Q + pl.tile_n - 1) / pl.tile_n);
+  // all tile rows are one group at most: the kernel multiplies by tiles_q in 32 bits
+  pl.group_m = pol.group_m < 0 ? 0 : pol.group_m < pl.tiles_p ? pol.group_m : pl.tiles_p;
   const int64_t tiles = (int64_t)pl.tiles_p * pl.tiles_q;
   const int kb_total = (int)((a->k + k8TK - 1) / k8TK);
   int s = 1;

@@ -213,3 +213,23 @@ def test_a_split_keeps_all_its_clusters_running_at_once(sms):
                 if pol["split_k"] > 1:
                     assert tiles <= module._clusters(pol["split_k"], sms)
                     assert pol["split_k"] <= -(-k // 128)  # no CTA without a block
+
+
+@pytest.mark.parametrize("group", [-3, 0, 1, 2, 3, 4, 1 << 20, 1 << 30, (1 << 31) - 1])
+@pytest.mark.parametrize("m,n,kw", [(700, 520, dict(tile_n=128)), (520, 700, dict(tile_n=128, swap_ab=1)), (700, 1030, dict(tile_n=256, cta_group=2)), (1, 1 << 30, dict(tile_n=16))])
+def test_a_group_of_tile_rows_is_no_larger_than_the_matrix(group, m, n, kw):
+    # the kernel multiplies the group by the tiles in a row, in 32 bits; here its walk is taken over all tiles, or the first and last
+    a = args8(m=m, n=n, ldo=n, ldb=256, **kw)
+    a.policy.group_m = group
+    pl = _lib.Plan()
+    assert _lib.load().b200_gemm_a8w8_plan_query(C.byref(a), C.byref(pl)) == 0
+    assert 0 <= pl.group_m <= pl.tiles_p and (pl.group_m > 0) == (group > 0)
+    assert pl.group_m * pl.tiles_q < 1 << 31
+    total = pl.tiles_p * pl.tiles_q
+    if pl.group_m and total < 10000:
+        seen = set()
+        for tile in range(total):
+            g, r = divmod(tile, pl.group_m * pl.tiles_q)
+            rows = min(pl.tiles_p - g * pl.group_m, pl.group_m)
+            seen.add((g * pl.group_m + r % rows, r // rows))
+        assert seen == {(p, q) for p in range(pl.tiles_p) for q in range(pl.tiles_q)}

@@ -592,3 +592,9 @@ def test_bias_gradient_of_infinities_and_nan(dtype, grad_dtype):
             odd = ~q.float().isfinite().all(1)
             assert odd.any() and not x_.grad[odd].isfinite().all(1).any() and x_.grad[~odd].isfinite().all()
     check_status()
+
+
+@pytest.mark.parametrize("kw", [{"tile_n": 128}, {"tile_n": 256, "cta_group": 2}, {"tile_n": 64, "swap_ab": True}], ids=str)
+@pytest.mark.parametrize("group", [1, 3, 1 << 30, (1 << 31) - 1])
+def test_groups_of_tile_rows(kw, group):
+    run(700, 1100, 300, kw={**kw, "group_m": group}, repeats=2)
