@@ -164,7 +164,6 @@ static int resolve(const b200_gemm_args* a, Resolved* r, bool need_sm_count, int
   pl.swap_ab = pol.swap_ab ? 1 : 0;
   pl.tile_m = kTileP * pl.cta_group;
   pl.tile_n = pol.tile_n;
-  pl.group_m = pol.group_m < 0 ? 0 : pol.group_m;
   const Variant* var = find_variant(pl.tile_n, pl.cta_group, pol.tile_k);
   if (var == nullptr) return B200_GEMM_ERR_BAD_POLICY;
   pl.tile_k = var->tile_k;
@@ -198,6 +197,8 @@ static int resolve(const b200_gemm_args* a, Resolved* r, bool need_sm_count, int
 
   pl.tiles_p = (r->P + pl.tile_m - 1) / pl.tile_m;
   pl.tiles_q = (r->Q + pl.tile_n - 1) / pl.tile_n;
+  // all tile rows are one group at most: the kernel multiplies by tiles_q in 32 bits
+  pl.group_m = pol.group_m < 0 ? 0 : pol.group_m < pl.tiles_p ? pol.group_m : pl.tiles_p;
   const int64_t tiles = (int64_t)pl.tiles_p * pl.tiles_q;
   const int kb_total = (int)((a->k + pl.tile_k - 1) / pl.tile_k);
   pl.split_k = pol.split_k <= 0 ? 1 : pol.split_k;

@@ -119,3 +119,19 @@ def test_ctypes_structures_match_the_header(tmp_path):
     want = [C.sizeof(_lib.Policy), C.sizeof(_lib.Args), C.sizeof(_lib.Plan), C.sizeof(_lib.PeerHandle),
             _lib.Policy.reserved.offset, _lib.Args.trace_words.offset, _lib.Plan.atomic_out.offset, _lib.Args.policy.offset]
     assert got == want, (got, want)
+
+
+def test_a_group_of_tile_rows_is_no_larger_than_the_matrix():
+    # the kernel multiplies the group by the tiles in a row, in 32 bits
+    lib = _lib.load()
+    for m, n, tile_n, cta_group, swap in ((700, 520, 128, 1, 0), (520, 700, 128, 1, 1), (700, 1030, 256, 2, 0), (1, 1 << 30, 16, 1, 0)):
+        for group in (-3, 0, 1, 2, 3, 4, 1 << 20, 1 << 30, (1 << 31) - 1):
+            args, pl = _lib.Args(), _lib.Plan()
+            args.m, args.n, args.k = m, n, 256
+            args.lda = args.ldb = 256
+            args.ldo = n
+            args.in_dtype = args.out_dtype = 2
+            args.b_trans = 1
+            args.policy.tile_n, args.policy.cta_group, args.policy.swap_ab, args.policy.group_m = tile_n, cta_group, swap, group
+            assert lib.b200_gemm_plan_query(C.byref(args), C.byref(pl)) == 0
+            assert 0 <= pl.group_m <= pl.tiles_p and (pl.group_m > 0) == (group > 0) and pl.group_m * pl.tiles_q < 1 << 31

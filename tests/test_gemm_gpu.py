@@ -813,3 +813,9 @@ def test_bounded_wait_runs_out_and_is_reported():
     assert int(ws.buf[:64].sum()) == 0  # the ticket region was cleared
     check_status()                      # nothing pending any more
     run_case(case, repeats=2)           # and the next split-K call on this stream is right
+
+
+@pytest.mark.parametrize("kw", [{"tile_n": 128}, {"tile_n": 256, "cta_group": 2}, {"tile_n": 64, "swap_ab": True}], ids=str)
+@pytest.mark.parametrize("group", [1, 3, 1 << 30, (1 << 31) - 1])
+def test_groups_of_tile_rows(kw, group):
+    run_case(O.Case("groups", "bf16", "nt", 700, 1100, 300, seed=31, user_kwargs={**kw, "group_m": group}))
