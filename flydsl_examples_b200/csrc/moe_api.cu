@@ -112,6 +112,8 @@ static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   u.dtype = a->dtype;
   u.list = static_cast<int*>(a->workspace);
   u.h = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a->workspace) + kMoeListBytes);
+  const bool fp16 = a->dtype == B200_GEMM_DTYPE_FP16;
+  u.value_scale = fp16 ? kMoeValueScale : 1.f, u.value_back = 1.f / u.value_scale, u.rest_back = fp16 ? 1.f / kMoeRestScale : 1.f;
   u.out = a->out, u.ldo = a->ldo;
   u.status = a->status;
   u.wait_limit_ns = a->wait_limit_us > 0 ? (unsigned long long)a->wait_limit_us * 1000ull : kWaitLimitNs;

@@ -16,7 +16,10 @@
 //  * First kernel: a tile is 64 gate rows over 64 up rows of one expert; its epilogue computes h[slot][t][i] = p * silu(gate) *
 //    up, zero for pairs that were not chosen, with the weight of the pair folded in. h is the second product's 16-bit
 //    operand; it is stored as two of them, the rounded value and the rounded remainder, which cost that product columns
-//    (2 TN instead of TN) that it has to spare. Rounded once, h would put as much error into y as y's own rounding does.
+//    (2 TN instead of TN) that it has to spare. Rounded once, h would put as much error into y as y's own rounding does. The two
+//    have accumulators of their own, so each may have a power of two of its own, undone when they are added. In fp16 the value
+//    is that of h / 16 and the remainder is kept 2^11 times as large: together they are exact to 2^-22 of h, or 2^-32 for
+//    |h| below 2^-10, up to 2^20 (with no such factors: infinite from 65520 on, and half steps of 2^-25). bf16 has fp32's range: 2^-16 of h.
 //  * Second kernel: the sum over experts is the K axis of one product, y[h, t] = sum over (slot, i) of W2 * h, accumulated
 //    in TMEM. K is cut into contiguous spans over the CTAs of a cluster, which add up through distributed shared
 //    memory in rank order: no atomics, the same bits every time.
@@ -34,6 +37,9 @@ namespace b200 {
 constexpr int kMoeThreads = 384;  // warp 0 TMA producer, warp 1 TMEM and MMA, warps 2-5 epilogue; 6-11 only help to route
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
 
+// Powers of two with which h is kept in fp16, see above.
+constexpr float kMoeValueScale = 1.f / 16, kMoeRestScale = 2048.f;
+
 struct alignas(64) MoeParams {
   CUtensorMap tmap_u;  // W13 as {H, 2I, E}, box {64, 64, 1}; or W2 as {I, H, E}, box {64, 128, 1}
   CUtensorMap tmap_v;  // x as {H, T}, box {64, TN}; or h as {I, T, 2 slots}, box {64, TN, 1}
@@ -43,6 +49,7 @@ struct alignas(64) MoeParams {
   int T, E, H, I, top_k, renorm;
   int dtype;         // 2 bf16, 3 fp16
   uint16_t* h;       // [slot][value, remainder][T][I]
+  float value_scale, value_back, rest_back;  // h's value is that of h * value_scale; the factors that undo that and kMoeRestScale in the sums
   int* list;         // [0] = number of experts that a token chose, [16..] = their indices in increasing order
   void* out;
   long long ldo;
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
           if (et < p.T)
             for (int j = 0; j < p.top_k; ++j)
               if (ids[et * kMoeMaxTopK + j] == experts[slot]) w = weights[et * kMoeMaxTopK + j];
-          pair_w[et] = w;
+          pair_w[et] = w * p.value_scale;
         }
       }
       float v[TN];
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
             if (c < TN)
               v[c + i] = __uint_as_float(r[i]);
             else
-              v[c - TN + i] += __uint_as_float(r[i]);  // the remainders' part
+              v[c - TN + i] = fmaf(__uint_as_float(r[i]), p.rest_back, v[c - TN + i]) * p.value_back;  // the remainders' part
           }
         }
         tc_fence_before();
@@ -487,7 +494,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_a16w16_sm100_kernel(const 
                 const __nv_bfloat16 h = __float2bfloat16_rn(a), l = __float2bfloat16_rn(a - __bfloat162float(h));
                 bits = __bfloat16_as_ushort(h), rest = __bfloat16_as_ushort(l);
               } else {
-                const __half h = __float2half_rn(a), l = __float2half_rn(a - __half2float(h));
+                const __half h = __float2half_rn(a), l = __float2half_rn((a - __half2float(h)) * kMoeRestScale);
                 bits = __half_as_ushort(h), rest = __half_as_ushort(l);
               }
               if ((p.dtype == 2 ? bits & 0x7f80u : bits & 0x7c00u) == (p.dtype == 2 ? 0x7f80u : 0x7c00u)) rest = 0;  // infinite or NaN

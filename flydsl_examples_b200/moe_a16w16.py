@@ -108,7 +108,7 @@ def moe_a16w16(
     w13 [E, 2 I, H] (gate rows, then up rows), w2 [E, H, I]; x, weights and `out` [T, H] are all bfloat16 or all float16. p is the
     softmax over all experts, ties go to the lowest index, and with `renormalize` the chosen weights are divided by their sum.
     Sums, softmax and SiLU are fp32; p * silu(g) * u, the second product's operand, is carried as a 16-bit value and a 16-bit
-    remainder.
+    remainder: to 2^-16 of it in bfloat16; in float16 to 2^-22 of it, or 2^-32 where it is below 2^-10, and infinite from 2^20 on.
 
     An expert of weight zero (a logit of -inf) is not evaluated, a token whose logits are all -inf gets zeros, a NaN logit
     makes its token's row NaN. Non-finite values in a chosen expert's weights reach every token of the call.

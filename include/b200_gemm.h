@@ -326,7 +326,8 @@ int b200_gemm_sequence(const void* records, void* cuda_stream);
  *   p = softmax(logits[t, :]); the top_k experts of each token, ties to the lowest index; weights divided by their sum when
  *   `renormalize`; out[t] = sum over them of p * W2[e] (silu(G) * U), [G; U] = W13[e] x[t], rounded once.
  * 16-bit x, weights and output (all `dtype`); sums, softmax and SiLU in fp32; p * silu(G) * U, the operand of the second
- * product, is carried as a value and a remainder of `dtype` (so in fp16 it has to stay below 65504). An expert whose weight is zero (a logit of -inf)
+ * product, is carried as a value and a remainder of `dtype`: to 2^-16 of it in bf16; in fp16 to 2^-22 of it, or 2^-32 where it is below
+ * 2^-10, and infinite from 2^20 on. An expert whose weight is zero (a logit of -inf)
  * is not evaluated; a token whose logits are all -inf gets zeros; a NaN logit makes its token's output NaN. Each chosen
  * expert's weights are read once for all tokens; non-finite values in them reach every token of the call.
  * Limits: 1 ... 64 tokens, up to 512 experts, top_k up to 16; hidden and inner multiples of 8; x and the weights on 16-byte

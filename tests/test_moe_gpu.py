@@ -279,3 +279,33 @@ def test_threads_on_one_stream():
     for y, of_thread in zip(want, got):
         assert len(of_thread) == 200 and all(torch.equal(y, v) for v in of_thread)
     check_status()
+
+
+# In fp16 the second product's operand h = p * silu(g) * u is a value rounded at h / 16 and a remainder kept 2^11 times as large: half a
+# step of half a step, (2^-11)^2 of h, or half of the remainder's smallest step, 2^-25 * 2^-11 * 16 = 2^-32. The error of the SiLU's
+# exponential grows with |g| only where g is negative; from -40 on h itself is below 2^-32 (40 e^-40 |u| < 2e-13 for |u| < 1000).
+@pytest.mark.parametrize("x_size,w2_size", [(1, 1), (100, 1e-3), (200, 1e-4), (0.1, 4), (0.02, 30), (0.004, 200), (0.001, 1000)])
+def test_small_and_large_activations_in_fp16(x_size, w2_size):
+    x, logits, w13, w2 = inputs(5, 3, 256, 320, torch.float16)
+    x, w2 = (x * x_size).half(), (w2.float() * w2_size).half()
+    got = moe_a16w16(x, logits, w13, w2, 2)
+    check_status()
+    y = torch.zeros(5, 256, dtype=torch.float64, device=DEV)
+    err, mag = torch.zeros_like(y), torch.zeros_like(y)
+    for t, chosen in routing(logits, 2, True).items():
+        for e, p in chosen:
+            a, b, v = w13[e].double(), w2[e].double(), x[t].double()
+            gu, s = a @ v, (a.abs() @ v.abs()) * (256 / 16 + 8) * U23
+            g, u = gu[:320], gu[320:]
+            silu = g / (1 + torch.exp(-g))
+            hv = p * silu * u
+            assert hv.abs().max() < 2 ** 20 * 0.99
+            d = p * (1.1 * u.abs() * s[:320] + (silu.abs() + 1.1 * s[:320]) * s[320:]) + hv.abs() * (32 + 2 * g.abs().clamp(max=40)) * U23
+            d = d + (hv.abs() + d) * 2.0 ** -22 + 2.0 ** -32
+            y[t] += b @ hv
+            err[t] += b.abs() @ d
+            mag[t] += b.abs() @ (hv.abs() + d)
+    err += mag * (2 * 320 / 16 + 24) * U23
+    bound = err + (y.abs() + err) * 2.0 ** -11 + 2.0 ** -25
+    assert y.abs().max() < 65504
+    assert ((got.double() - y).abs() <= bound * (1 + 1e-6)).all()
