@@ -444,11 +444,12 @@ def _at(base: int, offsets) -> tuple:
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, grad_dtype):
+    def forward(ctx, x, weight, bias, grad_dtype, grad_enabled):
         shape, (n, k) = x.shape, weight.shape
         x2, w2 = _row_major(x if x.ndim == 2 else x.reshape(-1, k)), _row_major(weight)
         m = x2.shape[0]
-        need_x, need_w = ctx.needs_input_grad[:2]
+        # needs_input_grad says what the tensors require, also where no backward pass can follow
+        need_x, need_w = ctx.needs_input_grad[:2] if grad_enabled else (False, False)
         index, device = x.get_device(), x.device
         bias_dtype = None if bias is None else bias.dtype
         plan = _forward_plan(m, n, k, x2.stride(0) if m > 1 else k, x.dtype, w2.stride(0) if n > 1 else k, weight.dtype, bias_dtype, need_x,
@@ -478,7 +479,7 @@ class _Linear8(torch.autograd.Function):
     def backward(ctx, dy):
         (keep,) = ctx.saved_tensors
         shape, m, n, k, x_dtype, w_dtype, b_dtype, g_id = ctx.meta
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g = _row_major(dy if dy.ndim == 2 else dy.reshape(m, n))  # an expanded gradient (of a sum) is spread out here
         index, device = dy.get_device(), dy.device
         plan = _backward_plan(m, n, k, g.stride(0) if m > 1 else n, g.dtype, g_id, x_dtype, w_dtype, b_dtype, need_x, need_w, need_b,
@@ -514,7 +515,7 @@ class _Linear8(torch.autograd.Function):
                     db = db[:n]
             if plan.records is not None and (need_x or need_w or need_b):
                 _run(plan.records.pack(*records, 0), stream)
-        return dx, dw, db, None
+        return dx, dw, db, None, None
 
 
 def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -524,7 +525,7 @@ def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 
     Forward: x in groups of 128 along K, the weight in 128 x 128 blocks, both e4m3. Backward: the output's gradient is quantized
     to `grad_dtype` once along N (for dx, against the weight as it was quantized) and once along the rows (for dweight, against x
-    quantized along the rows in the forward pass). The tensor cores apply the scales and sum in fp32. dbias is the sum of the
+    quantized along the rows in the forward pass, unless gradients are disabled). The tensor cores apply the scales and sum in fp32. dbias is the sum of the
     unquantized gradient in fp32, in a fixed order. Gradients have their tensor's type."""
     assert weight.ndim == 2 and x.ndim >= 1 and x.shape[-1] == weight.shape[1], f"x is {tuple(x.shape)}, weight {tuple(weight.shape)}"
     for name, t in (("x", x), ("weight", weight), ("bias", bias)):
@@ -537,4 +538,4 @@ def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if bias is not None:
         assert bias.shape == (weight.shape[0],) and bias.device == x.device
         bias = bias.contiguous()
-    return _Linear8.apply(x, weight, bias, grad_dtype)
+    return _Linear8.apply(x, weight, bias, grad_dtype, torch.is_grad_enabled())

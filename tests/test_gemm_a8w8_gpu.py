@@ -598,3 +598,25 @@ def test_bias_gradient_of_infinities_and_nan(dtype, grad_dtype):
 @pytest.mark.parametrize("group", [1, 3, 1 << 30, (1 << 31) - 1])
 def test_groups_of_tile_rows(kw, group):
     run(700, 1100, 300, kw={**kw, "group_m": group}, repeats=2)
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_linear_without_gradients_does_only_the_forward_work(monkeypatch, mode):
+    from flydsl_examples_b200 import gemm_a8w8 as module
+
+    g = torch.Generator(device=DEV).manual_seed(16)
+    x = torch.randn(70, 300, generator=g, device=DEV)
+    w, b = (torch.nn.Parameter(torch.randn(*s, generator=g, device=DEV)) for s in ((90, 300), (90,)))
+    plans = []
+    forward_plan = module._forward_plan
+    monkeypatch.setattr(module, "_forward_plan", lambda *a: plans.append(forward_plan(*a)) or plans[-1])
+    want = linear_a8w8(x, w, b)
+    assert plans[0].xc is not None and plans[0].keep_size > 0
+    with mode():
+        got = linear_a8w8(x.clone().requires_grad_(), w, b)
+    assert not got.requires_grad and torch.equal(got, want)
+    assert plans[1].xc is plans[1].wt is None and plans[1].keep_size == 0  # x by rows only, nothing kept
+    xl = x.clone().requires_grad_()  # and with them enabled again
+    linear_a8w8(xl, w, b).sum().backward()
+    assert xl.grad is not None and w.grad is not None and b.grad is not None
+    check_status()
