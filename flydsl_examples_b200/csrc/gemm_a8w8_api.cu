@@ -266,6 +266,9 @@ int b200_gemm_quantize_a8(const b200_gemm_quantize_args* a, void* cuda_stream) {
   if (row && (a->q_row == nullptr || a->s_row == nullptr || a->ldq_row < a->cols)) return B200_GEMM_ERR_BAD_ARG;
   if (col && (a->q_col == nullptr || a->s_col == nullptr || a->ldq_col < a->cols)) return B200_GEMM_ERR_BAD_ARG;
   if (a->colsum != nullptr && (!col || a->colsum_ld < a->cols)) return B200_GEMM_ERR_BAD_ARG;
+  auto off = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 4 != 0; };
+  if (!a->packed && ((row && off(a->s_row)) || (col && off(a->s_col)))) return B200_GEMM_ERR_BAD_ARG;
+  if (off(a->colsum)) return B200_GEMM_ERR_BAD_ARG;
   const int64_t tiles = ((a->rows + 127) / 128) * ((a->cols + 127) / 128);
   if (tiles > 0x7fffffffLL) return B200_GEMM_ERR_TOO_LARGE;
   b200::QuantParams p;

@@ -233,3 +233,18 @@ def test_a_group_of_tile_rows_is_no_larger_than_the_matrix(group, m, n, kw):
             rows = min(pl.tiles_p - g * pl.group_m, pl.group_m)
             seen.add((g * pl.group_m + r % rows, r // rows))
         assert seen == {(p, q) for p in range(pl.tiles_p) for q in range(pl.tiles_q)}
+
+
+def test_quantizer_refuses_scales_and_sums_off_their_alignment():
+    # fp32 stores to such addresses would fault; exponent tiles are bytes and start anywhere
+    def quant(**kw):
+        q = _lib.QuantizeArgs()
+        base = dict(x=4096, rows=4, cols=64, ldx=64, in_dtype=2, out_dtype=4, mode=3, q_row=4096, ldq_row=64, s_row=4096, sr_row=1, sr_group=4,
+                    q_col=4096, ldq_col=64, s_col=4096, sc_group=64, sc_col=1)
+        for key, v in {**base, **kw}.items():
+            setattr(q, key, v)
+        return _lib.load().b200_gemm_quantize_a8(C.byref(q), None)
+    for off in (1, 2, 3):
+        assert quant(s_row=4096 + off) == -1 and quant(s_col=4096 + off) == -1 and quant(colsum=4096 + off, colsum_ld=64) == -1
+        assert quant(colsum=4096 + off, colsum_ld=64, packed=1) == -1
+        assert quant(mode=4, s_row=4096 + off) == -1 and quant(mode=2, s_col=4096 + off) == -1
