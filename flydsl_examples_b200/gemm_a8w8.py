@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import struct
 from typing import Optional
 
@@ -446,8 +447,8 @@ class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, grad_dtype, grad_enabled):
         shape, (n, k) = x.shape, weight.shape
-        x2, w2 = _row_major(x if x.ndim == 2 else x.reshape(-1, k)), _row_major(weight)
-        m = x2.shape[0]
+        m = math.prod(shape[:-1])
+        x2, w2 = _row_major(x if x.ndim == 2 else x.reshape(m, k)), _row_major(weight)
         # needs_input_grad says what the tensors require, also where no backward pass can follow
         need_x, need_w = ctx.needs_input_grad[:2] if grad_enabled else (False, False)
         index, device = x.get_device(), x.device

@@ -620,3 +620,17 @@ def test_linear_without_gradients_does_only_the_forward_work(monkeypatch, mode):
     linear_a8w8(xl, w, b).sum().backward()
     assert xl.grad is not None and w.grad is not None and b.grad is not None
     check_status()
+
+
+@pytest.mark.parametrize("shape,n", [((2, 3, 0), 5), ((0,), 5), ((0, 3, 0), 5), ((2, 3, 0), 0), ((0, 4), 5), ((3, 4), 0)])
+def test_linear_of_empty_dimensions(shape, n):
+    k = shape[-1]
+    for bias in (True, False):
+        leaves = [torch.ones(*s, device=DEV, requires_grad=True) for s in (shape, (n, k), (n,))]
+        y = linear_a8w8(leaves[0], leaves[1], leaves[2] if bias else None)
+        assert y.shape == (*shape[:-1], n) and (k or (y == float(bias)).all())
+        y.sum().backward()
+        assert leaves[0].grad.shape == shape and leaves[1].grad.shape == (n, k) and not leaves[1].grad.any()
+        if bias:
+            assert (leaves[2].grad == y.numel() // max(n, 1)).all()
+    check_status()
