@@ -222,8 +222,9 @@ def gemm_a8w8(
     a [M, K], b [K, N]: logical shapes; `layout` says which dimension of each is contiguous ('n' row-major, 't' column-major), as
     in `gemm_a16w16`. Bases and leading strides are multiples of 16 bytes (`quantize_a8` pads its outputs).
     a_scale: float32 [M, ceil(K / 128)] or [ceil(M / 128), ceil(K / 128)]; b_scale: float32 [ceil(K / 128), N] or
-    [ceil(K / 128), ceil(N / 128)]; any strides. `out` may be any contiguous tensor of M * N elements; `out_dtype` (default:
-    out's, else bfloat16) and the bias are float32, bfloat16 or float16. Asynchronous on `stream`.
+    [ceil(K / 128), ceil(N / 128)]; any strides. The product of the two scales of a block is rounded to float32 before it meets the
+    block's sum: it should lie between 2^-126 and 2^128 (or be 0). `out` may be any contiguous tensor of M * N elements;
+    `out_dtype` (default: out's, else bfloat16) and the bias are float32, bfloat16 or float16. Asynchronous on `stream`.
 
     user_kwargs: tile_n (16, 32, 64, 128; with cta_group 2: 128, 256), cta_group, split_k (K blocks of a tile over the CTAs of a
     cluster), swap_ab, group_m, max_ctas, pdl, wait_limit_us; without tile_n the tiling is chosen by `heuristic_a8w8`."""

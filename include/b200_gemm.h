@@ -248,6 +248,8 @@ int b200_gemm_wait_selftest(int32_t* status, uint32_t limit_us, void* cuda_strea
  * 8-bit floating point with a scale for each block of 128.
  *   C[m, n] = sum over K blocks b of 128: sa[m, b] * sb[b, n] * (sum over k in b of A[m, k] * B[k, n])  (+ bias[n])
  * Products are exact and summed in fp32 on the tensor cores per block; the scaled sums are added in fp32; one rounding.
+ * sa * sb is rounded to fp32 first: where it is below 2^-126 it loses bits (or is 0), from 2^128 on it is infinite, and NaN times a
+ * block's sum of 0.
  * A scale belongs to one row of A (column of B), or to 128 of them (a_block / b_block: rows m with m / 128 equal). K need not
  * be a multiple of 128: the last block is shorter. Layouts as for b200_gemm_a16w16, so the forward product of a linear
  * layer, its input gradient and its weight gradient are all this entry point. Operand bases and leading strides are
