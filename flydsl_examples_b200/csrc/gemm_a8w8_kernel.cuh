@@ -16,11 +16,11 @@
 // 33 us; with a scale per row on both sides (two multiplications and a shared-memory read per element) 647 us.
 //
 // PACKED: where all scales are powers of two (what the quantizer makes), the tensor core applies them itself
-// (kind::mxf8f6f4, one exponent per row and 32 elements): all K blocks are summed in one accumulator, the epilogue warps only
-// drain it, and the operands' way into the SM is what is left (with plain kind::f8f6f4 and no scales at all 31.1 us where this
-// takes 31.3, 2048 x 4096 x 4096). 8192^3 403 us in any layout, 2048 x 4096 x 4096 30.1 us, 4096 x 4096 x 2048 with both operands
-// row-contiguous 31.3 us (a scale per row on both sides above: 55 us). The fp32 additions of the tensor core's own accumulation
-// are as good as those above: relative errors of 1e-8 to 6e-7 at K = 128 to 4096.
+// (kind::mxf8f6f4, one exponent per row and 32 elements): up to 32 K blocks are summed in one accumulator (k8Chunk says why no more),
+// the epilogue warps only drain it, and the operands' way into the SM is what is left (with plain kind::f8f6f4 and no scales at all
+// 31.1 us where this took 31.3, 2048 x 4096 x 4096, before its fifth ring stage). Replayed from a graph, operands in L2: 8192^3 373 -
+// 377 us in a burst in any layout, 2048 x 4096 x 4096 32.9 us, 4096 x 4096 x 2048 with both operands row-contiguous 34.5 us (a scale per
+// row on both sides above: 56 us).
 //
 // Roles (384 threads): warp 0 = TMA producer, warp 1 = TMEM owner and MMA issuer, warps 2-3 = scale loaders (PACKED: idle, the
 // producer loads the exponents), warps 4-11 = epilogue (warp w reads TMEM lanes 32 * (w % 4).. and column half (w - 4) / 4). The
@@ -40,6 +40,11 @@ constexpr int k8Threads = 384;
 constexpr int k8EpiThreads = 256;
 constexpr int k8ScaleStages = 8;
 constexpr int k8UBytes = k8TileP * k8TK;
+// PACKED: K blocks that the tensor core sums by itself. Its additions do not round to nearest, they cut off: sums of positive
+// products in one accumulator come out 1e-6 too small at K = 4096, 4.5e-5 at 65536 (values of either sign: off by 2.2e-7 and 7.6e-6). So
+// kernels for more blocks than these (LONG) add the sums over each 32 in fp32 registers. They are kernels of their own, since the mere
+// possibility costs short sums 1 to 11 % (4096 x 4096 x 512 16.5 -> 18.4 us).
+constexpr int k8Chunk = 32;
 
 struct alignas(64) Gemm8Params {
   CUtensorMap tmap_u;
@@ -69,7 +74,7 @@ struct alignas(64) Gemm8Params {
 };
 
 // VVEC: V has a scale per row; otherwise one per 128 rows, so one value serves each half of a tile's columns.
-// PACKED: scales are powers of two, in exponent tiles, and the tensor core applies them.
+// PACKED: scales are powers of two, in exponent tiles, and the tensor core applies them. LONG: of more than k8Chunk blocks.
 template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED>
 struct Smem8 {
   static constexpr int kVRows = TILE_Q / CG;
@@ -196,7 +201,7 @@ __device__ __forceinline__ bool wait_two(uint32_t bar0, uint32_t parity0, uint32
   return __all_sync(0xffffffffu, good);
 }
 
-template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED>
+template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED, bool LONG>
 __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __grid_constant__ Gemm8Params p) {
   using L = Smem8<TILE_Q, STAGES, CG, VVEC, PACKED>;
   constexpr int HC = TILE_Q / 2;               // columns per epilogue warp (the two warps of a lane quarter split the tile)
@@ -356,13 +361,14 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
       if (prank == 0) {
         int stage = 0;
         uint32_t phase = 0;
-        int g = 0;  // K blocks so far; each has an accumulator of its own (PACKED: tiles)
+        int g = 0;  // K blocks so far; each has an accumulator of its own (PACKED: tiles, LONG: chunks)
         int group = -1;  // PACKED: fours of K blocks so far
         bool ok = true;
 #pragma unroll 1
         for (int tile = tile0; ok && tile < p.num_tiles; tile += tile_step, g += PACKED) {
 #pragma unroll 1
           for (int kb = kb0; kb < p.kb_total; kb += kbstep, g += !PACKED) {
+            if (LONG && kb != 0 && kb % k8Chunk == 0) ++g;
             const int buf = g % kBufs;
             if (PACKED && (kb & 3) == 0) ++group;
             if (!wait_two(acce_bar(buf), ((g / kBufs) & 1) ^ 1u, full_bar(stage), phase, abort_s, wait_limit)) {
@@ -390,7 +396,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
 #pragma unroll
                 for (int j = 0; j < k8TK / 32; ++j)
                   umma_mxf8<CG>(d_tmem, du + uint64_t(j * p.u_kstep), dv + uint64_t(j * p.v_kstep), idesc, exps, exps + 4,
-                                kb != kb0 || j != 0 ? 1u : 0u);
+                                (LONG ? kb % k8Chunk != 0 : kb != kb0) || j != 0 ? 1u : 0u);
               }
 #pragma unroll
               for (int j = 0; j < (PACKED ? 0 : k8TK / 32); ++j)
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
               } else {
                 umma_commit(done_bar(stage));
               }
-              if (PACKED && kb + kbstep >= p.kb_total) {
+              if (PACKED && (kb + kbstep >= p.kb_total || (LONG && kb % k8Chunk == k8Chunk - 1))) {
                 if constexpr (CG == 2) {
                   umma_commit_pair(mapa_cluster(sfull_bar(buf), 0));
                   umma_commit_pair(mapa_cluster(sfull_bar(buf), 1));
@@ -487,31 +493,43 @@ __global__ void __launch_bounds__(k8Threads, 1) gemm_a8w8_sm100_kernel(const __g
       for (int i = 0; i < HC / 2; ++i) acc2[i] = 0;
       auto acc = [&](int i) { return __uint_as_float((uint32_t)(i & 1 ? acc2[i >> 1] >> 32 : acc2[i >> 1])); };
       bool ok = true, seen = false;
-      if constexpr (PACKED) {  // all K blocks are in one accumulator
-        const int buf = g % kBufs;
-        const uint32_t done = (g / kBufs) & 1;
-        ++g;
-        ok = wait_two(sfull_bar(buf), done, sfull_bar(buf), done, abort_s, wait_limit);
-        if (ok) {
-          tc_fence_after();
-          const uint32_t t_acc = tmem_base + buf * TILE_Q + half * HC + (uint32_t(quarter * 32) << 16);
+      if constexpr (PACKED) {
+        // all K blocks are in one accumulator, or (LONG) each chunk of them
+        auto take = [&]() {
+          const int buf = g % kBufs;
+          const uint32_t done = (g / kBufs) & 1;
+          ++g;
+          ok = wait_two(sfull_bar(buf), done, sfull_bar(buf), done, abort_s, wait_limit);
+          if (ok) {
+            tc_fence_after();
+            const uint32_t t_acc = tmem_base + buf * TILE_Q + half * HC + (uint32_t(quarter * 32) << 16);
 #pragma unroll
-          for (int c = 0; c < NCH; c += 2) {
-            uint32_t r[2][32];
-            tmem_ld_32x32(t_acc + c * 32, r[0]);
-            tmem_ld_32x32(t_acc + c * 32 + 32, r[1]);
-            tmem_ld_wait();
+            for (int c = 0; c < NCH; c += 2) {
+              uint32_t r[2][32];
+              tmem_ld_32x32(t_acc + c * 32, r[0]);
+              tmem_ld_32x32(t_acc + c * 32 + 32, r[1]);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) acc2[(c * 32 + i) / 2] = pack_u32x2(r[i >> 5][i & 31], r[i >> 5][(i & 31) + 1]);
+              for (int i = 0; i < 64; i += 2) {
+                const uint64_t v = pack_u32x2(r[i >> 5][i & 31], r[i >> 5][(i & 31) + 1]);
+                acc2[(c * 32 + i) / 2] = LONG ? add_f32x2(acc2[(c * 32 + i) / 2], v) : v;
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (CG == 2 && prank != 0)
+                mbar_arrive_remote(acce_bar(buf), 0);
+              else
+                mbar_arrive(acce_bar(buf));
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (CG == 2 && prank != 0)
-              mbar_arrive_remote(acce_bar(buf), 0);
-            else
-              mbar_arrive(acce_bar(buf));
-          }
+        };
+        if constexpr (!LONG) {
+          take();
+        } else {
+#pragma unroll 1
+          for (int kb = 0; ok && kb < p.kb_total; kb += k8Chunk) take();
         }
       }
 #pragma unroll 1

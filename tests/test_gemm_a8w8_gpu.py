@@ -634,3 +634,37 @@ def test_linear_of_empty_dimensions(shape, n):
         if bias:
             assert (leaves[2].grad == y.numel() // max(n, 1)).all()
     check_status()
+
+
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("k", [4096, 4100, 8200, 16384, 65536])
+def test_long_sums_do_not_drift(k, positive):
+    # The tensor core cuts its sums off instead of rounding them, so values of one sign drift by up to a unit per instruction; 32
+    # blocks of 128 at most are summed that way (8 units of 2^-23 for each block, as above), their sums in fp32: half a unit for each.
+    g = torch.Generator(device=DEV).manual_seed(k)
+    draw = torch.rand if positive else torch.randn
+    units = 8 * min(blocks(k), 32) + -(-blocks(k) // 32) / 2
+    for long in ("features", "tokens"):
+        if long == "features":
+            x, w = (draw(*s, generator=g, device=DEV) for s in ((130, k), (140, k)))
+            got = linear_a8w8(x, w)
+            (q, s), (p, t) = quantize_a8(x, "row"), quantize_a8(w, "block")
+        else:
+            x, dy = (draw(*s, generator=g, device=DEV) for s in ((k, 130), (k, 140)))
+            w = torch.zeros(140, 130, device=DEV, requires_grad=True)
+            linear_a8w8(x, w).backward(dy)
+            got = w.grad
+            (q, s), (p, t) = quantize_a8(dy, "col"), quantize_a8(x, "col")
+            q, s, p, t = q.t(), s.t(), p.t(), t.t()
+        a, b = values(q, s), values(p, t)
+        want, mag = a @ b.t(), a.abs() @ b.abs().t()
+        bound = units * 2.0 ** -23 * mag + 2.0 ** -24 * want.abs()
+        assert ((got.double() - want).abs() <= bound).all()
+    check_status()
+
+
+@pytest.mark.parametrize("tile_n", [128, 256])
+@pytest.mark.parametrize("layout", ["nt", "nn", "tn", "tt"])
+@pytest.mark.parametrize("m,n,k", [(129, 257, 4096), (129, 257, 4097), (300, 530, 8300), (2600, 2700, 4200), (40, 50, 12288)])
+def test_product_with_exponent_tiles_of_many_blocks(m, n, k, layout, tile_n):
+    run_packed(m, n, k, layout, tile_n, out_dtype=torch.float32)
