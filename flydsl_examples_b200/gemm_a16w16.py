@@ -37,6 +37,23 @@ _workspaces: dict[tuple, "_Workspace"] = {}
 _sm_count: dict[int, int] = {}
 
 
+_spare_status: dict[int, list] = {}
+
+
+def _status_block(device: torch.device) -> torch.Tensor:
+    """Zeroed words for a workspace. A stream that is first used while it is captured takes words that an earlier workspace of the device
+    brought along: allocated in the graph they would hold anything until its first replay, and each replay would clear them."""
+    if device.type != "cuda":
+        return torch.zeros(_STATUS_WORDS, dtype=torch.int32, device=device)
+    spare = _spare_status.setdefault(device.index if device.index is not None else torch.cuda.current_device(), [])
+    if not torch.cuda.is_current_stream_capturing():
+        if len(spare) < 32:
+            spare.extend(torch.zeros(64, _STATUS_WORDS, dtype=torch.int32, device=device).unbind())
+    elif not spare:
+        return torch.zeros(_STATUS_WORDS, dtype=torch.int32, device=device)
+    return spare.pop()
+
+
 class _Workspace:
     """Scratch owned by one (device, stream): split-K tickets + fp32 partial tiles + repack images, and the
     4-word status block kernels write when a bounded wait gives up. Grows on demand, never shrinks.
@@ -47,7 +64,7 @@ class _Workspace:
     def __init__(self, device: torch.device):
         self.buf = None
         self.generation = 0
-        self.status = torch.zeros(_STATUS_WORDS, dtype=torch.int32, device=device)
+        self.status = _status_block(device)
         self.status_ptr = self.status.data_ptr()
         self.status_bytes = self.status_ptr.to_bytes(8, "little")  # as the last member of an argument block
 
