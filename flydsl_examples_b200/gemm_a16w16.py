@@ -256,12 +256,23 @@ def _fill_args(a, b, out, bias, pol: _policy.Policy, a_t: bool, b_t: bool) -> _l
 
 
 class _Prepared:
-    """A resolved call kept for reuse: the C handle plus what it depends on."""
+    """A resolved call kept for reuse: the C handle plus what it depends on. `need`: bytes of the stream's workspace that it uses."""
 
-    __slots__ = ("handle", "ws", "ws_gen", "dev", "n")
+    __slots__ = ("handle", "ws", "ws_gen", "dev", "n", "need")
 
-    def __init__(self, handle, ws, dev, n):
-        self.handle, self.ws, self.ws_gen, self.dev, self.n = handle, ws, ws.generation, dev, n
+    def __init__(self, handle, ws, dev, n, need):
+        self.handle, self.ws, self.ws_gen, self.dev, self.n, self.need = handle, ws, ws.generation, dev, n, need
+
+    def usable(self, stream) -> bool:
+        """Whether it may be launched on its stream now: against a workspace that is still there, and not into a graph."""
+        return self.ws_gen == self.ws.generation and not (self.need and _capturing(stream))
+
+
+def _capturing(stream: Optional[torch.cuda.Stream]) -> bool:
+    if stream is None:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 _PREPARED_MAX = 2048
@@ -329,7 +340,7 @@ def gemm_a16w16(
         # table under the same lock, so none can be freed while a launch is reading it.
         with _prepared_lock:
             ent = _prepared.get(key)
-            hit = ent is not None and ent.ws_gen == ent.ws.generation
+            hit = ent is not None and ent.usable(stream)
             if hit:
                 if torch.cuda.current_device() == ent.dev:
                     rc = _lib.load().b200_gemm_launch(ent.handle, stream_ptr)
@@ -409,18 +420,16 @@ def gemm_a16w16(
     if _trace_buffer is not None:
         args.trace = _trace_buffer.data_ptr()
         args.trace_words = _trace_buffer.numel()
-    ent = _first_launch(args, n, device, stream)
     # Remember the launch only when it describes the caller's own tensors (a made-contiguous bias is a temporary).
-    if key is not None and bias is bias_in and out_in is not None:
-        _remember(key, ent)
-    else:
-        _lib.load().b200_gemm_release(ent.handle)
+    _first_launch(args, n, device, stream, key if bias is bias_in and out_in is not None else None)
     return out
 
 
-def _first_launch(args: _lib.Args, n: int, device: torch.device, stream: torch.cuda.Stream) -> _Prepared:
-    """Resolve and launch a call that is not in the table. The stream's workspace is one for all threads, and a call that repacks an
-    operand is two launches: from the growing of the workspace to the last launch the lock keeps other calls out."""
+def _first_launch(args: _lib.Args, n: int, device: torch.device, stream: torch.cuda.Stream, key: Optional[tuple]) -> None:
+    """Resolve and launch a call that is not in the table, and remember it under `key`. The stream's workspace is one for all threads,
+    and a call that repacks an operand is two launches: from the growing of the workspace to the last launch the lock keeps other
+    calls out. A captured call gets a workspace of its own from the graph's pool, its tickets cleared in the graph: graphs are replayed
+    in any order and at once, and the stream's buffer may have been replaced by then."""
     lib = _lib.load()
     ws = _workspace_for(device, stream)
     dev_index = device.index if device.index is not None else torch.cuda.current_device()
@@ -428,19 +437,31 @@ def _first_launch(args: _lib.Args, n: int, device: torch.device, stream: torch.c
     with _prepared_lock, torch.cuda.device(dev_index):
         need = lib.b200_gemm_workspace_bytes(C.byref(args))
         if need:
-            ws.ensure(need, device, stream)
-            args.workspace = ws.buf.data_ptr()
-            args.workspace_bytes = ws.buf.numel()
+            if _capturing(stream):
+                key = None
+                pl = _lib.Plan()
+                lib.b200_gemm_plan_query(C.byref(args), C.byref(pl))
+                with torch.cuda.stream(stream):
+                    buf = torch.empty(need, dtype=torch.uint8, device=device)
+                    if pl.partial_bytes:  # split K: a ticket for each CTA's tile
+                        buf[: 4 * pl.tiles_p * pl.tiles_q * pl.cta_group].zero_()
+            else:
+                ws.ensure(need, device, stream)
+                buf = ws.buf
+            args.workspace = buf.data_ptr()
+            args.workspace_bytes = buf.numel()
         args.status = ws.status.data_ptr()
         rc = lib.b200_gemm_prepare(C.byref(args), C.byref(handle))
         if rc != 0:
             raise RuntimeError(f"b200_gemm_prepare failed ({rc}): {_lib.strerror(rc)}")
-        ent = _Prepared(handle, ws, dev_index, n)
+        ent = _Prepared(handle, ws, dev_index, n, need)
         rc = lib.b200_gemm_launch(handle, C.c_void_p(stream.cuda_stream))
+    if rc == 0 and key is not None:
+        _remember(key, ent)  # only now can another thread find (and, by eviction, release) the handle
+        return
+    lib.b200_gemm_release(handle)
     if rc != 0:
-        lib.b200_gemm_release(handle)
         raise RuntimeError(f"b200_gemm_launch failed ({rc}): {_lib.strerror(rc)}")
-    return ent
 
 
 def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_dtype: torch.dtype, user_kwargs: dict = {},
@@ -461,7 +482,7 @@ def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_d
     lib = _lib.load()
     with _prepared_lock:  # held across lookup and launch, see gemm_a16w16
         ent = _prepared.get(key)
-        if ent is not None and ent.ws_gen == ent.ws.generation:
+        if ent is not None and ent.usable(stream):
             with torch.cuda.device(ent.dev):
                 rc = lib.b200_gemm_launch(ent.handle, C.c_void_p(stream.cuda_stream))
             if rc != 0:
@@ -478,7 +499,7 @@ def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_d
     assert why is None, f"unsupported gemm_a16w16 shape/config: {why}"
     args = _fill_args(a, b, torch.empty(0, dtype=out_dtype), None, pol, a_t, b_t)
     args.out = out_ptr
-    _remember(key, _first_launch(args, n, device, stream))  # only now can another thread find (and, by eviction, release) the handle
+    _first_launch(args, n, device, stream, key)
 
 
 def plan(a: torch.Tensor, b: torch.Tensor, layout: str = "nt", user_kwargs: dict = {},

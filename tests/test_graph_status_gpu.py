@@ -1,4 +1,4 @@
-"""The status block of a stream that is first used while it is captured: no part of the graph."""
+"""Captured calls: the status block of a stream that is first used then, and workspaces of graphs that are replayed in any order and at once."""
 import pytest
 import torch
 
@@ -43,4 +43,56 @@ def test_status_of_a_stream_first_used_in_a_capture(name):
     graph.replay()
     with pytest.raises(RuntimeError, match="gave up"):
         check_status()
+    check_status()
+
+
+def test_graphs_of_split_k_and_repacked_products():
+    g = torch.Generator(device="cuda").manual_seed(2)
+
+    def problem(m, n, k, pad, **kw):
+        a, b = (torch.randn(r, k + pad, generator=g, device="cuda").to(torch.bfloat16)[:, :k] for r in (m, n))
+        out = torch.empty(m, n, device="cuda")
+        return lambda: gemm_a16w16(a, b.t(), out, user_kwargs=kw, out_dtype=torch.float32)
+    problems = [problem(96, 320, 2048, 0, tile_n=128, split_k=8), problem(200, 264, 2048, 0, tile_n=64, split_k=4), problem(1000, 1100, 300, 1),
+                problem(33, 640, 1030, 5, tile_n=64, split_k=3), problem(300, 4000, 1000, 0, tile_n=128, stream_k=True)]
+    stream = torch.cuda.Stream()
+    outs, want = [], []
+    with torch.cuda.stream(stream):
+        for p in problems:  # resolved on the stream before it is captured
+            outs.append(p())
+            want.append(outs[-1].clone())
+    torch.cuda.synchronize()
+    dirty = torch.full((256 << 20,), 0x5A, dtype=torch.uint8, device="cuda")
+    del dirty
+    torch.cuda.empty_cache()  # what the graphs' pools get is not clear
+    graphs = []
+    for p in problems:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            p()
+    larger = problem(3000, 3000, 500, 1)  # the stream's workspace is replaced
+    with torch.cuda.stream(stream):
+        larger()
+    torch.cuda.synchronize()
+
+    def check():
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+        for o in outs:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+    check()
+    for graph in reversed(graphs):
+        graph.replay()
+    check()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    check()
+    with torch.cuda.stream(stream):
+        for p in problems:
+            p()
+    check()
     check_status()
