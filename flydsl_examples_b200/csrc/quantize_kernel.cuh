@@ -163,7 +163,8 @@ __device__ __forceinline__ void store_packed(float* tiles, long long step, int r
   reinterpret_cast<uint8_t*>(tiles)[((block >> 2) * step + row_tile) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (block & 3)] = (uint8_t)(bits >> 23);
 }
 
-// Which of a thread's eight columns have infinities of one sign and no NaN: those sums stay infinite although v gets NaN in their place.
+// Which of a thread's eight columns have infinities of one sign and no NaN (bit j +inf, bit 8 + j -inf): those sums stay infinite although v gets
+// NaN in their place.
 template <typename T>
 __device__ __forceinline__ uint32_t infinite_columns(const RawRow<T> (&v)[8]) {
   uint32_t up = 0, down = 0, nan = 0;
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
   constexpr int kPasses = 8;  // rows per thread: ty, ty + 16, ...
   __shared__ float red[8][128];
   __shared__ float red2[8][128];
+  __shared__ uint32_t infinite[MODE & 2 ? kQuantThreads : 1];  // of a thread that met an infinity or NaN (a register costs all: 1.7 %)
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5;
   const int tiles_c = (p.cols + 127) >> 7;
   const int tr = blockIdx.x / tiles_c, tc = blockIdx.x - tr * tiles_c;
@@ -233,11 +235,10 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     for (int i = 0; i < kPasses; ++i) all = M::max2(all, rmag[i]);
   }
   const bool odd = M::any_odd(all);  // an infinity or a NaN among them: it counts as zero
-  uint32_t infinite = 0;             // columns whose sum is an infinity: bit j +inf, bit 8 + j -inf
   if (odd) {
     maxima([](uint32_t m) { return M::only_finite(m); });
     if constexpr (!E5M2) {  // the conversion clamps infinities, e4m3 has none
-      if (MODE & 2) infinite = infinite_columns<T>(v);
+      if (MODE & 2) infinite[threadIdx.x] = infinite_columns<T>(v);
 #pragma unroll
       for (int i = 0; i < kPasses; ++i)
 #pragma unroll
@@ -315,12 +316,17 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
     }
     if (p.colsum != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) csum[j] += v[i].get(j);
-        if (!E5M2 && (infinite >> j & 0x101u)) csum[j] = __uint_as_float(infinite >> j & 1u ? 0x7f800000u : 0xff800000u);
-        csum[j] += __shfl_xor_sync(0xffffffffu, csum[j], 16);
+      if (!E5M2 && odd) {
+        const uint32_t bits = infinite[threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (bits >> j & 0x101u) csum[j] = __uint_as_float(bits >> j & 1u ? 0x7f800000u : 0xff800000u);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) csum[j] += __shfl_xor_sync(0xffffffffu, csum[j], 16);
     }
     if ((threadIdx.x & 16) == 0) {
 #pragma unroll
