@@ -39,8 +39,7 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   pl.tile_k = k8TK;
   const int v_vector = (pl.swap_ab ? a->a_block : a->b_block) ? 0 : 1;
   if (packed && (pl.swap_ab || pol.split_k > 1)) return B200_GEMM_ERR_BAD_POLICY;
-  const int kb_total = (int)((a->k + k8TK - 1) / k8TK);
-  if (!variant8(pl.tile_n, pl.cta_group, v_vector, packed, kb_total, var)) return B200_GEMM_ERR_BAD_POLICY;
+  if (!variant8(pl.tile_n, pl.cta_group, v_vector, packed, var)) return B200_GEMM_ERR_BAD_POLICY;
   pl.tile_m = k8TileP * pl.cta_group;
   pl.stages = var->stages;
   pl.smem_bytes = var->smem_bytes;
@@ -53,6 +52,7 @@ static int resolve8(const b200_gemm_a8w8_args* a, int sms, b200_gemm_plan* out, 
   // all tile rows are one group at most: the kernel multiplies by tiles_q in 32 bits
   pl.group_m = pol.group_m < 0 ? 0 : pol.group_m < pl.tiles_p ? pol.group_m : pl.tiles_p;
   const int64_t tiles = (int64_t)pl.tiles_p * pl.tiles_q;
+  const int kb_total = (int)((a->k + k8TK - 1) / k8TK);
   int s = 1;
   if (pol.split_k > 1) {  // the K blocks of a tile over the CTAs of a cluster: a power of two, no slice empty, a column each
     if (pl.cta_group != 1) return B200_GEMM_ERR_BAD_POLICY;

@@ -5,13 +5,13 @@
 namespace b200 {
 
 namespace {
-template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED, bool LONG = false>
+template <int TILE_Q, int STAGES, int CG, bool VVEC, bool PACKED>
 Variant8 make_one() {
   using L = Smem8<TILE_Q, STAGES, CG, VVEC, PACKED>;
   static_assert(L::kDynBytes <= 227 * 1024, "shared memory of a variant");
   Variant8 v;
   v.tile_q = TILE_Q, v.cta_group = CG, v.stages = STAGES;
-  v.fn = gemm_a8w8_sm100_kernel<TILE_Q, STAGES, CG, VVEC, PACKED, LONG>;
+  v.fn = gemm_a8w8_sm100_kernel<TILE_Q, STAGES, CG, VVEC, PACKED>;
   v.smem_bytes = L::kDynBytes;
   return v;
 }
@@ -21,11 +21,10 @@ Variant8 make(int v_vector) {
 }
 }  // namespace
 
-bool variant8(int tile_q, int cta_group, int v_vector, int packed, int kb_total, Variant8* out) {
+bool variant8(int tile_q, int cta_group, int v_vector, int packed, Variant8* out) {
   if (packed) {
-    const bool long_k = kb_total > k8Chunk;
-    if (cta_group == 1 && tile_q == 128) return *out = long_k ? make_one<128, 5, 1, false, true, true>() : make_one<128, 5, 1, false, true>(), true;
-    if (cta_group == 2 && tile_q == 256) return *out = long_k ? make_one<256, 5, 2, false, true, true>() : make_one<256, 5, 2, false, true>(), true;
+    if (cta_group == 1 && tile_q == 128) return *out = make_one<128, 5, 1, false, true>(), true;
+    if (cta_group == 2 && tile_q == 256) return *out = make_one<256, 5, 2, false, true>(), true;
     return false;
   }
   if (cta_group == 1 && tile_q == 16) return *out = make<16, 10, 1>(v_vector), true;

@@ -9,8 +9,7 @@ struct Variant8 {
   int tile_q, cta_group, stages, smem_bytes;
 };
 
-// packed: both operands' scales are exponent tiles; kb_total: K blocks. Otherwise v_vector: the operand on the MMA N axis has a scale per
-// row (otherwise per 128 rows). False: no such variant.
-bool variant8(int tile_q, int cta_group, int v_vector, int packed, int kb_total, Variant8* out);
+// packed: both operands' scales are exponent tiles. Otherwise v_vector: the operand on the MMA N axis has a scale per row (otherwise per 128 rows). False: no such variant.
+bool variant8(int tile_q, int cta_group, int v_vector, int packed, Variant8* out);
 
 }  // namespace b200
