@@ -134,6 +134,7 @@ static int prepare8(const b200_gemm_a8w8_args* a, Call8* h) {
     return B200_GEMM_ERR_BAD_ARG;
   rc = current_sms(&dev, &sms);
   if (rc) return rc;
+  ensure_context();
   rc = resolve8(a, sms, &pl, &var);
   if (rc) return rc;
 

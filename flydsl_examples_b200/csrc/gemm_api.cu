@@ -27,20 +27,20 @@ static void* driver_entry(const char* name) {
 }
 
 EncodeTiledFn get_encode_fn() {
-  typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
   static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, []() { fn = reinterpret_cast<EncodeTiledFn>(driver_entry("cuTensorMapEncodeTiled")); });
+  return fn;
+}
+
+void ensure_context() {
+  typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
   static CtxGetCurrentFn current = nullptr;
   static std::once_flag once;
-  std::call_once(once, []() {
-    fn = reinterpret_cast<EncodeTiledFn>(driver_entry("cuTensorMapEncodeTiled"));
-    current = reinterpret_cast<CtxGetCurrentFn>(driver_entry("cuCtxGetCurrent"));
-  });
-  // The driver encodes only with a context, which a thread gets with its first runtime call that needs one; where this is the
-  // thread's first, its device's is made current.
+  std::call_once(once, []() { current = reinterpret_cast<CtxGetCurrentFn>(driver_entry("cuCtxGetCurrent")); });
   CUcontext ctx = nullptr;
   int dev = 0;
   if (current != nullptr && current(&ctx) == CUDA_SUCCESS && ctx == nullptr && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
-  return fn;
 }
 
 typedef CUresult (*GetAddressRangeFn)(CUdeviceptr*, size_t*, CUdeviceptr);
@@ -397,6 +397,7 @@ static int prepare(const b200_gemm_args* a, b200_gemm_handle* h) {
   int dev_id = 0;
   int rc = current_device_info(&dev, &dev_id);
   if (rc) return rc;
+  ensure_context();
   Resolved r;
   rc = resolve(a, &r, true, dev->sm_count);
   if (rc) return rc;

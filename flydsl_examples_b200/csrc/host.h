@@ -12,8 +12,12 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// cuTensorMapEncodeTiled, looked up once; null when the driver does not have it. Gives the calling thread a context if it has none.
+// cuTensorMapEncodeTiled, looked up once; null when the driver does not have it.
 EncodeTiledFn get_encode_fn();
+
+// The driver encodes only with a context, which a thread gets with its first runtime call that needs one; where a call of this
+// library is the thread's first, its device's is made current. Called once before a call's tensor maps are encoded.
+void ensure_context();
 
 // Keeps the error's text for b200_gemm_strerror and returns B200_GEMM_ERR_LAUNCH.
 int set_cuda_error(cudaError_t e);

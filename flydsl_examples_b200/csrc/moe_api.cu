@@ -102,6 +102,7 @@ static int moe_prepare(const b200_gemm_moe_args* a, MoeCall* h) {
   int dev = 0, sms = 0;
   rc = current_sms(&dev, &sms);
   if (rc) return rc;
+  ensure_context();
 
   memset(h, 0, sizeof(*h));
   h->var = moe_variant(a->tokens);
