@@ -18,8 +18,8 @@
 // PACKED: where all scales are powers of two (what the quantizer makes), the tensor core applies them itself
 // (kind::mxf8f6f4, one exponent per row and 32 elements): up to 32 K blocks are summed in one accumulator (k8Chunk says why no more),
 // the epilogue warps only drain it, and the operands' way into the SM is what is left (with plain kind::f8f6f4 and no scales at all
-// 31.1 us where this took 31.3, 2048 x 4096 x 4096, before its fifth ring stage). Replayed from a graph, operands in L2: 8192^3 373 -
-// 377 us in a burst in any layout, 2048 x 4096 x 4096 32.9 us, 4096 x 4096 x 2048 with both operands row-contiguous 34.5 us (a scale per
+// 31.1 us where this took 31.3, 2048 x 4096 x 4096, before its fifth ring stage). Replayed from a graph, operands in L2: 8192^3 374 -
+// 382 us in a burst in any layout, 2048 x 4096 x 4096 32.8 us, 4096 x 4096 x 2048 with both operands row-contiguous 34.4 us (a scale per
 // row on both sides above: 56 us).
 //
 // Roles (384 threads): warp 0 = TMA producer, warp 1 = TMEM owner and MMA issuer, warps 2-3 = scale loaders (PACKED: idle, the
@@ -84,7 +84,7 @@ struct Smem8 {
   static constexpr int kOutOff = STAGES * kStageBytes;
   // swizzled 32 x 128-byte images of the epilogue warps on their way out: two each where a warp has two or more segments to
   // send (2 % on 256 columns; the fifth ring stage that they displace gained nothing), else one. PACKED has the fifth stage:
-  // 2048 x 4096 x 4096 30.1 instead of 31.3 us (a short K pays: 4096 x 4096 x 512 15.8 instead of 14.5)
+  // 2048 x 4096 x 4096 4 % faster when it was chosen (a short K pays: 4096 x 4096 x 512 15.8 instead of 14.5 us)
   static constexpr int kImages = TILE_Q >= 256 && !PACKED ? 2 : 1;
   static constexpr int kStagingBytes = TILE_Q >= 64 ? 8 * kImages * 4096 : 0;
   static constexpr int kRecvBytes = CG == 1 && !PACKED ? k8TileP * TILE_Q * 4 : 0;   // cluster split: [source][own column][128] fp32

@@ -23,9 +23,10 @@
 //  * Second kernel: the sum over experts is the K axis of one product, y[h, t] = sum over (slot, i) of W2 * h, accumulated
 //    in TMEM. K is cut into contiguous spans over the CTAs of a cluster, which add up through distributed shared
 //    memory in rank order: no atomics, the same bits every time.
-// Both keep about 190 KB of TMA loads in flight per SM. 32 tokens, 8 of 32 experts, H 7168, I 2048 (2.8 GB): 422 - 440 us, the copy
-// rate; 8 tokens, 2 of 16, 4096, 3584: 153 - 168 us, 95 %; one token, 8 of 128, 2048, 768 (75 MB): 24.4 us, 47 %, bound by the
-// latencies of two dependent kernels.
+// Both keep about 190 KB of TMA loads in flight per SM. 32 tokens, 8 of 32 experts, H 7168, I 2048 (2.8 GB): 431 - 452 us, 95 to
+// 100 % of the copy rate; 8 tokens, 2 of 16, 4096, 3584: 143 - 169 us by the experts chosen, 93 to 98 %; 64 tokens, 8 of 32, 4096, 2048 (1.6
+// GB): 287 - 290 us, 85 % (each weight tile comes with h for all tokens, as many bytes again); one token, 8 of 128, 2048, 768 (75 MB): 24.6
+// us, 47 %, bound by the latencies of two dependent kernels.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -275,7 +275,6 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Make `bar` (this CTA's smem) complete once all MMAs issued so far by this thread are done.
 // The same with a scale 2^(e - 127) per row of A and of B for the 32 K elements; the exponents are bytes in TMEM (row r: lane
 // r % 32, column r / 32, the byte that the instruction descriptor names).
 template <int kCtaGroup>
@@ -305,6 +304,7 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) 
   else
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
+// Make `bar` (this CTA's smem) complete once all MMAs issued so far by this thread are done.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }

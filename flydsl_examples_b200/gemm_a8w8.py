@@ -351,7 +351,7 @@ def quantize_a8(x: torch.Tensor, group: str = "row", dtype: torch.dtype = torch.
 
 
 # ------------------------------------------------------------------------------------------------------ linear layer
-# A step of the layer is eight launches, and a launch through the public calls costs the host more than the GPU needs for it at
+# A step of the layer is six launches, seven with a bias, and a launch through the public calls costs the host more than the GPU needs for it at
 # ordinary sizes. The layer checks its tensors once, keeps each pass's operands in one buffer, and works out sizes,
 # offsets and argument blocks once per combination of sizes and types (`_forward_plan`, `_backward_plan`).
 class _Pieces:
