@@ -263,14 +263,17 @@ class _Prepared:
     def __init__(self, handle, ws, dev, n, need):
         self.handle, self.ws, self.ws_gen, self.dev, self.n, self.need = handle, ws, ws.generation, dev, n, need
 
-    def usable(self, stream) -> bool:
+    def usable(self, stream, device) -> bool:
         """Whether it may be launched on its stream now: against a workspace that is still there, and not into a graph."""
-        return self.ws_gen == self.ws.generation and not (self.need and _capturing(stream))
+        return self.ws_gen == self.ws.generation and not (self.need and _capturing(stream, device))
 
 
-def _capturing(stream: Optional[torch.cuda.Stream]) -> bool:
+def _capturing(stream: Optional[torch.cuda.Stream], device: torch.device) -> bool:
+    """Whether the stream (None: the device's current one) is being captured."""
     if stream is None:
-        return torch.cuda.is_current_stream_capturing()
+        if device.index == torch.cuda.current_device():
+            return torch.cuda.is_current_stream_capturing()
+        stream = torch.cuda.current_stream(device)
     with torch.cuda.stream(stream):
         return torch.cuda.is_current_stream_capturing()
 
@@ -340,7 +343,7 @@ def gemm_a16w16(
         # table under the same lock, so none can be freed while a launch is reading it.
         with _prepared_lock:
             ent = _prepared.get(key)
-            hit = ent is not None and ent.usable(stream)
+            hit = ent is not None and ent.usable(stream, a.device)
             if hit:
                 if torch.cuda.current_device() == ent.dev:
                     rc = _lib.load().b200_gemm_launch(ent.handle, stream_ptr)
@@ -437,7 +440,7 @@ def _first_launch(args: _lib.Args, n: int, device: torch.device, stream: torch.c
     with _prepared_lock, torch.cuda.device(dev_index):
         need = lib.b200_gemm_workspace_bytes(C.byref(args))
         if need:
-            if _capturing(stream):
+            if _capturing(stream, device):
                 key = None
                 pl = _lib.Plan()
                 lib.b200_gemm_plan_query(C.byref(args), C.byref(pl))
@@ -482,7 +485,7 @@ def gemm_a16w16_to_pointer(a: torch.Tensor, b: torch.Tensor, out_ptr: int, out_d
     lib = _lib.load()
     with _prepared_lock:  # held across lookup and launch, see gemm_a16w16
         ent = _prepared.get(key)
-        if ent is not None and ent.usable(stream):
+        if ent is not None and ent.usable(stream, device):
             with torch.cuda.device(ent.dev):
                 rc = lib.b200_gemm_launch(ent.handle, C.c_void_p(stream.cuda_stream))
             if rc != 0:

@@ -351,9 +351,9 @@ def quantize_a8(x: torch.Tensor, group: str = "row", dtype: torch.dtype = torch.
 
 
 # ------------------------------------------------------------------------------------------------------ linear layer
-# A step of the layer is six launches, seven with a bias, and a launch through the public calls costs the host more than the GPU needs for it at
-# ordinary sizes. The layer checks its tensors once, keeps each pass's operands in one buffer, and works out sizes,
-# offsets and argument blocks once per combination of sizes and types (`_forward_plan`, `_backward_plan`).
+# A step of the layer is six launches, seven with a bias, and a launch through the public calls costs the host more than the
+# GPU needs for it at ordinary sizes. The layer checks its tensors once, keeps each pass's operands in one buffer, and works out
+# sizes, offsets and argument blocks once per combination of sizes and types (`_forward_plan`, `_backward_plan`).
 class _Pieces:
     """Offsets of the pieces of one allocation, each on a 256-byte boundary."""
 
@@ -527,8 +527,9 @@ def linear_a8w8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 
     Forward: x in groups of 128 along K, the weight in 128 x 128 blocks, both e4m3. Backward: the output's gradient is quantized
     to `grad_dtype` once along N (for dx, against the weight as it was quantized) and once along the rows (for dweight, against x
-    quantized along the rows in the forward pass, unless gradients are disabled). The tensor cores apply the scales and sum in fp32. dbias is the sum of the
-    unquantized gradient in fp32, in a fixed order. Gradients have their tensor's type."""
+    quantized along the rows in the forward pass, unless gradients are disabled). The tensor cores apply the scales and sum
+    32 groups, whose sums are added in fp32. dbias is the sum of the unquantized gradient in fp32, in a fixed order.
+    Gradients have their tensor's type."""
     assert weight.ndim == 2 and x.ndim >= 1 and x.shape[-1] == weight.shape[1], f"x is {tuple(x.shape)}, weight {tuple(weight.shape)}"
     for name, t in (("x", x), ("weight", weight), ("bias", bias)):
         if t is not None and t.dtype not in _F_ID:
