@@ -42,8 +42,8 @@ constexpr int k8ScaleStages = 8;
 constexpr int k8UBytes = k8TileP * k8TK;
 // PACKED: K blocks that the tensor core sums by itself. Its additions do not round to nearest, they cut off: sums of positive
 // products in one accumulator come out 1e-6 too small at K = 4096, 4.5e-5 at 65536 (values of either sign: off by 2.2e-7 and 7.6e-6). So
-// the sums over each 32 blocks are added in fp32 registers. That costs 1024 x 1024 x 65536 5 % and, for the addition
-// to nothing that short sums have, 4096 x 4096 x 512 4 %, else 1 % at most. (Kernels without it for up to 32 blocks: a linear layer's step
+// the sums over each 32 blocks are added in fp32 registers. That costs small products of long sums 4 to 5 % (1024 x 1024 x 65536, 256 x
+// 2048 x 16384) and, for the addition to nothing that short sums have, 4096 x 4096 x 512 4 %, else 1 % at most. (Kernels without it for up to 32 blocks: a linear layer's step
 // that uses both kinds takes 4 to 8 us more, 1000 x 3000 x 4100 118 instead of 110.)
 constexpr int k8Chunk = 32;
 
